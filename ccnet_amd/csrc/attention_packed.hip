@@ -1,0 +1,749 @@
+// Causal attention over packed prompts (sequences of different lengths end to end in one [rows][channels] matrix), grouped
+// heads, head dim 64 or 128, forward and backward, bf16 MFMA with fp32 accumulation and statistics.
+//
+//   S = scale * q k^T (key <= query, same sequence),  P = softmax(S),  O = P V,  lse = log2 sum_keys 2^(S log2 e)
+//   backward, from lse and delta = rowsum(dO o O):  P = 2^(S log2 e - lse),  dS = P o (dO V^T - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO, the last two summed over the query heads of a key head.
+//
+// Work is cut into (sequence, 128- or 256-row tile, head); which tile a workgroup takes follows from the offsets in device memory
+// (find_tile), so the host needs neither the lengths nor a copy of them, and a captured graph serves other lengths.  The longest
+// walks come first.  Rows are addressed relative to their sequence, so the diagonal always falls on aligned 32x32 blocks:
+// blocks above it are skipped, blocks on it masked, all others run without a mask.  Rows past a sequence's end are cut off by
+// the bounds of the buffer descriptor (read as zero), never by a branch.
+//
+// Layout of the products (v_mfma_f32_32x32x16_bf16): the forward and dQ kernels keep the QUERY on the lane (S^T = K Q^T, then
+// O^T += V^T P^T), the dK / dV kernel the KEY (S = Q K^T, then dV^T += dO^T P): an exponentiated accumulator block, rounded to
+// bf16, is then the B operand of the next product as it stands (k order 16 s + 8 (j >> 2) + 4 hh + (j & 3) for element j of
+// lane half hh), with the A operand brought in that order by ds_read_b64_tr_b16.  One LDS image serves row reads and transposed
+// reads: 16-byte chunk c of row r lies at chunk c ^ swz(r), swz spreading 8 consecutive rows' 64-byte spans as well as 16
+// consecutive rows' single chunks evenly over the 64 banks.
+#include "common.h"
+#include <type_traits>
+
+namespace {
+
+constexpr int PA_THREADS = 256;
+constexpr int PA_TILE = 64;  // rows of a staged tile
+
+struct PackedArgs {
+    const __bf16 *Q, *K, *V, *O, *dO;
+    __bf16 *out, *dQ, *dK, *dV;
+    long long ldq, ldk, ldv, ldo, lddo, lddq, lddk, lddv;
+    const int* cu;
+    int n_seq, rows, H, Hkv;
+    float scale, scale_log2e;
+    int zero_tail;  // rows behind the last sequence: 1 = written as zeros, 0 = left as they are
+    float* lse;     // [H][rows]
+    float* delta;   // [H][rows]
+};
+
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+    if constexpr (D == 64) {
+        const int x = (r >> 1) & 7;
+        return ((x & 1) << 2) | (x & 2) | (x >> 2);
+    } else {
+        return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+}
+
+__device__ __forceinline__ s16x4 lds_read_tr16(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+__device__ __forceinline__ bf16x8 tr_pair(const char* lo_p, const char* hi_p) {
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    const s16x4 lo = lds_read_tr16(lo_p), hi = lds_read_tr16(hi_p);
+    return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+}
+
+// 1 KiB of global memory straight to LDS (lane l lands at lds + 16 l).  Written as assembly without a register result: the
+// compiler then keeps its own counts for the reads of other stages instead of draining these loads in front of each; the
+// kernels wait for them themselves (dma_wait) before the barrier behind which a stage is read.
+__device__ __forceinline__ void dma16(const u32x4& rsrc, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+__device__ __forceinline__ void dma4(const u32x4& rsrc, unsigned lds, unsigned voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+// every load of this wave has landed and every LDS read of it has returned, then the workgroup's barrier
+__device__ __forceinline__ void stage_fence() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ unsigned lds_addr(const char* p) {
+    return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p;
+}
+// buffer descriptor over `rows` (<= 64) rows of `width` bytes, `ld` bytes apart: an access behind the last row reads zero
+__device__ __forceinline__ u32x4 row_rsrc(const char* base, int rows, long long ld, int width) {
+    const unsigned long long p = (unsigned long long)base;
+    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)p), (unsigned)__builtin_amdgcn_readfirstlane((int)((p >> 32) & 0xffffu)),
+                 (unsigned)__builtin_amdgcn_readfirstlane(rows > 0 ? (int)((rows - 1) * ld + width) : 0), 0x00020000u};
+}
+
+struct Tile { int start, len, tile, ntiles; bool tail; };
+
+__device__ __forceinline__ int wave_isum(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Tile `idx` of the tiles of `step` rows that the sequences have together, ordered by level: first every sequence's tile with
+// the highest level, where a tile's level is its index counted from the end that is walked least.  Tiles of level >= L:
+// f(L) = sum_i max(0, ntiles_i - L), falling in L, so a bisection finds the level and a ballot the sequence.  Sequence n_seq
+// stands for the rows behind the last one (when they are to be written).  Offsets are clamped to [0, rows] and to rising
+// order: wrong ones give wrong results but no access outside.  False: there is no such tile.
+__device__ bool find_tile(const PackedArgs& a, int idx, int step, bool from_end, Tile& t) {
+    const int lane = threadIdx.x & 63, n = a.n_seq + 1;
+    auto span = [&](int i, int& s) {
+        if (i >= n) { s = 0; return 0; }
+        s = min(max(a.cu[i], 0), a.rows);
+        const int e = i < a.n_seq ? min(max(a.cu[i + 1], s), a.rows) : (a.zero_tail ? a.rows : s);
+        return e - s;
+    };
+    int s0;
+    const int nt0 = (span(lane, s0) + step - 1) / step;  // the first 64 sequences stay in registers
+    auto total = [&](int L) {
+        int v = max(0, nt0 - L);
+        for (int i = lane + 64; i < n; i += 64) {
+            int s;
+            v += max(0, (span(i, s) + step - 1) / step - L);
+        }
+        return wave_isum(v);
+    };
+    if (total(0) <= idx) return false;
+    int lo = 0, hi = (a.rows + step - 1) / step;  // f(lo) > idx >= f(hi) = 0
+    {
+        int m = nt0;
+        for (int i = lane + 64; i < n; i += 64) {
+            int s;
+            m = max(m, (span(i, s) + step - 1) / step);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
+        hi = __builtin_amdgcn_readfirstlane(m);
+    }
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (total(mid) > idx) lo = mid;
+        else hi = mid;
+    }
+    int rank = idx - total(lo + 1);
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        int s = s0, len = 0;
+        len = span(i0 + lane, s);
+        const int nt = (len + step - 1) / step;
+        const unsigned long long has = __ballot(nt > lo);
+        const int c = __popcll(has);
+        if (rank < c) {
+            const int mine = __popcll(has & ((1ull << lane) - 1));
+            const unsigned long long pick = __ballot(nt > lo && mine == rank);
+            const int src = __ffsll((unsigned long long)pick) - 1;
+            t.start = __builtin_amdgcn_readlane(s, src);
+            t.len = __builtin_amdgcn_readlane(len, src);
+            t.ntiles = __builtin_amdgcn_readlane(nt, src);
+            t.tile = from_end ? t.ntiles - 1 - lo : lo;
+            t.tail = i0 + src == a.n_seq;
+            return true;
+        }
+        rank -= c;
+    }
+    return false;
+}
+
+// Consecutive workgroups go to the 8 XCDs in turn: with at least 8 key heads, workgroup slot s of a tile takes key head s mod 8
+// (+ 8 ...), so that an XCD's L2 sees the keys and values of its own heads only, all their query heads in turn.
+__device__ __forceinline__ int head_of_slot(int s, int H, int Hkv) {
+    if (Hkv & 7) return s;
+    const int G = H / Hkv, i = s >> 3;
+    return ((s & 7) + 8 * (i / G)) * G + i % G;
+}
+
+// A value that is not finite must reach only the queries that see its key, but 0 * inf in the product is no zero.  On the
+// diagonal block such values are taken out of the operand (finite_part) and, after the walk, put in by hand (add_nonfinite): a
+// query gets an infinity or a NaN in a channel from the first key on that holds one there.
+__device__ __forceinline__ u32x4 finite_part(const u32x4& f, bool& bad) {
+    u32x4 r;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        unsigned v = f[w];
+        if ((f[w] & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+        if ((f[w] & 0x7f800000u) == 0x7f800000u) v &= 0xffffu;
+        bad |= v != f[w];
+        r[w] = v;
+    }
+    return r;
+}
+// o: block of 32 channels x 32 queries (query l31 on the lane); v: the value of channel l31 at the block's first key
+__device__ __forceinline__ void add_nonfinite(f32x16& o, const __bf16* v, long long ldv, int keys, int l31, int hh) {
+    int pos = 32, neg = 32, nan = 32;
+    for (int k = keys - 1; k >= 0; --k) {
+        const unsigned b = *(const unsigned short*)(v + k * ldv);
+        if ((b & 0x7f80u) != 0x7f80u) continue;
+        if (b & 0x7fu) nan = k;
+        else if (b >> 15) neg = k;
+        else pos = k;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int c = (e & 3) + 8 * (e >> 2) + 4 * hh;
+        if (__shfl(pos, c) <= l31) o[e] += INFINITY;
+        if (__shfl(neg, c) <= l31) o[e] -= INFINITY;
+        if (__shfl(nan, c) <= l31) o[e] += NAN;
+    }
+}
+
+// lane addresses of the two transposed 8-byte reads (rows 4 hh + tq and + 8) that fill the A operand of 32-channel block d
+template <int D>
+__device__ __forceinline__ void tr_lane(int lane, int d, int& lo, int& hi) {
+    const int hh = lane >> 5, g16 = (lane >> 4) & 1, tq = (lane & 15) >> 2, tp = lane & 3;
+    const int chunk = d * 4 + g16 * 2 + (tp >> 1), r = 4 * hh + tq;
+    lo = r * D * 2 + ((chunk ^ swz<D>(r)) << 4) + (tp & 1) * 8;
+    hi = (r + 8) * D * 2 + ((chunk ^ swz<D>(r + 8)) << 4) + (tp & 1) * 8;
+}
+
+// the DMA pieces of a 64-row tile that a wave brings: piece p holds 1024 / (2 D) rows, lane l of it chunk position l mod (D / 8)
+template <int D>
+struct TileDma {
+    static constexpr int ROWB = 2 * D, CH = D / 8, BYTES = PA_TILE * ROWB, PIECES = BYTES / 1024 / 4;
+    unsigned voff[PIECES];
+    int wave;
+    __device__ __forceinline__ void init(int wave_, int lane, long long ldb) {
+        wave = wave_;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = (wave * PIECES + i) * (1024 / ROWB) + lane / CH, c = (lane % CH) ^ swz<D>(r);
+            voff[i] = (unsigned)(r * (int)ldb + c * 16);
+        }
+    }
+    __device__ __forceinline__ void issue(const u32x4& rsrc, unsigned lds) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) dma16(rsrc, lds + (wave * PIECES + i) * 1024, voff[i]);
+    }
+};
+
+// a lane's row of `D` values as B-operand fragments (lane: row, half hh: channels 16 ks + 8 hh .. + 7); zeros where !ok
+template <int D>
+__device__ __forceinline__ void load_frags(bf16x8* f, const __bf16* row, int hh, bool ok) {
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (ok) v = *(const u32x4*)(row + ks * 16 + hh * 8);
+        f[ks] = __builtin_bit_cast(bf16x8, v);
+    }
+}
+
+// Values that the compiler has loaded from memory are in their registers from here on: without this it would wait for them at
+// their first use, inside the walk, on every round, and drain the tile in flight with them.
+template <int N>
+__device__ __forceinline__ void settle(bf16x8 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
+// a lane's row of an accumulator (register e of block d: channel 32 d + (e & 3) + 8 (e >> 2) + 4 hh) as 16-byte stores: the
+// swap of packed quads between the lane halves leaves 8 consecutive channels in each
+template <int D>
+__device__ __forceinline__ void store_row(__bf16* row, const f32x16* o, float mul, int hh, bool ok) {
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int qp = 0; qp < 2; ++qp) {
+            u32x4 v;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const unsigned e0 = pack_bf16x2(o[d][8 * qp + 2 * w] * mul, o[d][8 * qp + 2 * w + 1] * mul);
+                const unsigned e1 = pack_bf16x2(o[d][8 * qp + 4 + 2 * w] * mul, o[d][8 * qp + 4 + 2 * w + 1] * mul);
+                const auto sw = __builtin_amdgcn_permlane32_swap(e0, e1, false, false);
+                v[w] = sw[0];
+                v[2 + w] = sw[1];
+            }
+            if (ok) *(u32x4*)(row + d * 32 + 16 * qp + 8 * hh) = v;
+        }
+}
+
+__device__ __forceinline__ float half_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ------------------------------------------------------------------ forward
+// A wave owns QB blocks of 32 queries; the workgroup's four waves walk the keys in tiles of 64 through a double-buffered stage.
+template <int D, int QB>
+__global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedArgs a) {
+    constexpr int BM = 128 * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TILEB];  // per stage: K, V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hh = lane >> 5;
+    Tile tl;
+    if (!find_tile(a, blockIdx.x / a.H, BM, false, tl)) return;
+    const int h = head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), kvh = h / (a.H / a.Hkv);
+    const int q0 = tl.tile * BM + wave * 32 * QB;  // in the sequence
+
+    f32x16 o[QB][ND];
+    float m_run[QB], l_run[QB];
+#pragma unroll
+    for (int X = 0; X < QB; ++X) {
+        m_run[X] = -INFINITY;
+        l_run[X] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[X][d][e] = 0.f;
+    }
+    if (!tl.tail) {
+        bf16x8 qf[QB][NK];
+#pragma unroll
+        for (int X = 0; X < QB; ++X) {
+            const int q = q0 + 32 * X + l31;
+            load_frags<D>(qf[X], a.Q + (long long)(tl.start + min(q, tl.len - 1)) * a.ldq + h * D, hh, q < tl.len);
+        }
+        const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
+        const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
+        const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
+        TileDma<D> kd, vd;
+        kd.init(wave, lane, ldkb);
+        vd.init(wave, lane, ldvb);
+        const unsigned lds0 = lds_addr(smem);
+        auto issue = [&](int t) {
+            const int left = tl.len - t * PA_TILE;
+            const unsigned st = lds0 + (t & 1) * 2 * TILEB;
+            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, min(left, PA_TILE), ldkb, ROWB), st);
+            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, min(left, PA_TILE), ldvb, ROWB), st + TILEB);
+        };
+        int kread[NK], vlo[ND], vhi[ND];
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) kread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, vlo[d], vhi[d]);
+
+        bool bad = false;  // a value on this wave's diagonal that is not finite
+        // keys that the workgroup sees: up to its last query
+        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
+        // one 64-key tile: NB blocks of 32 keys of it are seen by some query of the wave; DIAG: block 32 X' on the diagonal
+        auto body = [&](int t, auto nb_c, auto diag_c) {
+            constexpr int NB = decltype(nb_c)::value;
+            constexpr bool DIAG = decltype(diag_c)::value;
+            const char* kb = smem + (t & 1) * 2 * TILEB;
+            const char* vb = kb + TILEB;
+            // block kbk against query block X: above the diagonal (skipped) or on it, where DIAG
+            auto hidden = [](int kbk, int X) { return DIAG && (QB == 1 ? false : kbk > X); };
+            auto ondiag = [](int kbk, int X) { return DIAG && (QB == 1 ? kbk == NB - 1 : kbk == X); };
+            f32x16 s[QB][NB];
+#pragma unroll
+            for (int kbk = 0; kbk < NB; ++kbk) {
+#pragma unroll
+                for (int X = 0; X < QB; ++X)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[X][kbk][e] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    const bf16x8 kf = *(const bf16x8*)(kb + kbk * 32 * ROWB + kread[ks]);
+#pragma unroll
+                    for (int X = 0; X < QB; ++X)
+                        if (!hidden(kbk, X)) s[X][kbk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[X][ks], s[X][kbk], 0, 0, 0);
+                }
+#pragma unroll
+                for (int X = 0; X < QB; ++X)
+                    if (ondiag(kbk, X)) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if ((e & 3) + 8 * (e >> 2) + 4 * hh > l31) s[X][kbk][e] = -INFINITY;
+                    }
+            }
+            // running maximum in the scaled log2 domain; kept while no row of the wave outgrows it by more than 2^6, so that the
+            // rescaling of O and l is rare (P <= 64 stays exact in fp32, and its rounding to bf16 is relative)
+            float mx[QB];
+            bool grew = false;
+#pragma unroll
+            for (int X = 0; X < QB; ++X) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int kbk = 0; kbk < NB; ++kbk)
+                    if (!hidden(kbk, X)) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) m = fmaxf(m, s[X][kbk][e]);
+                    }
+                mx[X] = half_max(m) * a.scale_log2e;
+                grew |= !(mx[X] - m_run[X] <= 6.0f);
+            }
+            if (__any(grew)) {
+#pragma unroll
+                for (int X = 0; X < QB; ++X) {
+                    const float m_new = fmaxf(m_run[X], mx[X]);
+                    // a row that has seen only -inf scores keeps -inf as its maximum; its l stays 0 and its result 0 / 0
+                    const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[X] - m_new);
+                    m_run[X] = m_new;
+                    l_run[X] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[X][d][e] *= alpha;
+                }
+            }
+            u32x4 pf[QB][NB][2];
+#pragma unroll
+            for (int X = 0; X < QB; ++X) {
+                const float m = m_run[X] == -INFINITY ? 0.f : m_run[X];
+#pragma unroll
+                for (int kbk = 0; kbk < NB; ++kbk)
+                    if (!hidden(kbk, X)) {
+#pragma unroll
+                        for (int sI = 0; sI < 2; ++sI) {
+                            float p[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[X][kbk][8 * sI + j], a.scale_log2e, -m));
+                            l_run[X] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                            pf[X][kbk][sI] = pack8(p);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int kbk = 0; kbk < NB; ++kbk) {
+                u32x4 vf[ND][2];
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int sI = 0; sI < 2; ++sI)
+                        vf[d][sI] = __builtin_bit_cast(u32x4, tr_pair(vb + (kbk * 32 + sI * 16) * ROWB + vlo[d], vb + (kbk * 32 + sI * 16) * ROWB + vhi[d]));
+                auto pv = [&](int X) {
+#pragma unroll
+                    for (int sI = 0; sI < 2; ++sI)
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+                            o[X][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d][sI]),
+                                                                             __builtin_bit_cast(bf16x8, pf[X][kbk][sI]), o[X][d], 0, 0, 0);
+                };
+#pragma unroll
+                for (int X = 0; X < QB; ++X)
+                    if (!hidden(kbk, X) && !ondiag(kbk, X)) pv(X);
+#pragma unroll
+                for (int X = 0; X < QB; ++X)
+                    if (ondiag(kbk, X)) {
+#pragma unroll
+                        for (int d = 0; d < ND; ++d)
+#pragma unroll
+                            for (int sI = 0; sI < 2; ++sI) vf[d][sI] = finite_part(vf[d][sI], bad);
+                        pv(X);
+                    }
+            }
+        };
+        using one = std::integral_constant<int, 1>;
+        using two = std::integral_constant<int, 2>;
+        const int dt = q0 / PA_TILE;  // the tile that holds the wave's diagonal
+#pragma unroll
+        for (int X = 0; X < QB; ++X) settle(qf[X]);
+        issue(0);
+        stage_fence();
+        for (int t = 0; t < ntiles; ++t) {
+            if (t + 1 < ntiles) issue(t + 1);
+            if (t < dt) body(t, two{}, std::false_type{});
+            else if (t == dt && q0 < tl.len) {
+                if (QB == 1 && !(q0 & 32)) body(t, one{}, std::true_type{});
+                else body(t, two{}, std::true_type{});
+            }
+            stage_fence();
+        }
+        if (__any(bad)) {
+#pragma unroll
+            for (int X = 0; X < QB; ++X) {
+                const int k0 = q0 + 32 * X;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    add_nonfinite(o[X][d], a.V + (long long)(tl.start + k0) * a.ldv + kvh * D + d * 32 + l31, a.ldv, min(tl.len - k0, 32), l31, hh);
+            }
+        }
+    }
+#pragma unroll
+    for (int X = 0; X < QB; ++X) {
+        const int q = q0 + 32 * X + l31;
+        const bool ok = q < tl.len;
+        const float l = half_sum(l_run[X]);
+        if (a.lse && hh == 0 && ok) a.lse[(long long)h * a.rows + tl.start + q] = tl.tail ? -INFINITY : m_run[X] + __builtin_amdgcn_logf(l);
+        store_row<D>(a.out + (long long)(tl.start + (ok ? q : 0)) * a.ldo + h * D, o[X], tl.tail ? 0.f : 1.0f / l, hh, ok);
+    }
+}
+
+// ------------------------------------------------------------------ backward: dQ (and delta)
+// The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, dQ^T += K^T dS^T from transposed
+// reads of the same K tile.  delta is taken from the wave's own dO and O rows and left for the dK / dV kernel.
+template <int D>
+__global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
+    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TILEB];  // per stage: K, V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hh = lane >> 5;
+    Tile tl;
+    if (!find_tile(a, blockIdx.x / a.H, BM, false, tl)) return;
+    const int h = head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), kvh = h / (a.H / a.Hkv);
+    const int q0 = tl.tile * BM + wave * 32, q = q0 + l31;
+    const bool qok = q < tl.len;
+    const long long row = tl.start + (qok ? q : 0);
+    f32x16 dq[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+    if (!tl.tail) {
+        bf16x8 qf[NK], dof[NK];
+        load_frags<D>(qf, a.Q + row * a.ldq + h * D, hh, qok);
+        load_frags<D>(dof, a.dO + row * a.lddo + h * D, hh, qok);
+        float dlt = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            u32x4 ov = {0u, 0u, 0u, 0u};
+            if (qok) ov = *(const u32x4*)(a.O + row * a.ldo + h * D + ks * 16 + hh * 8);
+            float x[8], y[8];
+            unpack8(ov, x);
+            unpack8(__builtin_bit_cast(u32x4, dof[ks]), y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dlt = fmaf(x[j], y[j], dlt);
+        }
+        dlt = half_sum(dlt);
+        if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = dlt;
+        float lse = qok ? a.lse[(long long)h * a.rows + row] : 0.f;
+
+        const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
+        const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
+        const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
+        TileDma<D> kd, vd;
+        kd.init(wave, lane, ldkb);
+        vd.init(wave, lane, ldvb);
+        const unsigned lds0 = lds_addr(smem);
+        auto issue = [&](int t) {
+            const int left = tl.len - t * PA_TILE;
+            const unsigned st = lds0 + (t & 1) * 2 * TILEB;
+            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, min(left, PA_TILE), ldkb, ROWB), st);
+            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, min(left, PA_TILE), ldvb, ROWB), st + TILEB);
+        };
+        int rread[NK], klo[ND], khi[ND];
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, klo[d], khi[d]);
+        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
+        auto block = [&](const char* kb, const char* vb, auto diag_c) {
+            constexpr bool DIAG = decltype(diag_c)::value;
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kb + rread[ks]), qf[ks], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vb + rread[ks]), dof[ks], dp, 0, 0, 0);
+            }
+#pragma unroll
+            for (int sI = 0; sI < 2; ++sI) {
+                float ds[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = 8 * sI + j;
+                    ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dlt);
+                    if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > l31) ds[j] = 0.f;
+                }
+                const bf16x8 dsf = __builtin_bit_cast(bf16x8, pack8(ds));
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(kb + sI * 16 * ROWB + klo[d], kb + sI * 16 * ROWB + khi[d]), dsf, dq[d], 0, 0, 0);
+            }
+        };
+        settle(qf);
+        settle(dof);
+        asm volatile("" : "+v"(lse), "+v"(dlt));
+        issue(0);
+        stage_fence();
+        for (int t = 0; t < ntiles; ++t) {
+            if (t + 1 < ntiles) issue(t + 1);
+            const char* kb = smem + (t & 1) * 2 * TILEB;
+            const char* vb = kb + TILEB;
+            if (q0 < tl.len) {
+#pragma unroll 1
+                for (int kbk = 0; kbk < 2; ++kbk) {
+                    const int k0 = t * PA_TILE + kbk * 32;
+                    if (k0 < q0) block(kb + kbk * 32 * ROWB, vb + kbk * 32 * ROWB, std::false_type{});
+                    else if (k0 == q0) block(kb + kbk * 32 * ROWB, vb + kbk * 32 * ROWB, std::true_type{});
+                }
+            }
+            stage_fence();
+        }
+    }
+    store_row<D>(a.dQ + row * a.lddq + h * D, dq, a.scale, hh, qok);
+}
+
+// ------------------------------------------------------------------ backward: dK, dV
+// A wave owns 32 keys of a key head; the workgroup walks the query tiles from its own diagonal on, for every query head of the
+// group in turn, so the group's sum is taken in the accumulators, in a fixed order.
+template <int D>
+__global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
+    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, STAGEB = 2 * TILEB + 512;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGEB];  // per stage: Q, dO, lse and delta of the 64 queries
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hh = lane >> 5;
+    Tile tl;
+    if (!find_tile(a, blockIdx.x / a.Hkv, BM, true, tl)) return;
+    const int kvh = blockIdx.x % a.Hkv, G = a.H / a.Hkv;
+    const int k0 = tl.tile * BM + wave * 32, key = k0 + l31;
+    const bool kok = key < tl.len;
+    const long long row = tl.start + (kok ? key : 0);
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    if (!tl.tail) {
+        bf16x8 kf[NK], vf[NK];
+        load_frags<D>(kf, a.K + row * a.ldk + kvh * D, hh, kok);
+        load_frags<D>(vf, a.V + row * a.ldv + kvh * D, hh, kok);
+        const long long ldqb = a.ldq * 2, lddob = a.lddo * 2;
+        TileDma<D> qd, dd;
+        qd.init(wave, lane, ldqb);
+        dd.init(wave, lane, lddob);
+        const unsigned lds0 = lds_addr(smem);
+        const int t0 = tl.tile * BM / PA_TILE, per_head = (tl.len + PA_TILE - 1) / PA_TILE - t0;
+        auto issue = [&](int i) {  // step i of the walk: head i / per_head of the group, query tile t0 + i % per_head
+            const int g = i / per_head, t = t0 + i - g * per_head, h = kvh * G + g;
+            const long long r0 = (long long)tl.start + t * PA_TILE;
+            const int left = min(tl.len - t * PA_TILE, PA_TILE);
+            const unsigned st = lds0 + (i & 1) * STAGEB;
+            qd.issue(row_rsrc((const char*)(a.Q + r0 * a.ldq + h * D), left, ldqb, ROWB), st);
+            dd.issue(row_rsrc((const char*)(a.dO + r0 * a.lddo + h * D), left, lddob, ROWB), st + TILEB);
+            if (wave < 2) {  // queries behind the end read as lse = delta = 0, q = dO = 0: P = 1 meets only zeros
+                const float* p = (wave == 0 ? a.lse : a.delta) + (long long)h * a.rows + r0;
+                dma4(row_rsrc((const char*)p, left, 4, 4), st + 2 * TILEB + wave * 256, lane * 4);
+            }
+        };
+        int rread[NK], tlo[ND], thi[ND];
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, tlo[d], thi[d]);
+        auto block = [&](const char* qb, const char* db, const float* stat, auto diag_c) {
+            constexpr bool DIAG = decltype(diag_c)::value;
+            f32x16 s, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(db + rread[ks]), vf[ks], dp, 0, 0, 0);
+            }
+#pragma unroll
+            for (int sI = 0; sI < 2; ++sI) {
+                float p[8], ds[8];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int qo = 16 * sI + 8 * g + 4 * hh;  // registers 8 sI + 4 g .. + 3: four consecutive queries
+                    const f32x4 l4 = *(const f32x4*)(stat + qo), d4 = *(const f32x4*)(stat + 64 + qo);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int e = 8 * sI + 4 * g + j;
+                        float pe = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -l4[j]));
+                        float de = pe * (dp[e] - d4[j]);
+                        if (DIAG && qo + j < l31) { pe = 0.f; de = 0.f; }
+                        p[4 * g + j] = pe;
+                        ds[4 * g + j] = de;
+                    }
+                }
+                const bf16x8 pfr = __builtin_bit_cast(bf16x8, pack8(p)), dsf = __builtin_bit_cast(bf16x8, pack8(ds));
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(db + sI * 16 * ROWB + tlo[d], db + sI * 16 * ROWB + thi[d]), pfr, dv[d], 0, 0, 0);
+                    dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(qb + sI * 16 * ROWB + tlo[d], qb + sI * 16 * ROWB + thi[d]), dsf, dk[d], 0, 0, 0);
+                }
+            }
+        };
+        const int steps = per_head * G;
+        settle(kf);
+        settle(vf);
+        issue(0);
+        stage_fence();
+        for (int i = 0, t = t0; i < steps; ++i, t = t + 1 == t0 + per_head ? t0 : t + 1) {
+            if (i + 1 < steps) issue(i + 1);
+            const char* qb = smem + (i & 1) * STAGEB;
+            const char* db = qb + TILEB;
+            const float* stat = (const float*)(db + TILEB);
+            if (k0 < tl.len) {
+#pragma unroll
+                for (int qbk = 0; qbk < 2; ++qbk) {
+                    const int q0 = t * PA_TILE + qbk * 32;
+                    if (q0 > k0) block(qb + qbk * 32 * ROWB, db + qbk * 32 * ROWB, stat + qbk * 32, std::false_type{});
+                    else if (q0 == k0) block(qb + qbk * 32 * ROWB, db + qbk * 32 * ROWB, stat + qbk * 32, std::true_type{});
+                }
+            }
+            stage_fence();
+        }
+    }
+    store_row<D>(a.dK + row * a.lddk + kvh * D, dk, a.scale, hh, kok);
+    store_row<D>(a.dV + row * a.lddv + kvh * D, dv, 1.0f, hh, kok);
+}
+
+// the most tiles of `step` rows that n_seq sequences (and the rows behind them) can have in `rows` rows
+long long most_tiles(int rows, int n_seq, int step, int tail) {
+    return ((long long)rows + (long long)(n_seq + tail) * (step - 1)) / step;
+}
+
+bool row_ok(const void* p, int ld, int width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
+
+}  // namespace
+
+extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo,
+                                           const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale,
+                                           int zero_tail, float* lse, void* stream) {
+    if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
+    if (d != 64 && d != 128) return CCNET_EUNSUP;
+    if (rows == 0) return CCNET_OK;
+    if (!cu_seqlens || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d)) return CCNET_EINVAL;
+    if (ldk > (1 << 24) || ldv > (1 << 24)) return CCNET_EUNSUP;
+    PackedArgs a{};
+    a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.out = (__bf16*)O;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
+    a.cu = cu_seqlens; a.n_seq = n_seq; a.rows = rows; a.H = H; a.Hkv = Hkv;
+    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f; a.zero_tail = zero_tail != 0; a.lse = lse;
+    const bool wide = d == 64 && rows >= 256ll * n_seq;  // (mean length of at least 256: whole 256-query tiles are the rule)
+    const long long grid = most_tiles(rows, n_seq, wide ? 256 : 128, a.zero_tail) * H;
+    if (grid > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (grid == 0) return CCNET_OK;
+    hipStream_t st = (hipStream_t)stream;
+    if (d == 128) hipLaunchKernelGGL((packed_fwd_kernel<128, 1>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
+    else if (wide) hipLaunchKernelGGL((packed_fwd_kernel<64, 2>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
+    else hipLaunchKernelGGL((packed_fwd_kernel<64, 1>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
+    CCNET_LAUNCH_CHECK();
+    return CCNET_OK;
+}
+
+extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, const void* O,
+                                               int ldo, const void* dO, int lddo, const float* lse, float* delta, void* dQ, int lddq,
+                                               void* dK, int lddk, void* dV, int lddv, const int32_t* cu_seqlens, int n_seq, int rows,
+                                               int H, int Hkv, int d, float scale, int zero_tail, void* stream) {
+    if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
+    if (d != 64 && d != 128) return CCNET_EUNSUP;
+    if (rows == 0) return CCNET_OK;
+    if (!cu_seqlens || !lse || !delta || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) ||
+        !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) || !row_ok(dQ, lddq, H * d) || !row_ok(dK, lddk, Hkv * d) ||
+        !row_ok(dV, lddv, Hkv * d))
+        return CCNET_EINVAL;
+    if (ldq > (1 << 24) || ldk > (1 << 24) || ldv > (1 << 24) || lddo > (1 << 24)) return CCNET_EUNSUP;
+    PackedArgs a{};
+    a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.O = (const __bf16*)O; a.dO = (const __bf16*)dO;
+    a.dQ = (__bf16*)dQ; a.dK = (__bf16*)dK; a.dV = (__bf16*)dV;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;
+    a.cu = cu_seqlens; a.n_seq = n_seq; a.rows = rows; a.H = H; a.Hkv = Hkv;
+    a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f; a.zero_tail = zero_tail != 0;
+    a.lse = (float*)lse; a.delta = delta;
+    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail);
+    if (tiles * H > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (tiles == 0) return CCNET_OK;
+    hipStream_t st = (hipStream_t)stream;
+    if (d == 128) hipLaunchKernelGGL(packed_bwd_dq_kernel<128>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(packed_bwd_dq_kernel<64>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
+    CCNET_LAUNCH_CHECK();
+    if (d == 128) hipLaunchKernelGGL(packed_bwd_dkv_kernel<128>, dim3((unsigned)(tiles * Hkv)), dim3(PA_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(packed_bwd_dkv_kernel<64>, dim3((unsigned)(tiles * Hkv)), dim3(PA_THREADS), 0, st, a);
+    CCNET_LAUNCH_CHECK();
+    return CCNET_OK;
+}

@@ -1,0 +1,262 @@
+// Global gradient norm over many tensors, and clipping by it or by value.
+//
+//   norm = sqrt(sum over all tensors of g^2),  factor = min(1, max_norm / (norm + 1e-6)),  out = factor g
+//
+// The tensors are cut into tiles of CL_VECS 16-byte vectors; a launch takes up to CL_MOST tensors, their addresses and sizes by
+// value in the kernel's arguments (no table in memory that would have to outlive the call or be copied into a captured
+// graph).  Squares are summed in fp64: exact products, no overflow, and at 6 TB/s still far below the fp64 rate.  Every tile leaves
+// its sum in the workspace; norm_final_kernel adds them in tile order, so the result does not depend on the order of execution.
+#include "common.h"
+
+namespace {
+
+constexpr int CL_MOST = 128;           // tensors of a launch (28 bytes each of the 4 KiB of kernel arguments)
+constexpr int CL_VECS = 8192;          // 16-byte vectors of a tile (128 KiB)
+constexpr int CL_THREADS = 256;
+
+struct ClipArgs {
+    const void* in[CL_MOST];
+    void* out[CL_MOST];
+    long long n[CL_MOST];
+    int first[CL_MOST];  // the tensor's first tile, counted from the launch's first
+    int count;
+    double* partial;     // the launch's first tile's
+    const float* factor;
+    float limit;         // by value: clamp to [-limit, limit] instead of scaling by *factor
+};
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    typedef f32x4 __attribute__((aligned(4))) V;
+    static __device__ __forceinline__ float get(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ void unpack(const f32x4& v, float* f) { f[0] = v[0]; f[1] = v[1]; f[2] = v[2]; f[3] = v[3]; }
+    static __device__ __forceinline__ f32x4 pack(const float* f) { return f32x4{f[0], f[1], f[2], f[3]}; }
+    typedef f32x4 R;
+};
+template <> struct Vec<unsigned short> {
+    static constexpr int N = 8;
+    typedef u32x4 __attribute__((aligned(2))) V;
+    static __device__ __forceinline__ float get(const unsigned short* p) { return bf16_bits_to_f32(*p); }
+    static __device__ __forceinline__ void put(unsigned short* p, float v) { *p = f32_to_bf16_bits(v); }
+    static __device__ __forceinline__ void unpack(const u32x4& v, float* f) { unpack8(v, f); }
+    static __device__ __forceinline__ u32x4 pack(const float* f) { return pack8(f); }
+    typedef u32x4 R;
+};
+
+// elements in front of the first 16-byte boundary of a tensor, and its whole vectors behind it
+template <typename T>
+__host__ __device__ __forceinline__ long long head_of(const void* p, long long n) {
+    const long long h = (long long)((16 - ((uintptr_t)p & 15)) & 15) / (long long)sizeof(T);
+    return h < n ? h : n;
+}
+template <typename T>
+__host__ __device__ __forceinline__ long long tiles_of(const void* p, long long n) {
+    const long long vecs = (n - head_of<T>(p, n)) / (16 / (long long)sizeof(T));
+    const long long t = (vecs + CL_VECS - 1) / CL_VECS;
+    return n == 0 ? 0 : t > 0 ? t : 1;
+}
+
+// the tensor of tile `tile` of the launch: the last one whose first tile is not behind it (tensors without elements have none)
+__device__ __forceinline__ int tensor_of(const ClipArgs& a, int tile) {
+    int lo = 0, hi = a.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.first[mid] <= tile) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T>
+__global__ __launch_bounds__(CL_THREADS) void norm_tile_kernel(const ClipArgs a) {
+    typedef Vec<T> X;
+    const int k = tensor_of(a, blockIdx.x), tile = blockIdx.x - a.first[k];
+    const T* p = (const T*)a.in[k];
+    const long long n = a.n[k], head = head_of<T>(p, n), vecs = (n - head) / X::N;
+    const long long v0 = (long long)tile * CL_VECS, v1 = min(vecs, v0 + CL_VECS);
+    double s[X::N] = {};
+    for (long long v = v0 + threadIdx.x; v < v1; v += CL_THREADS) {
+        float f[X::N];
+        X::unpack(*(const typename X::R*)(p + head + v * X::N), f);
+#pragma unroll
+        for (int e = 0; e < X::N; ++e) s[e] = fma((double)f[e], (double)f[e], s[e]);
+    }
+    if (tile == 0) {  // what lies outside the whole vectors: at most N - 1 elements on either side
+        const long long tail = head + vecs * X::N;
+        const long long i = threadIdx.x < head ? (long long)threadIdx.x : tail + ((long long)threadIdx.x - head);
+        if (i < n) {
+            const double f = X::get(p + i);
+            s[0] = fma(f, f, s[0]);
+        }
+    }
+    double t = 0;
+#pragma unroll
+    for (int e = 0; e < X::N; ++e) t += s[e];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+    __shared__ double red[CL_THREADS / 64];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+__global__ __launch_bounds__(1024) void norm_final_kernel(const double* partial, int n, float max_norm, float* norm, float* factor) {
+    double t = 0;
+    for (int i = threadIdx.x; i < n; i += 1024) t += partial[i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+    __shared__ double red[16];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0;
+        for (int i = 0; i < 16; ++i) s += red[i];
+        const double r = sqrt(s);
+        *norm = (float)r;
+        // a norm that is not finite scales nothing: the caller sees it and skips its step
+        const float f = (float)((double)max_norm / (r + 1e-6));
+        if (factor) *factor = (float)r <= 3.4028235e38f && f < 1.0f ? f : 1.0f;
+    }
+}
+
+template <typename T, bool VALUE>
+__global__ __launch_bounds__(CL_THREADS) void clip_tile_kernel(const ClipArgs a) {
+    typedef Vec<T> X;
+    const int k = tensor_of(a, blockIdx.x), tile = blockIdx.x - a.first[k];
+    const T* p = (const T*)a.in[k];
+    T* q = (T*)a.out[k];
+    const float f = VALUE ? 1.0f : *a.factor, lim = a.limit;
+    if (!VALUE && f == 1.0f && p == q) return;
+    // (a NaN stays one: it compares with neither limit)
+    auto one = [&](float v) { return VALUE ? (v > lim ? lim : v < -lim ? -lim : v) : v * f; };
+    const long long n = a.n[k], head = head_of<T>(p, n), vecs = (n - head) / X::N;
+    const long long v0 = (long long)tile * CL_VECS, v1 = min(vecs, v0 + CL_VECS);
+    for (long long v = v0 + threadIdx.x; v < v1; v += CL_THREADS) {
+        float x[X::N];
+        X::unpack(*(const typename X::R*)(p + head + v * X::N), x);
+#pragma unroll
+        for (int e = 0; e < X::N; ++e) x[e] = one(x[e]);
+        *(typename X::V*)(q + head + v * X::N) = X::pack(x);  // (the output may be aligned to its elements only)
+    }
+    if (tile == 0) {
+        const long long tail = head + vecs * X::N;
+        const long long i = threadIdx.x < head ? (long long)threadIdx.x : tail + ((long long)threadIdx.x - head);
+        if (i < n) X::put(q + i, one(X::get(p + i)));
+    }
+}
+
+// fills the launches of a list in turn: launch(args, first tile of all, tiles)
+template <typename T, typename F>
+int each_launch(const void* const* in, void* const* out, const int64_t* numel, int count, F launch) {
+    long long before = 0;
+    for (int i = 0; i < count;) {
+        ClipArgs a{};
+        long long tiles = 0;
+        while (i < count && a.count < CL_MOST) {
+            const long long t = tiles_of<T>(in[i], numel[i]);
+            if (t == 0) { ++i; continue; }
+            if (tiles + t > 0x7fffffffLL) {
+                if (a.count == 0) return CCNET_EUNSUP;
+                break;
+            }
+            a.in[a.count] = in[i];
+            a.out[a.count] = out ? out[i] : nullptr;
+            a.n[a.count] = numel[i];
+            a.first[a.count] = (int)tiles;
+            ++a.count;
+            tiles += t;
+            ++i;
+        }
+        if (a.count == 0) break;
+        launch(a, before, (unsigned)tiles);
+        CCNET_LAUNCH_CHECK();
+        before += tiles;
+    }
+    return CCNET_OK;
+}
+
+bool list_ok(const void* const* p, const int64_t* numel, int count, int esz) {
+    if (count < 0 || (count > 0 && (!p || !numel))) return false;
+    for (int i = 0; i < count; ++i)
+        if (numel[i] < 0 || (numel[i] > 0 && (!p[i] || (uintptr_t)p[i] % esz))) return false;
+    return true;
+}
+
+template <typename T>
+int norm_launches(const void* const* g, const int64_t* numel, int count, double* ws, hipStream_t st) {
+    return each_launch<T>(g, nullptr, numel, count, [&](ClipArgs& a, long long before, unsigned tiles) {
+        a.partial = ws + 1 + before;
+        hipLaunchKernelGGL(norm_tile_kernel<T>, dim3(tiles), dim3(CL_THREADS), 0, st, a);
+    });
+}
+template <typename T, bool VALUE>
+int clip_launches(const void* const* g, void* const* out, const int64_t* numel, int count, const float* factor, float limit, hipStream_t st) {
+    return each_launch<T>(g, out, numel, count, [&](ClipArgs& a, long long, unsigned tiles) {
+        a.factor = factor;
+        a.limit = limit;
+        hipLaunchKernelGGL((clip_tile_kernel<T, VALUE>), dim3(tiles), dim3(CL_THREADS), 0, st, a);
+    });
+}
+
+long long all_tiles(const void* const* g, const int64_t* numel, int count, int dtype) {
+    long long t = 0;
+    for (int i = 0; i < count; ++i) t += dtype == 0 ? tiles_of<float>(g[i], numel[i]) : tiles_of<unsigned short>(g[i], numel[i]);
+    return t;
+}
+
+}  // namespace
+
+extern "C" size_t ccnet_grad_norm_workspace_bytes(const void* const* grads, const int64_t* numel, int count, int dtype) {
+    if ((dtype != 0 && dtype != 1) || !list_ok(grads, numel, count, dtype == 0 ? 4 : 2)) return 0;
+    return 8 * (size_t)(1 + all_tiles(grads, numel, count, dtype));
+}
+
+extern "C" int ccnet_grad_norm(const void* const* grads, const int64_t* numel, int count, int dtype, void* workspace,
+                               size_t workspace_bytes, float* norm, void* stream) {
+    if ((dtype != 0 && dtype != 1) || !norm || !list_ok(grads, numel, count, dtype == 0 ? 4 : 2)) return CCNET_EINVAL;
+    const long long tiles = all_tiles(grads, numel, count, dtype);
+    if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (!workspace || ((uintptr_t)workspace & 7)) return CCNET_EINVAL;
+    if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
+    hipStream_t st = (hipStream_t)stream;
+    double* ws = (double*)workspace;
+    const int rc = dtype == 0 ? norm_launches<float>(grads, numel, count, ws, st) : norm_launches<unsigned short>(grads, numel, count, ws, st);
+    if (rc != CCNET_OK) return rc;
+    hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(1024), 0, st, ws + 1, (int)tiles, 0.f, norm, (float*)nullptr);
+    CCNET_LAUNCH_CHECK();
+    return CCNET_OK;
+}
+
+extern "C" int ccnet_clip_grad_norm(const void* const* grads, void* const* out, const int64_t* numel, int count, int dtype,
+                                    float max_norm, void* workspace, size_t workspace_bytes, float* norm, void* stream) {
+    const int esz = dtype == 0 ? 4 : 2;
+    if ((dtype != 0 && dtype != 1) || !norm || !(max_norm >= 0.f) || !list_ok(grads, numel, count, esz) ||
+        !list_ok((const void* const*)out, numel, count, esz))
+        return CCNET_EINVAL;
+    const long long tiles = all_tiles(grads, numel, count, dtype);
+    if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (!workspace || ((uintptr_t)workspace & 7)) return CCNET_EINVAL;
+    if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
+    hipStream_t st = (hipStream_t)stream;
+    double* ws = (double*)workspace;
+    float* factor = (float*)workspace;  // the workspace's first 8 bytes
+    int rc = dtype == 0 ? norm_launches<float>(grads, numel, count, ws, st) : norm_launches<unsigned short>(grads, numel, count, ws, st);
+    if (rc != CCNET_OK) return rc;
+    hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(1024), 0, st, ws + 1, (int)tiles, max_norm, norm, factor);
+    CCNET_LAUNCH_CHECK();
+    return dtype == 0 ? clip_launches<float, false>(grads, out, numel, count, factor, 0.f, st)
+                      : clip_launches<unsigned short, false>(grads, out, numel, count, factor, 0.f, st);
+}
+
+extern "C" int ccnet_clip_grad_value(const void* const* grads, void* const* out, const int64_t* numel, int count, int dtype,
+                                     float limit, void* stream) {
+    const int esz = dtype == 0 ? 4 : 2;
+    if ((dtype != 0 && dtype != 1) || !(limit >= 0.f) || !list_ok(grads, numel, count, esz) ||
+        !list_ok((const void* const*)out, numel, count, esz))
+        return CCNET_EINVAL;
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == 0 ? clip_launches<float, true>(grads, out, numel, count, nullptr, limit, st)
+                      : clip_launches<unsigned short, true>(grads, out, numel, count, nullptr, limit, st);
+}

@@ -29,6 +29,10 @@ EXPORTS = [
     "ccnet_resample_bwd_bf16", "ccnet_attention_d64_lse_bf16", "ccnet_attention_d64_bwd_bf16",
     "ccnet_attention_d64_prescaled_bf16", "ccnet_ff_geglu_fused_bf16", "ccnet_ff_packed_bytes", "ccnet_noalloc_init",
     "ccnet_xattn_fused_bf16", "ccnet_xattn_packed_bytes", "ccnet_xattn_kv_image_bytes",
+    # token lookup, packed causal attention, gradient clipping
+    "ccnet_embedding", "ccnet_embedding_grad_workspace_bytes", "ccnet_embedding_grad", "ccnet_attention_packed_bf16",
+    "ccnet_attention_packed_bwd_bf16", "ccnet_grad_norm_workspace_bytes", "ccnet_grad_norm", "ccnet_clip_grad_norm",
+    "ccnet_clip_grad_value",
 ]
 
 
@@ -129,6 +133,19 @@ def load() -> C.CDLL:
     lib.ccnet_xattn_packed_bytes.restype = C.c_int64
     lib.ccnet_xattn_kv_image_bytes.argtypes = [i, i]
     lib.ccnet_xattn_kv_image_bytes.restype = C.c_int64
+    lib.ccnet_embedding.argtypes = [vp, i, i, i, vp, i, i, i, f, vp, i, i, vp]
+    lib.ccnet_embedding_grad_workspace_bytes.argtypes = [i, i]
+    lib.ccnet_embedding_grad_workspace_bytes.restype = sz
+    lib.ccnet_embedding_grad.argtypes = [vp, i, i, i, vp, i, i, i, f, i64, vp, i, i, vp, sz, vp]
+    lib.ccnet_attention_packed_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, i, vp, vp]
+    lib.ccnet_attention_packed_bwd_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, vp, vp, vp, i, vp, i, vp, i, vp, i, i, i, i, i,
+                                                    f, i, vp]
+    pp, pi64 = C.POINTER(vp), C.POINTER(i64)
+    lib.ccnet_grad_norm_workspace_bytes.argtypes = [pp, pi64, i, i]
+    lib.ccnet_grad_norm_workspace_bytes.restype = sz
+    lib.ccnet_grad_norm.argtypes = [pp, pi64, i, i, vp, sz, vp, vp]
+    lib.ccnet_clip_grad_norm.argtypes = [pp, pp, pi64, i, i, f, vp, sz, vp, vp]
+    lib.ccnet_clip_grad_value.argtypes = [pp, pp, pi64, i, i, f, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is C.c_int:  # default

@@ -590,6 +590,251 @@ def axpy_f32(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ------------------------------------------------------------------ token lookup, packed attention, gradient clipping
+_F32_BF16 = {torch.float32: 0, BF16: 1}
+
+
+class _on_device_of:
+    """Makes the tensors' device current for the launch (a no-op where it is): the stream is that device's current one."""
+
+    def __init__(self, *ts: Optional[torch.Tensor]):
+        ts = [t for t in ts if t is not None]
+        _need_cuda(*ts)
+        if any(t.device != ts[0].device for t in ts):
+            raise _l.CcnetError("operands are on different devices: " + ", ".join(str(t.device) for t in ts))
+        self.device = ts[0].device
+        self.guard = None
+
+    def __enter__(self) -> int:
+        if self.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+        return _stream()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
+    """Row stride of a 2-D operand [rows, width] whose rows are contiguous; raises on anything else."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype not in dtypes:
+        raise _l.CcnetError(f"{what}: expected {' or '.join(str(d) for d in dtypes)} [{rows}, {width}], got {t.dtype} {list(t.shape)}")
+    if width > 1 and t.stride(1) != 1:
+        raise _l.CcnetError(f"{what}: rows must be contiguous (column stride {t.stride(1)})")
+    ld = t.stride(0) if rows > 1 else max(t.stride(0), (width + 7) // 8 * 8)
+    if max(rows, ld) > 0x7fffffff:
+        raise _l.CcnetError(f"{what}: {rows} rows of stride {ld} pass the 32 bits of the C ABI")
+    return ld
+
+
+def _ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise _l.CcnetError(f"ids must be int64 or int32, got {ids.dtype}")
+    return ids.reshape(-1).contiguous()
+
+
+def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype: torch.dtype = BF16,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """scale * table[ids] as [ids.numel(), C] rows: ids int64 / int32, table fp32 / bf16 [vocab, C] (row stride free), result in
+    `dtype` (fp32 / bf16, rounded once) or in `out`.  An id outside the table gives a row of zeros."""
+    lib = _l.load()
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise _l.CcnetError(f"table must be [vocab, C], got {list(table.shape)}")
+    ldt = _rows_ld(table, "table", table.shape[0], table.shape[1], tuple(_F32_BF16))
+    with _on_device_of(ids, table, out) as st:
+        flat = _ids(ids)
+        T, Cc = flat.numel(), table.shape[1]
+        if out is None:
+            out = torch.empty((T, Cc), dtype=dtype, device=ids.device)
+        ldo = _rows_ld(out, "out", T, Cc, tuple(_F32_BF16))
+        _l.check(lib.ccnet_embedding(flat.data_ptr(), flat.element_size(), T, table.shape[0], table.data_ptr(), _F32_BF16[table.dtype],
+                                     ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, st), "embedding")
+    return out
+
+
+def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float = 1.0, padding_idx: Optional[int] = None,
+                   out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """Gradient of `embedding` with respect to its table, fp32 [vocab, C]: row v = scale * sum of dy[t] over ids[t] == v (zeros
+    for rows no position names).  dy fp32 / bf16 [T, C].  Positions with padding_idx or an id outside the table take no part.
+    accumulate: added to `out`, whose other rows are not touched."""
+    lib = _l.load()
+    if accumulate and out is None:
+        raise _l.CcnetError("embedding_grad: accumulate needs out")
+    if not 0 < vocab < 0x7fffffff:
+        raise _l.CcnetError(f"embedding_grad: vocab {vocab}")
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise _l.CcnetError(f"embedding_grad: padding_idx {padding_idx} outside the table of {vocab}")
+    with _on_device_of(ids, dy, out) as st:
+        flat = _ids(ids)
+        T = flat.numel()
+        if dy.dim() != 2 or dy.shape[1] < 1:
+            raise _l.CcnetError(f"dy must be [T, C], got {list(dy.shape)}")
+        Cc = dy.shape[1]
+        lddy = _rows_ld(dy, "dy", T, Cc, tuple(_F32_BF16))
+        if out is None:
+            out = torch.empty((vocab, Cc), dtype=torch.float32, device=dy.device)
+        ldg = _rows_ld(out, "out", vocab, Cc, (torch.float32,))
+        wsb = lib.ccnet_embedding_grad_workspace_bytes(T, Cc)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device)
+        _l.check(lib.ccnet_embedding_grad(flat.data_ptr(), flat.element_size(), T, vocab, dy.data_ptr(), _F32_BF16[dy.dtype], lddy, Cc,
+                                          scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ldg, int(accumulate),
+                                          ws.data_ptr(), wsb, st), "embedding_grad")
+    return out
+
+
+def _packed_operands(q, k, v, cu_seqlens, H: int, Hkv: int, d: int):
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise _l.CcnetError(f"attention_packed: {H} query heads do not divide into {Hkv} key heads")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or not cu_seqlens.is_contiguous():
+        raise _l.CcnetError("attention_packed: cu_seqlens must be a contiguous int32 vector (0, end of sequence 0, ...)")
+    rows = q.shape[0]
+    return rows, (_rows_ld(q, "q", rows, H * d, (BF16,)), _rows_ld(k, "k", rows, Hkv * d, (BF16,)),
+                  _rows_ld(v, "v", rows, Hkv * d, (BF16,)))
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, H: int, Hkv: int, d: int,
+                     scale: float, with_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Causal self-attention over sequences that lie end to end in the rows: q [rows, H*d], k / v [rows, Hkv*d] bf16 (column
+    slices of one matrix allowed), query head h on key head h // (H // Hkv), d 64 or 128, sequence i = rows
+    cu_seqlens[i] .. cu_seqlens[i+1] (int32 on the GPU, never copied to the host).  Returns o [rows, H*d], with_lse: (o, lse) for
+    `attention_packed_bwd`.  Rows behind the last sequence are zeros, or with `out` (which must not overlap k or v) left as
+    they are."""
+    lib = _l.load()
+    with _on_device_of(q, k, v, cu_seqlens, out) as st:
+        rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
+        o = torch.empty((rows, H * d), dtype=BF16, device=q.device) if out is None else out
+        lse = torch.empty((H, rows), dtype=torch.float32, device=q.device) if with_lse else None
+        _l.check(lib.ccnet_attention_packed_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(),
+                                                 _rows_ld(o, "out", rows, H * d, (BF16,)), cu_seqlens.data_ptr(),
+                                                 cu_seqlens.numel() - 1, rows, H, Hkv, d, scale, int(out is None), _ptr(lse), st),
+                 "attention_packed")
+    return (o, lse) if with_lse else o
+
+
+def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, lse: torch.Tensor,
+                         cu_seqlens: torch.Tensor, H: int, Hkv: int, d: int, scale: float, dq: Optional[torch.Tensor] = None,
+                         dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
+    """(dq, dk, dv) of `attention_packed` from its o, lse and the gradient `do` of o; dk / dv hold the sum over the query heads of
+    a key head.  The results overwrite dq / dk / dv where given (all three, e.g. column slices of one matrix; rows behind the
+    last sequence are then left as they are) or are new tensors (those rows zeros)."""
+    lib = _l.load()
+    given = [g is not None for g in (dq, dk, dv)]
+    if any(given) and not all(given):
+        raise _l.CcnetError("attention_packed_bwd: give all of dq, dk, dv or none")
+    with _on_device_of(q, k, v, o, do, lse, cu_seqlens, dq, dk, dv) as st:
+        rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
+        if lse.dtype != torch.float32 or tuple(lse.shape) != (H, rows) or not lse.is_contiguous():
+            raise _l.CcnetError(f"attention_packed_bwd: lse must be the forward's fp32 [{H}, {rows}]")
+        if not given[0]:
+            dq, dk, dv = (torch.empty((rows, n * d), dtype=BF16, device=q.device) for n in (H, Hkv, Hkv))
+        delta = torch.empty((H, rows), dtype=torch.float32, device=q.device)
+        _l.check(lib.ccnet_attention_packed_bwd_bf16(
+            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), _rows_ld(o, "o", rows, H * d, (BF16,)),
+            do.data_ptr(), _rows_ld(do, "do", rows, H * d, (BF16,)), lse.data_ptr(), delta.data_ptr(),
+            dq.data_ptr(), _rows_ld(dq, "dq", rows, H * d, (BF16,)), dk.data_ptr(), _rows_ld(dk, "dk", rows, Hkv * d, (BF16,)),
+            dv.data_ptr(), _rows_ld(dv, "dv", rows, Hkv * d, (BF16,)), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, H, Hkv, d,
+            scale, int(not given[0]), st), "attention_packed_bwd")
+    return dq, dk, dv
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one range of memory, each place once (in any order of the dimensions)."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _grad_list(grads, what: str):
+    grads = list(grads)
+    if not grads:
+        raise _l.CcnetError(f"{what}: no gradients")
+    dt = grads[0].dtype
+    if dt not in _F32_BF16 or any(g.dtype != dt for g in grads):
+        raise _l.CcnetError(f"{what}: gradients must all be fp32 or all bf16, got {sorted({str(g.dtype) for g in grads})}")
+    if not all(_dense(g) for g in grads):
+        raise _l.CcnetError(f"{what}: a gradient's elements must fill one range of memory (expanded or strided views do not)")
+    n = len(grads)
+    return grads, (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads]), n, _F32_BF16[dt]
+
+
+def _clip_outputs(grads, ptrs, out, what: str):
+    """(pointers to write to, the tensors written): in place, or `out` with the same shapes, strides and type."""
+    if out is None:
+        outs, optrs = grads, ptrs
+    else:
+        outs = list(out)
+        if len(outs) != len(grads) or any(o.shape != g.shape or o.stride() != g.stride() or o.dtype != g.dtype
+                                          for o, g in zip(outs, grads)):
+            raise _l.CcnetError(f"{what}: out must match the gradients' shapes, strides and type")
+        optrs = (C.c_void_p * len(outs))(*[o.data_ptr() for o in outs])
+    esz = grads[0].element_size()
+    spans = sorted((o.data_ptr(), o.data_ptr() + o.numel() * esz, i) for i, o in enumerate(outs) if o.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise _l.CcnetError(f"{what}: the tensors written overlap (one tensor given twice?)")
+    if out is not None:  # a gradient read by one tile while another writes there
+        reads = sorted((g.data_ptr(), g.data_ptr() + g.numel() * esz, i) for i, g in enumerate(grads) if g.numel())
+        j = 0
+        for lo, hi, i in reads:
+            while j > 0 and spans[j - 1][1] > lo:
+                j -= 1
+            while j < len(spans) and spans[j][1] <= lo:
+                j += 1
+            m = j
+            while m < len(spans) and spans[m][0] < hi:
+                if not (spans[m][2] == i and spans[m][0] == lo):
+                    raise _l.CcnetError(f"{what}: out overlaps a gradient other than its own")
+                m += 1
+    return optrs, outs
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """The L2 norm over all elements of all tensors (fp32 or bf16, contiguous in any order of their dimensions), summed in fp64:
+    an fp32 scalar on the GPU."""
+    lib = _l.load()
+    grads, ptrs, numel, n, dt = _grad_list(grads, "grad_norm")
+    with _on_device_of(*grads) as st:
+        wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
+        ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), st), "grad_norm")
+    return norm
+
+
+def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
+    """grads *= min(1, max_norm / (norm + 1e-6)) for the norm over all of them (util.py:1176-1206, clip_grad_norm_), without a
+    synchronisation: returns the norm before clipping as an fp32 scalar on the GPU.  A norm that is not finite scales nothing.
+    out: tensors of the same shapes that receive the clipped values instead; the tensors written must not overlap."""
+    lib = _l.load()
+    grads, ptrs, numel, n, dt = _grad_list(grads, "clip_grad_norm")
+    if not max_norm >= 0:
+        raise _l.CcnetError(f"clip_grad_norm: max_norm {max_norm}")
+    optrs, outs = _clip_outputs(grads, ptrs, out, "clip_grad_norm")
+    with _on_device_of(*grads, *(outs if out is not None else ())) as st:
+        wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
+        ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), st),
+                 "clip_grad_norm")
+    return norm
+
+
+def clip_grad_value(grads, limit: float, out=None) -> None:
+    """Every element clamped to [-limit, limit] in place (clip_grad_value_), or into `out` as in `clip_grad_norm`."""
+    lib = _l.load()
+    grads, ptrs, numel, n, dt = _grad_list(grads, "clip_grad_value")
+    if not limit >= 0:
+        raise _l.CcnetError(f"clip_grad_value: limit {limit}")
+    optrs, outs = _clip_outputs(grads, ptrs, out, "clip_grad_value")
+    with _on_device_of(*grads, *(outs if out is not None else ())) as st:
+        _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, st), "clip_grad_value")
+
+
 _prof_on = False
 
 

@@ -1,0 +1,164 @@
+"""What the entry points for token lookup, packed attention and gradient clipping refuse, on the host: nothing here launches."""
+import ctypes as C
+
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+def _err():
+    from ccnet_amd.lib import CcnetError
+    return CcnetError
+
+
+def _lib():
+    from ccnet_amd import lib
+    return lib.load()
+
+
+def test_cpu_tensors_are_refused():
+    from ccnet_amd import ops
+    ids, x = torch.zeros(4, dtype=torch.int64), torch.zeros(4, 64)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    b = x.to(BF16)
+    for call in (lambda: ops.embedding(ids, x), lambda: ops.embedding_grad(ids, x, 9), lambda: ops.attention_packed(b, b, b, cu, 1, 1, 64, 1.0),
+                 lambda: ops.attention_packed_bwd(b, b, b, b, b, x[:1, :4], cu, 1, 1, 64, 1.0), lambda: ops.grad_norm([x]),
+                 lambda: ops.clip_grad_norm([x], 1.0), lambda: ops.clip_grad_value([x], 1.0)):
+        with pytest.raises(_err(), match="GPU only"):
+            call()
+
+
+def test_wrapper_refusals_before_any_launch():
+    from ccnet_amd import ops
+    x = torch.zeros(4, 64)
+    ids = torch.zeros(4, dtype=torch.int64)
+    for call in (lambda: ops.embedding(ids, x[0]), lambda: ops.embedding(ids, x.t()), lambda: ops.embedding(ids, x.half()),
+                 lambda: ops.embedding_grad(ids, x, 9, accumulate=True), lambda: ops.embedding_grad(ids, x, 0),
+                 lambda: ops.embedding_grad(ids, x, 9, padding_idx=9), lambda: ops.grad_norm([]), lambda: ops.grad_norm([x, x.to(BF16)]),
+                 lambda: ops.grad_norm([x.half()]), lambda: ops.grad_norm([x[:, :3]]), lambda: ops.grad_norm([x[:1].expand(4, 64)]),
+                 lambda: ops.clip_grad_norm([x], -1.0), lambda: ops.clip_grad_norm([x], float("nan")),
+                 lambda: ops.clip_grad_value([x], -1.0), lambda: ops.clip_grad_norm([x, x], 1.0),
+                 lambda: ops.clip_grad_norm([x, x[1]], 1.0), lambda: ops.clip_grad_norm([x], 1.0, out=[]),
+                 lambda: ops.clip_grad_norm([x], 1.0, out=[x.t()]), lambda: ops.clip_grad_norm([x], 1.0, out=[x.to(BF16)])):
+        with pytest.raises(_err()):
+            call()
+
+
+def test_clip_outputs_must_not_overlap_other_gradients():
+    """The aliasing rules by themselves (they are checked before the device): in place and apart are fine, shifted is not."""
+    from ccnet_amd import ops
+
+    def go(grads, out):
+        grads, ptrs, *_ = ops._grad_list(grads, "t")
+        return ops._clip_outputs(grads, ptrs, out, "t")
+
+    f = torch.zeros(100)
+    a, b, c = f[:10], f[10:20], f[20:30]
+    go([a, b, c], None)
+    go([a, b], [a, b])
+    go([a, b], [c, f[40:50]])
+    go([a, b], [a, c])
+    go([c, a], [f[50:60], a])
+    go([a, a[:0], b], [c, a[:0], f[40:50]])
+    go([a, a], [b, c])  # reading one twice is fine
+    for grads, out in (([a, b], [b, a]), ([a, b], [f[5:15], c]), ([a], [f[1:11]]), ([a, b, c], [f[50:60], f[12:22], f[70:80]]),
+                       ([a, b], [c, c]), ([a, b], [f[60:70], f[65:75]]), ([f[:50], c], [f[50:], f[30:40]])):
+        with pytest.raises(_err()):
+            go(grads, out)
+
+
+def test_dense_layouts():
+    from ccnet_amd import ops
+    x = torch.zeros(4, 6, 5)
+    assert all(ops._dense(t) for t in (x, x.permute(2, 0, 1), x.transpose(0, 1), x[1], x[:1], torch.zeros(0), x[1, 1, 1]))
+    assert not any(ops._dense(t) for t in (x[:, ::2], x[:, :3], x[..., 1], x[:1].expand(4, 6, 5)))
+
+
+EINVAL, EUNSUP, EWS = -1, -2, -4
+
+
+def test_c_abi_refusals():
+    l = _lib()
+    p = C.c_void_p(1 << 20)  # never dereferenced: every call here returns before a launch
+    E = l.ccnet_embedding
+    ok = [p, 8, 4, 10, p, 0, 64, 64, 1.0, p, 1, 64, None]
+    for i, v in ((1, 2), (2, -1), (3, 0), (4, None), (5, 2), (6, 63), (7, 0), (9, None), (10, 3), (11, 10), (0, None), (0, C.c_void_p(1028)),
+                 (4, C.c_void_p(1026)), (9, C.c_void_p(1025))):
+        a = list(ok)
+        a[i] = v
+        assert E(*a) == EINVAL, (i, v)
+    a = list(ok)
+    a[2] = 0
+    assert E(*a) == 0  # no rows: nothing to do
+    G = l.ccnet_embedding_grad
+    need = l.ccnet_embedding_grad_workspace_bytes(1000, 64)
+    assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 64) == 0
+    ok = [p, 8, 1000, 10, p, 1, 64, 64, 1.0, -1, p, 64, 0, p, need, None]
+    for i, v, rc in ((1, 3, EINVAL), (2, -1, EINVAL), (3, 0, EINVAL), (3, 0x7fffffff, EINVAL), (4, None, EINVAL), (5, 2, EINVAL), (6, 8, EINVAL),
+                     (7, 0, EINVAL), (10, None, EINVAL), (10, C.c_void_p(1026), EINVAL), (11, 63, EINVAL), (13, None, EINVAL),
+                     (13, C.c_void_p(1028), EINVAL), (14, need - 1, EWS), (2, (1 << 30) + 1, EUNSUP)):
+        a = list(ok)
+        a[i] = v
+        assert G(*a) == rc, (i, v)
+    F = l.ccnet_attention_packed_bf16
+    ok = [p, 256, p, 128, p, 128, p, 256, p, 3, 100, 4, 2, 64, 0.125, 1, None, None]
+    odd = C.c_void_p(1 << 20 | 8)
+    for i, v, rc in ((0, None, EINVAL), (0, odd, EINVAL), (1, 255, EINVAL), (1, 248, EINVAL), (2, None, EINVAL), (3, 64, EINVAL), (4, odd, EINVAL),
+                     (5, 132, EINVAL), (6, None, EINVAL), (7, 192, EINVAL), (8, None, EINVAL), (9, -1, EINVAL), (10, -1, EINVAL), (11, 0, EINVAL),
+                     (11, 3, EINVAL), (12, 0, EINVAL), (13, 96, EUNSUP), (13, 32, EUNSUP), (14, 0.0, EINVAL), (14, -1.0, EINVAL),
+                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP)):
+        a = list(ok)
+        a[i] = v
+        assert F(*a) == rc, (i, v)
+    a = list(ok)
+    a[10] = 0
+    assert F(*a) == 0
+    B = l.ccnet_attention_packed_bwd_bf16
+    ok = [p, 256, p, 128, p, 128, p, 256, p, 256, p, p, p, 256, p, 128, p, 128, p, 3, 100, 4, 2, 64, 0.125, 1, None]
+    for i in (0, 2, 4, 6, 8, 10, 11, 12, 14, 16, 18):
+        a = list(ok)
+        a[i] = None
+        assert B(*a) == EINVAL, i
+    for i in (1, 3, 5, 7, 9, 13, 15, 17):
+        a = list(ok)
+        a[i] = 100
+        assert B(*a) == EINVAL, i
+    for i, v, rc in ((21, 3, EINVAL), (23, 80, EUNSUP), (24, 0.0, EINVAL), (20, 0, 0)):
+        a = list(ok)
+        a[i] = v
+        assert B(*a) == rc, (i, v)
+    ptrs, n = (C.c_void_p * 2)(1 << 20, 1 << 24), (C.c_int64 * 2)(1000, 70000)
+    need = l.ccnet_grad_norm_workspace_bytes(ptrs, n, 2, 0)
+    assert need == 8 * (1 + 1 + 3)
+    for args, rc in (((ptrs, n, 2, 2, p, need, p, None), EINVAL), ((ptrs, n, -1, 0, p, need, p, None), EINVAL), ((None, n, 2, 0, p, need, p, None), EINVAL),
+                     ((ptrs, n, 2, 0, None, need, p, None), EINVAL), ((ptrs, n, 2, 0, p, need - 1, p, None), EWS), ((ptrs, n, 2, 0, p, need, None, None), EINVAL)):
+        assert l.ccnet_grad_norm(*args) == rc
+    bad = (C.c_void_p * 2)(1 << 20 | 2, 1 << 24)
+    none = (C.c_void_p * 2)(1 << 20, None)
+    neg = (C.c_int64 * 2)(-1, 5)
+    for q in (bad, none):
+        assert l.ccnet_grad_norm(q, n, 2, 0, p, need, p, None) == EINVAL
+        assert l.ccnet_clip_grad_norm(ptrs, q, n, 2, 0, 1.0, p, need, p, None) == EINVAL
+        assert l.ccnet_clip_grad_value(ptrs, q, n, 2, 0, 1.0, None) == EINVAL
+    assert l.ccnet_grad_norm(ptrs, neg, 2, 0, p, need, p, None) == EINVAL and l.ccnet_grad_norm_workspace_bytes(ptrs, neg, 2, 0) == 0
+    for m in (-1.0, float("nan")):
+        assert l.ccnet_clip_grad_norm(ptrs, ptrs, n, 2, 0, m, p, need, p, None) == EINVAL
+        assert l.ccnet_clip_grad_value(ptrs, ptrs, n, 2, 0, m, None) == EINVAL
+    assert l.ccnet_clip_grad_norm(ptrs, ptrs, n, 2, 0, 1.0, p, need - 1, p, None) == EWS
+
+
+def test_packed_attention_wrapper_refusals():
+    from ccnet_amd import ops
+    b = torch.zeros(4, 256, dtype=BF16)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(_err(), match="divide"):
+        ops._packed_operands(b, b, b, cu, 3, 2, 64)
+    for bad in (cu.long(), cu[None], cu[:0], torch.zeros(4, dtype=torch.int32)[::2]):
+        with pytest.raises(_err(), match="cu_seqlens"):
+            ops._packed_operands(b, b, b, bad, 4, 4, 64)
+    for q, k, v in ((b.float(), b, b), (b[:, :64], b, b), (b, b[:2], b), (b, b, b[:, ::2]), (b[0], b, b)):
+        with pytest.raises(_err()):
+            ops._packed_operands(q, k, v, cu, 4, 4, 64)
+    with pytest.raises(_err(), match="all of dq"):
+        ops.attention_packed_bwd(b, b, b, b, b, b, cu, 4, 4, 64, 1.0, dq=b)

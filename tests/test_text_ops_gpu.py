@@ -1,0 +1,559 @@
+"""Token lookup and its gradient, packed causal attention forward and backward, gradient norm and clipping: every kernel
+through its public entry point against the definition in 64 bits.  Tolerances count roundings: half a step of a value x is
+at most 2^-24 |x| in fp32 and 2^-8 |x| in bf16."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+H16, H32 = 2.0 ** -8, 2.0 ** -24  # half a step, relative
+
+
+def _ops():
+    from ccnet_amd import ops
+    return ops
+
+
+def _randn(*shape, seed=0, dtype=F32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype).cuda()
+
+
+def _within(got, ref, tol, what):
+    err = (got.double() - ref).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} outside, worst {float((err - tol).max()):.3g} over its bound"
+
+
+# ------------------------------------------------------------------ lookup
+@pytest.mark.parametrize("T", [0, 1, 3, 77, 1000])
+@pytest.mark.parametrize("C", [1, 7, 64, 320, 333, 1024, 1032])
+@pytest.mark.parametrize("tdt,odt", [(F32, BF16), (F32, F32), (BF16, BF16), (BF16, F32)])
+def test_lookup_is_one_rounding_of_the_scaled_row(cuda, T, C, tdt, odt):
+    ops = _ops()
+    table = _randn(50, C, seed=C, dtype=tdt)
+    g = torch.Generator().manual_seed(T)
+    ids = torch.randint(0, 50, (T,), generator=g).cuda()
+    for scale in (1.0, 22.627417):
+        got = ops.embedding(ids, table, scale=scale, dtype=odt)
+        assert got.dtype == odt and torch.equal(got, (table[ids].float() * scale).to(odt))
+    assert torch.equal(ops.embedding(ids.int(), table, dtype=odt), ops.embedding(ids, table, dtype=odt))
+
+
+def test_lookup_strides_shapes_and_ids_outside(cuda):
+    ops = _ops()
+    wide = _randn(40, 100, seed=1)
+    ids = torch.tensor([[0, 39, -1], [40, 7, 1 << 40]], device="cuda")
+    ref = wide[:, 4:68][ids.clamp(0, 39).reshape(-1)]
+    ref[[2, 3, 5]] = 0
+    for off in (4, 3):  # 16-byte aligned columns, and columns aligned to the element only
+        ref = wide[:, off:off + 64][ids.clamp(0, 39).reshape(-1)]
+        ref[[2, 3, 5]] = 0
+        assert torch.equal(ops.embedding(ids, wide[:, off:off + 64], dtype=F32), ref)
+        assert torch.equal(ops.embedding(ids.t(), wide[:, off:off + 64], dtype=F32), ref[[0, 3, 1, 4, 2, 5]])
+    buf = torch.full((6, 80), 5.0, device="cuda")
+    ops.embedding(ids, wide[:, :64], out=buf[:, 8:72])
+    assert torch.equal(buf[:, 8:72], torch.where(torch.tensor([1, 1, 0, 0, 1, 0], device="cuda")[:, None] > 0, wide[ids.clamp(0, 39).reshape(-1), :64], 0.0))
+    assert (buf[:, :8] == 5).all() and (buf[:, 72:] == 5).all()
+    ids32 = torch.tensor([0, -1, 50, -(1 << 31), 39], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.embedding(ids32, wide, dtype=F32)[[1, 2, 3]], torch.zeros(3, 100, device="cuda"))
+
+
+# ------------------------------------------------------------------ its gradient
+def _grad_ref(ids, dy, vocab, scale, padding=None):
+    ok = (ids >= 0) & (ids < vocab)
+    if padding is not None:
+        ok &= ids != padding
+    ref = torch.zeros(vocab, dy.shape[1], dtype=F64, device="cuda")
+    mag, count = torch.zeros_like(ref), torch.zeros(vocab, dtype=F64, device="cuda")
+    ref.index_add_(0, ids[ok].long(), dy[ok].double())
+    mag.index_add_(0, ids[ok].long(), dy[ok].double().abs())
+    count.index_add_(0, ids[ok].long(), torch.ones(int(ok.sum()), dtype=F64, device="cuda"))
+    # a sum of n terms in any tree: at most n - 1 roundings of partial sums, none above the sum of magnitudes (the tree of
+    # long runs is shallower than 512); then one rounding of the product with the scale
+    return ref * scale, (count.clamp(max=512)[:, None] * H32 * mag + 2 * H32 * ref.abs()) * scale
+
+
+def _ids_of(kind, T, vocab, seed):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, vocab, (T,), generator=g)
+    if kind == "one":
+        ids[:] = vocab // 2
+    elif kind == "mostly":
+        ids[torch.rand(T, generator=g) < 0.8] = vocab - 1
+    elif kind == "two":
+        ids = torch.where(torch.arange(T) % 3 == 0, 0, vocab - 1)
+    return ids.cuda()
+
+
+@pytest.mark.parametrize("T,vocab,C", [(0, 5, 8), (1, 1, 1), (1, 300000, 8), (63, 2, 64), (64, 17, 333), (65, 1000, 1024), (97, 3, 520),
+                                       (511, 17, 40), (512, 1, 512), (513, 2, 1032), (2464, 49408, 64), (8192, 1000, 24),
+                                       (8193, 1000, 24), (8192, 262143, 8), (5000, 262144, 8), (20000, 70000, 16), (50001, 255, 72),
+                                       (12289, 256, 9)])
+@pytest.mark.parametrize("kind", ["uniform", "one", "mostly", "two"])
+def test_table_gradient(cuda, T, vocab, C, kind):
+    ops = _ops()
+    ids = _ids_of(kind, T, vocab, T + vocab)
+    for dt in (F32, BF16):
+        dy = _randn(T, C, seed=C, dtype=dt)
+        ref, tol = _grad_ref(ids, dy, vocab, 22.0)
+        got = ops.embedding_grad(ids, dy, vocab, scale=22.0)
+        assert got.dtype == F32 and got.shape == (vocab, C)
+        _within(got, ref, tol, f"T {T} vocab {vocab} C {C} {kind} {dt}")
+        assert torch.equal(got, ops.embedding_grad(ids.int(), dy, vocab, scale=22.0)), "the sum's order depends on something else"
+
+
+def test_table_gradient_padding_and_ids_outside(cuda):
+    ops = _ops()
+    for T in (300, 9000):
+        ids = _ids_of("mostly", T, 20, 3)
+        ids[::7] = -1
+        ids[1::7] = 20
+        ids[2::7] = 1 << 33
+        dy = _randn(T, 96, seed=4, dtype=BF16)
+        ref, tol = _grad_ref(ids, dy, 20, 1.0, padding=19)
+        got = ops.embedding_grad(ids, dy, 20, padding_idx=19)
+        _within(got, ref, tol, "padding")
+        assert (got[19] == 0).all()
+        dy[ids == 19] = float("nan")  # what takes no part does not count, whatever it holds
+        dy[ids < 0] = float("inf")
+        assert torch.equal(got, ops.embedding_grad(ids, dy, 20, padding_idx=19))
+
+
+def test_table_gradient_accumulates_and_leaves_other_rows(cuda):
+    ops = _ops()
+    ids = torch.tensor([3, 3, 9, 3], device="cuda")
+    dy = _randn(4, 50, seed=1)
+    base = _randn(12, 64, seed=2)
+    out = base.clone()
+    r = ops.embedding_grad(ids, dy, 12, scale=0.5, out=out[:, 7:57], accumulate=True)
+    assert r.data_ptr() == out[:, 7:57].data_ptr()
+    ref, tol = _grad_ref(ids, dy, 12, 0.5)
+    want = base.double()
+    want[:, 7:57] += ref
+    _within(out[:, 7:57], want[:, 7:57], tol + H32 * want[:, 7:57].abs() * 2, "accumulate")
+    keep = torch.ones(12, dtype=torch.bool)
+    keep[[3, 9]] = False
+    assert torch.equal(out[keep], base[keep]) and torch.equal(out[:, :7], base[:, :7]) and torch.equal(out[:, 57:], base[:, 57:])
+    same = out.clone()
+    ops.embedding_grad(ids[:0], dy[:0], 12, out=out[:, 7:57], accumulate=True)
+    assert torch.equal(out, same)
+
+
+def test_table_gradient_in_strided_memory(cuda):
+    ops = _ops()
+    ids = _ids_of("uniform", 500, 33, 1)
+    wide = _randn(500, 200, seed=2, dtype=BF16)
+    for off, C in ((8, 64), (3, 64), (8, 65)):
+        dy = wide[:, off:off + C]
+        ref, tol = _grad_ref(ids, dy, 33, 1.0)
+        buf = torch.full((33, 160), 2.0, device="cuda")
+        ops.embedding_grad(ids, dy, 33, out=buf[:, off:off + C])
+        _within(buf[:, off:off + C], ref, tol, "strided")
+        assert (buf[:, :off] == 2).all() and (buf[:, off + C:] == 2).all()
+
+
+def test_table_gradient_against_differences(cuda):
+    ops = _ops()
+    ids = _ids_of("mostly", 200, 11, 5)
+    dy = _randn(200, 24, seed=6)
+    grad = ops.embedding_grad(ids, dy, 11, scale=3.0).double()
+    w, u = _randn(11, 24, seed=7, dtype=F64), _randn(11, 24, seed=8, dtype=F64)
+    loss = lambda t: float((3.0 * t[ids] * dy.double()).sum())  # noqa: E731
+    slope = (loss(w + u) - loss(w - u)) / 2  # linear: the difference is the derivative
+    _, tol = _grad_ref(ids, dy, 11, 3.0)
+    assert abs(float((grad * u).sum()) - slope) <= float((tol * u.abs()).sum()) + 1e-9 * abs(slope)
+
+
+# ------------------------------------------------------------------ packed causal attention
+def _packed_inputs(lens, H, Hkv, d, pad=0, seed=0, gap=0):
+    rows = sum(lens) + pad
+    qkv = _randn(rows, (H + 2 * Hkv) * d + gap, seed=seed, dtype=BF16)
+    q, k, v = qkv[:, :H * d], qkv[:, H * d:(H + Hkv) * d], qkv[:, (H + Hkv) * d:(H + 2 * Hkv) * d]
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)) if lens else [0], dtype=torch.int32).cuda()
+    return q, k, v, _randn(rows, H * d, seed=seed + 1, dtype=BF16), cu
+
+
+def _attention_ref(q, k, v, do, lens, H, Hkv, d, scale):
+    """Outputs, log2-sum-exp and gradients by the formulas in 64 bits, each with its bound.  Roundings: P (2^-8 relative), the
+    output; in the backward P, dS, the forward's output inside delta, and the result.  2^-10 covers the fp32 scores and
+    exponentials (128 products of at most 2^-24 of the sum of magnitudes, which is below 2^9 here)."""
+    rows, G = q.shape[0], H // Hkv
+    z = lambda h: torch.zeros(rows, h * d, dtype=F64, device="cuda")  # noqa: E731
+    o, to, dq, tq, dk, tk, dv, tv = z(H), z(H), z(H), z(H), z(Hkv), z(Hkv), z(Hkv), z(Hkv)
+    lse = torch.full((H, rows), -math.inf, dtype=F64, device="cuda")
+    first = 0
+    for n in lens:
+        r = slice(first, first + n)
+        first += n
+        future = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)
+        for h in range(H):
+            a, b = slice(h * d, h * d + d), slice(h // G * d, h // G * d + d)
+            Q, K, V, D = (x[r, c].double() for x, c in ((q, a), (k, b), (v, b), (do, a)))
+            s = (scale * Q @ K.T).masked_fill(future, -math.inf)
+            lse[h, r] = torch.logsumexp(s, 1) / math.log(2)
+            p = torch.softmax(s, 1)
+            O = p @ V
+            o[r, a] = O
+            near = (H16 + 2.0 ** -10) * (p @ V.abs())
+            to[r, a] = near + H16 * (O.abs() + near)
+            dp = D @ V.T
+            delta = (D * O).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            eds = (H16 + 2.0 ** -10) * ds.abs() + p * (D.abs() * to[r, a]).sum(1, keepdim=True) + 2.0 ** -10 * p * (dp.abs() + delta.abs())
+            dq[r, a] = scale * ds @ K
+            tq[r, a] = scale * eds @ K.abs()
+            dk[r, b] += scale * ds.T @ Q
+            tk[r, b] += scale * eds.T @ Q.abs()
+            dv[r, b] += p.T @ D
+            tv[r, b] += (H16 + 2.0 ** -9) * p.T @ D.abs()
+    out = {"o": (o, to), "lse": (lse, None)}
+    for name, x, t in (("dq", dq, tq), ("dk", dk, tk), ("dv", dv, tv)):
+        out[name] = (x, t + H16 * (x.abs() + t))
+    return out
+
+
+def _check_attention(got, ref, what):
+    for name in ("o", "dq", "dk", "dv"):
+        x, t = ref[name]
+        _within(got[name], x, t, f"{what} {name}")
+        # the worst case above adds magnitudes; of independent roundings (rms 2^-8 / sqrt 3 each, at most four in a row) the root
+        # of the summed squares stays below 2^-7 of the result
+        if x.norm() > 0 and x.shape[0] > 8:
+            rel = float((got[name].double() - x).norm() / x.norm())
+            assert rel <= 2.0 ** -7, f"{what} {name}: relative error {rel:.3g}"
+    fin = ref["lse"][0] > -math.inf
+    assert torch.equal(fin, got["lse"] > -math.inf)
+    _within(got["lse"][fin], ref["lse"][0][fin], 2.0 ** -10 + 2.0 ** -20 * ref["lse"][0][fin].abs(), f"{what} lse")
+
+
+def _run_attention(q, k, v, do, cu, H, Hkv, d, scale):
+    ops = _ops()
+    o, lse = ops.attention_packed(q, k, v, cu, H, Hkv, d, scale, with_lse=True)
+    dq, dk, dv = ops.attention_packed_bwd(q, k, v, o, do, lse, cu, H, Hkv, d, scale)
+    return {"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+LENS = [(1,), (2,), (31,), (32,), (33,), (77,), (63, 64, 65), (127, 128, 129), (0, 5, 0, 0, 77, 0), (256,), (257, 300), (511, 3, 640),
+        tuple(range(1, 78)), (1,) * 130]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: f"{len(x)}x{max(x)}")
+def test_packed_attention(cuda, lens, d):
+    for H, Hkv in ((1, 1), (6, 2)):
+        q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=sum(lens) + d + H)
+        scale = d ** -0.5
+        got = _run_attention(q, k, v, do, cu, H, Hkv, d, scale)
+        _check_attention(got, _attention_ref(q, k, v, do, lens, H, Hkv, d, scale), f"{H}/{Hkv}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(8, 8), (16, 8), (32, 8), (5, 5), (4, 1), (24, 8), (16, 16)])
+def test_packed_attention_head_layouts(cuda, H, Hkv, d):
+    lens = (40, 150, 1, 77)
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, pad=9, seed=H + d, gap=24)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.2)
+    _check_attention(got, _attention_ref(q, k, v, do, lens, H, Hkv, d, 0.2), f"{H}/{Hkv}")
+    for name in ("o", "dq", "dk", "dv"):
+        assert (got[name][sum(lens):] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_without_sequences_or_rows(cuda, d):
+    q, k, v, do, cu = _packed_inputs((), 2, 1, d, pad=70)
+    for offsets in (cu, torch.zeros(4, dtype=torch.int32, device="cuda")):
+        got = _run_attention(q, k, v, do, offsets, 2, 1, d, 0.1)
+        for name in ("o", "dq", "dk", "dv"):
+            assert (got[name] == 0).all()
+    got = _run_attention(q[:0], k[:0], v[:0], do[:0], cu, 2, 1, d, 0.1)
+    assert got["o"].shape == (0, 2 * d)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_behind_the_last_sequence(cuda, d):
+    ops = _ops()
+    lens, H, Hkv = (70, 33), 4, 2
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, pad=141, seed=3)
+    n = sum(lens)
+    clean = _run_attention(q[:n], k[:n], v[:n], do[:n], cu, H, Hkv, d, 0.1)
+    for t in (q, k, v, do):
+        t[n:] = float("nan")
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    for name in ("o", "dq", "dk", "dv"):
+        assert torch.equal(got[name][:n], clean[name]) and (got[name][n:] == 0).all(), name
+    o = torch.full((n + 141, H * d), 7.0, dtype=BF16, device="cuda")
+    both = torch.full((n + 141, (H + 2 * Hkv) * d), 7.0, dtype=BF16, device="cuda")
+    ops.attention_packed(q, k, v, cu, H, Hkv, d, 0.1, out=o)
+    dq, dk, dv = both[:, :H * d], both[:, H * d:(H + Hkv) * d], both[:, (H + Hkv) * d:]
+    ops.attention_packed_bwd(q, k, v, got["o"], do, got["lse"], cu, H, Hkv, d, 0.1, dq=dq, dk=dk, dv=dv)
+    for t, name in ((o, "o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
+        assert torch.equal(t[:n], clean[name]) and (t[n:] == 7).all(), name
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [50, 300])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_values_that_are_not_finite_reach_only_who_sees_them(cuda, d, n, value):
+    lens, H, Hkv = (20, n, 45), 2, 1
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=n)
+    clean = _ops().attention_packed(q, k, v, cu, H, Hkv, d, 0.1)
+    for at in (0, 5, 31, 32, n - 1):
+        for which in ("k", "v"):
+            k2, v2 = k.clone(), v.clone()
+            (k2 if which == "k" else v2)[20 + at, 3:6] = value
+            got = _ops().attention_packed(q, k2, v2, cu, H, Hkv, d, 0.1)
+            before = torch.ones(sum(lens), dtype=torch.bool)
+            before[20 + at:20 + n] = False
+            assert torch.equal(got[before], clean[before]), (which, at)
+            if which == "v":  # every query that sees it has it, in its channels only
+                after, cols = got[20 + at:20 + n].reshape(n - at, H, d), [3, 4, 5]
+                rest = [c for c in range(d) if c not in cols]
+                assert torch.equal(after[:, :, rest], clean[20 + at:20 + n].reshape(n - at, H, d)[:, :, rest])
+                if math.isnan(value):
+                    assert after[:, :, cols].isnan().all()
+                else:  # (a probability that rounds to zero makes a NaN of it)
+                    assert ((after[:, :, cols] == value) | after[:, :, cols].isnan()).all()
+    k2, v2 = k.clone(), v.clone()
+    k2[20:20 + n], v2[20:20 + n] = value, value
+    got = _run_attention(q, k2, v2, do, cu, H, Hkv, d, 0.1)
+    ref = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    for name in ("o", "dq", "dk", "dv"):  # no other sequence notices, in any gradient
+        assert torch.equal(got[name][:20], ref[name][:20]) and torch.equal(got[name][20 + n:], ref[name][20 + n:]), name
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_scores_of_any_size(cuda, d):
+    """Scores far below and above zero, rising along the keys (the running maximum grows all the way) and falling."""
+    n, H = 200, 1
+    for sign, big in ((1, 8.0), (-1, 8.0), (1, 3e4), (-1, 3e4)):
+        q = torch.zeros(n, d, dtype=BF16, device="cuda")
+        k = torch.zeros(n, d, dtype=BF16, device="cuda")
+        q[:, 0] = sign
+        k[:, 0] = (torch.arange(n, device="cuda") * big).to(BF16)
+        v, do = _randn(n, d, seed=1, dtype=BF16), _randn(n, d, seed=2, dtype=BF16)
+        cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        got = _run_attention(q, k, v, do, cu, H, H, d, 1.0)
+        ref = _attention_ref(q, k, v, do, (n,), H, H, d, 1.0)
+        # a score of 2^22 is known to 2^-24 of it: exponents off by 0.25 at most where big = 3e4, where one key takes all
+        _within(got["o"], ref["o"][0], ref["o"][1] + (0 if big < 1e3 else 1e-6), f"{sign} {big}")
+        assert all(torch.isfinite(got[x]).all() for x in ("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_gradients_against_differences(cuda, d):
+    lens, H, Hkv, scale = (45, 70), 2, 1, 0.15
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=11)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, scale)
+    ref = _attention_ref(q, k, v, do, lens, H, Hkv, d, scale)
+
+    def loss(q, k, v):
+        return float((_attention_ref(q, k, v, do, lens, H, Hkv, d, scale)["o"][0] * do.double()).sum())
+
+    args = {"dq": q.double(), "dk": k.double(), "dv": v.double()}
+    for i, name in enumerate(args):
+        u, eps = _randn(*args[name].shape, seed=20 + i, dtype=F64), 1e-4
+        up = [a + eps * u if n == name else a for n, a in args.items()]
+        dn = [a - eps * u if n == name else a for n, a in args.items()]
+        slope = (loss(*up) - loss(*dn)) / (2 * eps)
+        have = float((got[name].double() * u).sum())
+        assert abs(have - slope) <= float((ref[name][1] * u.abs()).sum()) + 1e-5 * abs(slope)
+        # and much nearer than that bound, which adds magnitudes: the errors' signs are independent
+        near = float((ref[name][1] * u).square().sum().sqrt()) * 4
+        assert abs(have - slope) <= near + 1e-5 * abs(slope), (name, have, slope, near)
+
+
+def test_packed_attention_repeats_bit_for_bit(cuda):
+    lens = (300, 7, 129, 64)
+    q, k, v, do, cu = _packed_inputs(lens, 8, 2, 64, seed=5)
+    a, b = (_run_attention(q, k, v, do, cu, 8, 2, 64, 0.1) for _ in range(2))
+    assert all(torch.equal(a[x], b[x]) for x in a)
+
+
+def test_packed_attention_rows_past_two_gigabytes(cuda):
+    """Row offsets of more than 2^31 bytes, and a sequence that begins behind them."""
+    rows, ld, d = 70000, 16384, 64
+    big = torch.zeros(rows, ld, dtype=BF16, device="cuda")
+    lens = (69000, 600, 400)
+    small = _randn(1000, 3 * d, seed=9, dtype=BF16)
+    big[69000:, 16000:16000 + 3 * d] = small
+    q, k, v = (big[:, 16000 + i * d:16000 + (i + 1) * d] for i in range(3))
+    assert 69000 * ld * 2 > 1 << 31
+    cu = torch.tensor([0, 69000, 69600, 70000], dtype=torch.int32, device="cuda")
+    do = torch.zeros(rows, d, dtype=BF16, device="cuda")
+    do[69000:] = _randn(1000, d, seed=10, dtype=BF16)
+    got = _run_attention(q, k, v, do, cu, 1, 1, d, 0.125)
+    alone = _run_attention(small[:, :d], small[:, d:2 * d], small[:, 2 * d:], do[69000:], cu[1:] - 69000, 1, 1, d, 0.125)
+    for name in ("o", "dq", "dk", "dv"):
+        assert torch.equal(got[name][69000:], alone[name]), name
+    assert (got["o"][:69000] == 0).all() and torch.equal(got["lse"][:, 69000:], alone["lse"])
+    del lens
+
+
+def test_packed_attention_offsets_that_are_wrong_stay_inside(cuda):
+    """Offsets are clamped to the rows and to rising order by the kernel: such calls give rows of no meaning, no access outside."""
+    q, k, v, do, _ = _packed_inputs((100,), 2, 2, 64, seed=1)
+    ref = _run_attention(q, k, v, do, torch.tensor([0, 100], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
+    got = _run_attention(q, k, v, do, torch.tensor([0, 5000], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
+    assert all(torch.equal(got[x], ref[x]) for x in ref)
+    got = _run_attention(q, k, v, do, torch.tensor([0, 100, 40], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
+    assert torch.isfinite(got["o"]).all()
+
+
+def test_packed_attention_in_a_graph_serves_other_lengths(cuda):
+    H, Hkv, d = 4, 2, 64
+    q, k, v, do, cu = _packed_inputs((60, 40, 100), H, Hkv, d, seed=6)
+    _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    for lens in ((60, 40, 100), (1, 198, 1), (0, 0, 200), (10, 20, 30), (60, 40, 100)):
+        cu.copy_(torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32))
+        q.copy_(_randn(*q.shape, seed=sum(lens), dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+        assert all(torch.equal(got[x], ref[x]) for x in ref), lens
+
+
+# ------------------------------------------------------------------ gradient norm and clipping
+SIZES = [0, 1, 2, 3, 4, 5, 7, 8, 9, 255, 1000, 4096, 32768 * 4 + 3, 1, 0]
+
+
+def _grads(dtype, seed=0, scale=1.0, odd=True):
+    flat = _randn(sum(SIZES) + 64, seed=seed, dtype=dtype, scale=scale)
+    out, at = [], 1 if odd else 0
+    for n in SIZES:
+        out.append(flat[at:at + n])
+        at += n
+        if not odd:
+            at = -(-at // 8) * 8
+    return flat, out
+
+
+def _norm64(grads):
+    return math.sqrt(math.fsum(float(g.double().square().sum()) for g in grads))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("odd", [True, False])
+@pytest.mark.parametrize("max_norm", [0.0, 0.5, 1e3, 1e9])
+def test_clip_by_norm(cuda, dtype, odd, max_norm):
+    ops = _ops()
+    flat, grads = _grads(dtype, odd=odd)
+    before = flat.clone()
+    copies = [g.clone() for g in grads]
+    norm = _norm64(grads)
+    assert abs(float(ops.grad_norm(grads)) - norm) <= 2 * H32 * norm
+    outs = [torch.full_like(g, 9.0) for g in grads]
+    got = ops.clip_grad_norm(grads, max_norm, out=outs)
+    assert got.dtype == F32 and got.dim() == 0 and abs(float(got) - norm) <= 2 * H32 * norm
+    assert torch.equal(flat, before)  # `out`: the gradients stay
+    got = ops.clip_grad_norm(grads, max_norm)
+    factor = min(1.0, max_norm / (norm + 1e-6))
+    for g, o, c in zip(grads, outs, copies):
+        assert torch.equal(g, o)
+        # the factor's rounding and the product's (bf16: the product's to fp32 too)
+        _within(g, c.double() * factor, c.double().abs() * factor * (H16 + 4 * H32 if dtype == BF16 else 4 * H32), "clipped")
+    if factor == 1.0:
+        assert torch.equal(flat, before)
+    inside = torch.zeros_like(flat, dtype=torch.bool)
+    for g in grads:
+        inside[g.storage_offset():g.storage_offset() + g.numel()] = True
+    assert torch.equal(flat[~inside], before[~inside])  # nothing between and behind the tensors
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_clip_by_value(cuda, dtype):
+    ops = _ops()
+    flat, grads = _grads(dtype)
+    flat[40:44] = torch.tensor([float("nan"), float("inf"), float("-inf"), 0.25])
+    want = [g.clamp(-0.25, 0.25) for g in grads]
+    outs = [torch.empty_like(g) for g in grads]
+    ops.clip_grad_value(grads, 0.25, out=outs)
+    ops.clip_grad_value(grads, 0.25)
+    for g, o, w in zip(grads, outs, want):
+        assert torch.equal(g.nan_to_num(7), w.nan_to_num(7)) and torch.equal(o.nan_to_num(7), w.nan_to_num(7))
+        assert torch.equal(g.isnan(), w.isnan())
+
+
+def test_norm_of_many_tensors_and_of_any_size(cuda):
+    ops = _ops()
+    many = [_randn(1 + i % 37, seed=i) for i in range(401)]
+    norm = _norm64(many)
+    assert abs(float(ops.grad_norm(many)) - norm) <= 2 * H32 * norm
+    assert abs(float(ops.clip_grad_norm(many, norm / 2)) - norm) <= 2 * H32 * norm
+    assert abs(_norm64(many) - norm / 2) <= 1e-5 * norm
+    for scale in (1e30, 1e-30, 1e-42):  # squares that leave the range of fp32
+        g = [_randn(1000, seed=1, scale=scale), _randn(33, seed=2, scale=scale)]
+        norm = _norm64(g)
+        assert abs(float(ops.grad_norm(g)) - norm) <= 2 * H32 * norm + 2.0 ** -149
+    assert float(ops.grad_norm([torch.zeros(0, device="cuda"), torch.zeros(3, device="cuda")])) == 0.0
+    assert float(ops.grad_norm([torch.zeros(0, device="cuda")])) == 0.0
+    g = torch.ones(5, device="cuda")
+    assert abs(float(ops.grad_norm([g, g])) - math.sqrt(10)) <= 1e-6  # reading one tensor twice is no race
+
+
+def test_dense_tensors_in_any_order_of_dimensions(cuda):
+    ops = _ops()
+    base = _randn(6, 5, 3, 4, seed=1)
+    g = base.permute(0, 3, 1, 2)
+    want = base.double() * (1.0 / (float(base.double().norm()) + 1e-6))
+    ops.clip_grad_norm([g], 1.0)
+    _within(base, want, want.abs() * 4 * H32, "permuted")
+    out = torch.empty(6, 5, 3, 4, device="cuda").permute(0, 3, 1, 2)
+    ops.clip_grad_norm([g], 0.5, out=[out])
+    _within(out, g.double() * (0.5 / (float(g.double().norm()) + 1e-6)), g.double().abs() * 4 * H32, "permuted out")
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_a_norm_that_is_not_finite_scales_nothing(cuda, value):
+    ops = _ops()
+    flat, grads = _grads(F32)
+    flat[1000] = value
+    before = flat.clone()
+    norm = ops.clip_grad_norm(grads, 1.0)
+    assert not math.isfinite(float(norm)) and math.isnan(float(norm)) == math.isnan(value)
+    assert torch.equal(flat.nan_to_num(7), before.nan_to_num(7))
+
+
+def test_clip_in_a_graph(cuda):
+    ops = _ops()
+    flat, grads = _grads(F32, odd=False)
+    outs = [torch.empty_like(g) for g in grads]
+    ops.clip_grad_norm(grads, 1.0, out=outs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grad_norm(grads, 1.0, out=outs)
+    for seed in (3, 4, 5):
+        flat.copy_(_randn(flat.numel(), seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        ref = ops.clip_grad_norm(grads, 1.0, out=outs)
+        assert torch.equal(norm, ref) and all(torch.equal(a, b) for a, b in zip(got, outs))
+
+
+# ------------------------------------------------------------------ streams and devices
+def test_text_ops_on_another_stream(cuda):
+    ops = _ops()
+    ids = _ids_of("mostly", 9000, 500, 1)
+    dy = _randn(9000, 64, seed=1, dtype=BF16)
+    q, k, v, do, cu = _packed_inputs((300, 77), 4, 4, 64, seed=2)
+    grads = [_randn(100000, seed=3), _randn(77, seed=4)]
+    want = (ops.embedding_grad(ids, dy, 500), _run_attention(q, k, v, do, cu, 4, 4, 64, 0.1), ops.grad_norm(grads))
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):  # two streams at once, each with workspaces of its own
+        for st in s:
+            with torch.cuda.stream(st):
+                got.append((ops.embedding_grad(ids, dy, 500), _run_attention(q, k, v, do, cu, 4, 4, 64, 0.1), ops.grad_norm(grads)))
+    torch.cuda.synchronize()
+    for g in got:
+        assert torch.equal(g[0], want[0]) and all(torch.equal(g[1][x], want[1][x]) for x in want[1]) and torch.equal(g[2], want[2])

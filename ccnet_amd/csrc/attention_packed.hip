@@ -18,6 +18,7 @@
 // reads: 16-byte chunk c of row r lies at chunk c ^ swz(r), swz spreading 8 consecutive rows' 64-byte spans as well as 16
 // consecutive rows' single chunks evenly over the 64 banks.
 #include "common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -35,6 +36,9 @@ struct PackedArgs {
     int zero_tail;  // rows behind the last sequence: 1 = written as zeros, 0 = left as they are
     float* lse;     // [H][rows]
     float* delta;   // [H][rows]
+    __bf16* o_low;  // [rows][H d]: what the rounding of O took away
+    int parts;      // dK / dV: workgroups that share a key tile's walk, each with H / Hkv / parts query heads
+    float* part;    // parts > 1: [parts][2][rows][Hkv d] sums of dK (not scaled yet) and dV
 };
 
 template <int D>
@@ -244,22 +248,35 @@ __device__ __forceinline__ void settle(bf16x8 (&f)[N]) {
 
 // a lane's row of an accumulator (register e of block d: channel 32 d + (e & 3) + 8 (e >> 2) + 4 hh) as 16-byte stores: the
 // swap of packed quads between the lane halves leaves 8 consecutive channels in each
+__device__ __forceinline__ u32x4 swap_quads(const unsigned (&p)[4]) {
+    u32x4 v;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(p[w], p[2 + w], false, false);
+        v[w] = sw[0];
+        v[2 + w] = sw[1];
+    }
+    return v;
+}
 template <int D>
-__device__ __forceinline__ void store_row(__bf16* row, const f32x16* o, float mul, int hh, bool ok) {
+__device__ __forceinline__ void store_row(__bf16* row, __bf16* low_row, const f32x16* o, float mul, int hh, bool ok) {
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int qp = 0; qp < 2; ++qp) {
-            u32x4 v;
+            unsigned hi[4], lo[4];
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const unsigned e0 = pack_bf16x2(o[d][8 * qp + 2 * w] * mul, o[d][8 * qp + 2 * w + 1] * mul);
-                const unsigned e1 = pack_bf16x2(o[d][8 * qp + 4 + 2 * w] * mul, o[d][8 * qp + 4 + 2 * w + 1] * mul);
-                const auto sw = __builtin_amdgcn_permlane32_swap(e0, e1, false, false);
-                v[w] = sw[0];
-                v[2 + w] = sw[1];
+            for (int w = 0; w < 4; ++w) {
+                const float a = o[d][8 * qp + 2 * w] * mul, b = o[d][8 * qp + 2 * w + 1] * mul;
+                hi[w] = pack_bf16x2(a, b);
+                lo[w] = pack_bf16x2(a - __uint_as_float(hi[w] << 16), b - __uint_as_float(hi[w] & 0xffff0000u));
             }
+            const u32x4 v = swap_quads(hi);
             if (ok) *(u32x4*)(row + d * 32 + 16 * qp + 8 * hh) = v;
+            if (low_row) {
+                const u32x4 r = swap_quads(lo);
+                if (ok) *(u32x4*)(low_row + d * 32 + 16 * qp + 8 * hh) = r;
+            }
         }
 }
 
@@ -465,7 +482,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
         const bool ok = q < tl.len;
         const float l = half_sum(l_run[X]);
         if (a.lse && hh == 0 && ok) a.lse[(long long)h * a.rows + tl.start + q] = tl.tail ? -INFINITY : m_run[X] + __builtin_amdgcn_logf(l);
-        store_row<D>(a.out + (long long)(tl.start + (ok ? q : 0)) * a.ldo + h * D, o[X], tl.tail ? 0.f : 1.0f / l, hh, ok);
+        const long long row = tl.start + (ok ? q : 0);
+        store_row<D>(a.out + row * a.ldo + h * D, a.o_low ? a.o_low + (row * a.H + h) * D : nullptr, o[X], tl.tail ? 0.f : 1.0f / l, hh, ok);
     }
 }
 
@@ -498,11 +516,14 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         for (int ks = 0; ks < NK; ++ks) {
             u32x4 ov = {0u, 0u, 0u, 0u};
             if (qok) ov = *(const u32x4*)(a.O + row * a.ldo + h * D + ks * 16 + hh * 8);
-            float x[8], y[8];
+            u32x4 lv = {0u, 0u, 0u, 0u};
+            if (qok && a.o_low) lv = *(const u32x4*)(a.o_low + (row * a.H + h) * D + ks * 16 + hh * 8);
+            float x[8], l[8], y[8];
             unpack8(ov, x);
+            unpack8(lv, l);
             unpack8(__builtin_bit_cast(u32x4, dof[ks]), y);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dlt = fmaf(x[j], y[j], dlt);
+            for (int j = 0; j < 8; ++j) dlt = fmaf(x[j] + l[j], y[j], dlt);
         }
         dlt = half_sum(dlt);
         if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = dlt;
@@ -572,7 +593,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
             stage_fence();
         }
     }
-    store_row<D>(a.dQ + row * a.lddq + h * D, dq, a.scale, hh, qok);
+    store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, qok);
 }
 
 // ------------------------------------------------------------------ backward: dK, dV
@@ -585,8 +606,10 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
-    if (!find_tile(a, blockIdx.x / a.Hkv, BM, true, tl)) return;
-    const int kvh = blockIdx.x % a.Hkv, G = a.H / a.Hkv;
+    const int units = a.Hkv * a.parts;
+    if (!find_tile(a, blockIdx.x / units, BM, true, tl)) return;
+    const int kvh = blockIdx.x % a.Hkv, part = blockIdx.x % units / a.Hkv, G = a.H / a.Hkv / a.parts, h0 = (kvh * a.parts + part) * G;
+    if (a.parts > 1 && tl.tail) return;  // (packed_join_kernel's)
     const int k0 = tl.tile * BM + wave * 32, key = k0 + l31;
     const bool kok = key < tl.len;
     const long long row = tl.start + (kok ? key : 0);
@@ -606,7 +629,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
         const unsigned lds0 = lds_addr(smem);
         const int t0 = tl.tile * BM / PA_TILE, per_head = (tl.len + PA_TILE - 1) / PA_TILE - t0;
         auto issue = [&](int i) {  // step i of the walk: head i / per_head of the group, query tile t0 + i % per_head
-            const int g = i / per_head, t = t0 + i - g * per_head, h = kvh * G + g;
+            const int g = i / per_head, t = t0 + i - g * per_head, h = h0 + g;
             const long long r0 = (long long)tl.start + t * PA_TILE;
             const int left = min(tl.len - t * PA_TILE, PA_TILE);
             const unsigned st = lds0 + (i & 1) * STAGEB;
@@ -678,8 +701,45 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
             stage_fence();
         }
     }
-    store_row<D>(a.dK + row * a.lddk + kvh * D, dk, a.scale, hh, kok);
-    store_row<D>(a.dV + row * a.lddv + kvh * D, dv, 1.0f, hh, kok);
+    if (a.parts > 1) {
+        if (!kok) return;
+        const long long w = (long long)a.Hkv * D, plane = a.rows * w;
+        float* p = a.part + 2 * part * plane + row * w + kvh * D + 4 * hh;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                *(f32x4*)(p + d * 32 + 8 * g) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+                *(f32x4*)(p + plane + d * 32 + 8 * g) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+            }
+        return;
+    }
+    store_row<D>(a.dK + row * a.lddk + kvh * D, nullptr, dk, a.scale, hh, kok);
+    store_row<D>(a.dV + row * a.lddv + kvh * D, nullptr, dv, 1.0f, hh, kok);
+}
+
+// dK and dV of the parts, in their order: a thread per 8 channels of a row and gradient
+__global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a, int width) {
+    const int end = min(max(a.cu[a.n_seq], 0), a.rows), chunks = width / 8;
+    const long long plane = (long long)a.rows * width, n = 2ll * a.rows * chunks;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const int c = (int)(i % chunks) * 8, which = (int)(i / chunks & 1);
+        const long long row = i / chunks >> 1;
+        float s[8] = {};
+        if (row < end) {
+            const float* p = a.part + which * plane + row * width + c;
+            for (int k = 0; k < a.parts; ++k, p += 2 * plane) {
+                const f32x4 x = *(const f32x4*)p, y = *(const f32x4*)(p + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { s[e] += x[e]; s[4 + e] += y[e]; }
+            }
+        } else if (!a.zero_tail) continue;
+        if (which == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] *= a.scale;
+        }
+        *(u32x4*)((which ? a.dV + row * a.lddv : a.dK + row * a.lddk) + c) = pack8(s);
+    }
 }
 
 // the most tiles of `step` rows that n_seq sequences (and the rows behind them) can have in `rows` rows
@@ -687,23 +747,41 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
     return ((long long)rows + (long long)(n_seq + tail) * (step - 1)) / step;
 }
 
+// Into how many parts the walk of a key tile over its group's query heads is cut.  One workgroup walks G heads x the queries
+// behind its keys; with few key heads and long sequences the longest of those walks outlasts the rest of the grid.  Parts cost
+// fp32 sums through memory (16 bytes a channel), so only walks of at least 8 tiles a head on average are cut, and only while the
+// grid has fewer than 2048 workgroups (four rounds of 512).
+int parts_of(int n_seq, int rows, int H, int Hkv) {
+    const int G = H / Hkv;
+    if (rows < 512ll * (n_seq > 0 ? n_seq : 1)) return 1;
+    int p = 1;
+    while (p < G && most_tiles(rows, n_seq, 128, 0) * Hkv * p < 2048) {
+        do ++p;
+        while (G % p);
+    }
+    return p;
+}
+size_t delta_bytes(int rows, int H) { return ((size_t)rows * H * 4 + 255) & ~(size_t)255; }
+
 bool row_ok(const void* p, int ld, int width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
 
 }  // namespace
 
 extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo,
                                            const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale,
-                                           int zero_tail, float* lse, void* stream) {
+                                           int zero_tail, float* lse, void* o_low, void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
     if (d != 64 && d != 128) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d)) return CCNET_EINVAL;
+    if ((uintptr_t)o_low & 15) return CCNET_EINVAL;
     if (ldk > (1 << 24) || ldv > (1 << 24)) return CCNET_EUNSUP;
     PackedArgs a{};
     a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.out = (__bf16*)O;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
     a.cu = cu_seqlens; a.n_seq = n_seq; a.rows = rows; a.H = H; a.Hkv = Hkv;
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f; a.zero_tail = zero_tail != 0; a.lse = lse;
+    a.o_low = (__bf16*)o_low;
     const bool wide = d == 64 && rows >= 256ll * n_seq;  // (mean length of at least 256: whole 256-query tiles are the rule)
     const long long grid = most_tiles(rows, n_seq, wide ? 256 : 128, a.zero_tail) * H;
     if (grid > 0x7fffffffLL) return CCNET_EUNSUP;
@@ -716,25 +794,37 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     return CCNET_OK;
 }
 
+extern "C" size_t ccnet_attention_packed_bwd_workspace_bytes(int n_seq, int rows, int H, int Hkv, int d) {
+    if (rows <= 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || (d != 64 && d != 128)) return 0;
+    const int parts = parts_of(n_seq, rows, H, Hkv);
+    return delta_bytes(rows, H) + (parts > 1 ? (size_t)parts * 2 * rows * Hkv * d * 4 : 0);
+}
+
 extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, const void* O,
-                                               int ldo, const void* dO, int lddo, const float* lse, float* delta, void* dQ, int lddq,
+                                               int ldo, const void* o_low, const void* dO, int lddo, const float* lse, void* dQ, int lddq,
                                                void* dK, int lddk, void* dV, int lddv, const int32_t* cu_seqlens, int n_seq, int rows,
-                                               int H, int Hkv, int d, float scale, int zero_tail, void* stream) {
+                                               int H, int Hkv, int d, float scale, int zero_tail, void* workspace, size_t workspace_bytes,
+                                               void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
     if (d != 64 && d != 128) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
-    if (!cu_seqlens || !lse || !delta || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) ||
-        !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) || !row_ok(dQ, lddq, H * d) || !row_ok(dK, lddk, Hkv * d) ||
-        !row_ok(dV, lddv, Hkv * d))
+    if (!cu_seqlens || !lse || !workspace || ((uintptr_t)workspace & 15) || ((uintptr_t)o_low & 15) || !row_ok(Q, ldq, H * d) ||
+        !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) ||
+        !row_ok(dQ, lddq, H * d) || !row_ok(dK, lddk, Hkv * d) || !row_ok(dV, lddv, Hkv * d))
         return CCNET_EINVAL;
     if (ldq > (1 << 24) || ldk > (1 << 24) || ldv > (1 << 24) || lddo > (1 << 24)) return CCNET_EUNSUP;
+    if (workspace_bytes < ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d)) return CCNET_EWS;
     PackedArgs a{};
     a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.O = (const __bf16*)O; a.dO = (const __bf16*)dO;
+    a.o_low = (__bf16*)o_low;
     a.dQ = (__bf16*)dQ; a.dK = (__bf16*)dK; a.dV = (__bf16*)dV;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo; a.lddo = lddo; a.lddq = lddq; a.lddk = lddk; a.lddv = lddv;
     a.cu = cu_seqlens; a.n_seq = n_seq; a.rows = rows; a.H = H; a.Hkv = Hkv;
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f; a.zero_tail = zero_tail != 0;
-    a.lse = (float*)lse; a.delta = delta;
+    a.lse = (float*)lse;
+    a.delta = (float*)workspace;
+    a.part = (float*)((char*)workspace + delta_bytes(rows, H));
+    a.parts = parts_of(n_seq, rows, H, Hkv);
     const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail);
     if (tiles * H > 0x7fffffffLL) return CCNET_EUNSUP;
     if (tiles == 0) return CCNET_OK;
@@ -742,8 +832,14 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     if (d == 128) hipLaunchKernelGGL(packed_bwd_dq_kernel<128>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
     else hipLaunchKernelGGL(packed_bwd_dq_kernel<64>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
     CCNET_LAUNCH_CHECK();
-    if (d == 128) hipLaunchKernelGGL(packed_bwd_dkv_kernel<128>, dim3((unsigned)(tiles * Hkv)), dim3(PA_THREADS), 0, st, a);
-    else hipLaunchKernelGGL(packed_bwd_dkv_kernel<64>, dim3((unsigned)(tiles * Hkv)), dim3(PA_THREADS), 0, st, a);
+    const dim3 grid((unsigned)(tiles * Hkv * a.parts));
+    if (d == 128) hipLaunchKernelGGL(packed_bwd_dkv_kernel<128>, grid, dim3(PA_THREADS), 0, st, a);
+    else hipLaunchKernelGGL(packed_bwd_dkv_kernel<64>, grid, dim3(PA_THREADS), 0, st, a);
     CCNET_LAUNCH_CHECK();
+    if (a.parts > 1) {
+        const long long threads = 2ll * rows * (Hkv * d / 8);
+        hipLaunchKernelGGL(packed_join_kernel, dim3((unsigned)std::min<long long>((threads + 255) / 256, 1 << 20)), dim3(256), 0, st, a, Hkv * d);
+        CCNET_LAUNCH_CHECK();
+    }
     return CCNET_OK;
 }

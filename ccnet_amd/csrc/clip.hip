@@ -8,11 +8,15 @@
 // its sum in the workspace; norm_final_kernel adds them in tile order, so the result does not depend on the order of execution.
 #include "common.h"
 
+#include <algorithm>
+#include <new>
+
 namespace {
 
 constexpr int CL_MOST = 128;           // tensors of a launch (28 bytes each of the 4 KiB of kernel arguments)
 constexpr int CL_VECS = 8192;          // 16-byte vectors of a tile (128 KiB)
 constexpr int CL_THREADS = 256;
+constexpr int CL_DEEP = 8;             // vectors a thread has in flight
 
 struct ClipArgs {
     const void* in[CL_MOST];
@@ -76,13 +80,23 @@ __global__ __launch_bounds__(CL_THREADS) void norm_tile_kernel(const ClipArgs a)
     const T* p = (const T*)a.in[k];
     const long long n = a.n[k], head = head_of<T>(p, n), vecs = (n - head) / X::N;
     const long long v0 = (long long)tile * CL_VECS, v1 = min(vecs, v0 + CL_VECS);
+    const typename X::R* body = (const typename X::R*)(p + head);
     double s[X::N] = {};
-    for (long long v = v0 + threadIdx.x; v < v1; v += CL_THREADS) {
+    auto add = [&](const typename X::R& r) {
         float f[X::N];
-        X::unpack(*(const typename X::R*)(p + head + v * X::N), f);
+        X::unpack(r, f);
 #pragma unroll
         for (int e = 0; e < X::N; ++e) s[e] = fma((double)f[e], (double)f[e], s[e]);
+    };
+    long long v = v0 + threadIdx.x;
+    for (; v + (CL_DEEP - 1) * CL_THREADS < v1; v += CL_DEEP * CL_THREADS) {
+        typename X::R r[CL_DEEP];
+#pragma unroll
+        for (int u = 0; u < CL_DEEP; ++u) r[u] = body[v + u * CL_THREADS];
+#pragma unroll
+        for (int u = 0; u < CL_DEEP; ++u) add(r[u]);
     }
+    for (; v < v1; v += CL_THREADS) add(body[v]);
     if (tile == 0) {  // what lies outside the whole vectors: at most N - 1 elements on either side
         const long long tail = head + vecs * X::N;
         const long long i = threadIdx.x < head ? (long long)threadIdx.x : tail + ((long long)threadIdx.x - head);
@@ -124,7 +138,8 @@ __global__ __launch_bounds__(1024) void norm_final_kernel(const double* partial,
 template <typename T, bool VALUE>
 __global__ __launch_bounds__(CL_THREADS) void clip_tile_kernel(const ClipArgs a) {
     typedef Vec<T> X;
-    const int k = tensor_of(a, blockIdx.x), tile = blockIdx.x - a.first[k];
+    const int at = gridDim.x - 1 - blockIdx.x;  // the tiles that the norm read last, and the cache may still hold, first
+    const int k = tensor_of(a, at), tile = at - a.first[k];
     const T* p = (const T*)a.in[k];
     T* q = (T*)a.out[k];
     const float f = VALUE ? 1.0f : *a.factor, lim = a.limit;
@@ -133,13 +148,23 @@ __global__ __launch_bounds__(CL_THREADS) void clip_tile_kernel(const ClipArgs a)
     auto one = [&](float v) { return VALUE ? (v > lim ? lim : v < -lim ? -lim : v) : v * f; };
     const long long n = a.n[k], head = head_of<T>(p, n), vecs = (n - head) / X::N;
     const long long v0 = (long long)tile * CL_VECS, v1 = min(vecs, v0 + CL_VECS);
-    for (long long v = v0 + threadIdx.x; v < v1; v += CL_THREADS) {
+    const typename X::R* body = (const typename X::R*)(p + head);
+    auto put = [&](long long v, const typename X::R& r) {
         float x[X::N];
-        X::unpack(*(const typename X::R*)(p + head + v * X::N), x);
+        X::unpack(r, x);
 #pragma unroll
         for (int e = 0; e < X::N; ++e) x[e] = one(x[e]);
         *(typename X::V*)(q + head + v * X::N) = X::pack(x);  // (the output may be aligned to its elements only)
+    };
+    long long v = v0 + threadIdx.x;
+    for (; v + (CL_DEEP - 1) * CL_THREADS < v1; v += CL_DEEP * CL_THREADS) {
+        typename X::R r[CL_DEEP];
+#pragma unroll
+        for (int u = 0; u < CL_DEEP; ++u) r[u] = body[v + u * CL_THREADS];
+#pragma unroll
+        for (int u = 0; u < CL_DEEP; ++u) put(v + u * CL_THREADS, r[u]);
     }
+    for (; v < v1; v += CL_THREADS) put(v, body[v]);
     if (tile == 0) {
         const long long tail = head + vecs * X::N;
         const long long i = threadIdx.x < head ? (long long)threadIdx.x : tail + ((long long)threadIdx.x - head);
@@ -147,11 +172,11 @@ __global__ __launch_bounds__(CL_THREADS) void clip_tile_kernel(const ClipArgs a)
     }
 }
 
-// fills the launches of a list in turn: launch(args, first tile of all, tiles)
+// fills the launches of the tensors [i, count) in turn: launch(args, first tile of all, tiles)
 template <typename T, typename F>
-int each_launch(const void* const* in, void* const* out, const int64_t* numel, int count, F launch) {
+int each_launch(const void* const* in, void* const* out, const int64_t* numel, int i, int count, F launch) {
     long long before = 0;
-    for (int i = 0; i < count;) {
+    while (i < count) {
         ClipArgs a{};
         long long tiles = 0;
         while (i < count && a.count < CL_MOST) {
@@ -186,18 +211,51 @@ bool list_ok(const void* const* p, const int64_t* numel, int count, int esz) {
 
 template <typename T>
 int norm_launches(const void* const* g, const int64_t* numel, int count, double* ws, hipStream_t st) {
-    return each_launch<T>(g, nullptr, numel, count, [&](ClipArgs& a, long long before, unsigned tiles) {
+    return each_launch<T>(g, nullptr, numel, 0, count, [&](ClipArgs& a, long long before, unsigned tiles) {
         a.partial = ws + 1 + before;
         hipLaunchKernelGGL(norm_tile_kernel<T>, dim3(tiles), dim3(CL_THREADS), 0, st, a);
     });
 }
 template <typename T, bool VALUE>
 int clip_launches(const void* const* g, void* const* out, const int64_t* numel, int count, const float* factor, float limit, hipStream_t st) {
-    return each_launch<T>(g, out, numel, count, [&](ClipArgs& a, long long, unsigned tiles) {
-        a.factor = factor;
-        a.limit = limit;
-        hipLaunchKernelGGL((clip_tile_kernel<T, VALUE>), dim3(tiles), dim3(CL_THREADS), 0, st, a);
-    });
+    for (int end = count; end > 0;) {  // the list from its end, as the tiles of a launch
+        const int begin = end > CL_MOST ? end - CL_MOST : 0;
+        const int rc = each_launch<T>(g, out, numel, begin, end, [&](ClipArgs& a, long long, unsigned tiles) {
+            a.factor = factor;
+            a.limit = limit;
+            hipLaunchKernelGGL((clip_tile_kernel<T, VALUE>), dim3(tiles), dim3(CL_THREADS), 0, st, a);
+        });
+        if (rc != CCNET_OK) return rc;
+        end = begin;
+    }
+    return CCNET_OK;
+}
+
+// Whether no two of the tensors written overlap, and none of them a tensor read other than its own whole.
+struct Span { uintptr_t lo, hi; int i; };
+int aliases_ok(const void* const* in, void* const* out, const int64_t* numel, int count, int esz) {
+    if (count == 0) return CCNET_OK;
+    Span* s = new (std::nothrow) Span[2 * (size_t)count];
+    if (!s) return CCNET_EWS;
+    Span* r = s + count;
+    int n = 0;
+    bool apart = false;
+    for (int i = 0; i < count; ++i) {
+        if (numel[i] == 0) continue;
+        s[n] = Span{(uintptr_t)out[i], (uintptr_t)out[i] + (uintptr_t)numel[i] * esz, i};
+        r[n++] = Span{(uintptr_t)in[i], (uintptr_t)in[i] + (uintptr_t)numel[i] * esz, i};
+        apart |= out[i] != in[i];
+    }
+    auto less = [](const Span& a, const Span& b) { return a.lo < b.lo; };
+    std::sort(s, s + n, less);
+    bool ok = true;
+    for (int i = 0; i + 1 < n; ++i) ok &= s[i].hi <= s[i + 1].lo;
+    for (int i = 0; ok && apart && i < n; ++i) {  // the written spans are disjoint: the ones that touch r[i] are neighbours
+        Span* w = std::lower_bound(s, s + n, r[i], [](const Span& a, const Span& b) { return a.hi <= b.lo; });
+        for (; w != s + n && w->lo < r[i].hi; ++w) ok &= w->i == r[i].i && w->lo == r[i].lo;
+    }
+    delete[] s;
+    return ok ? CCNET_OK : CCNET_EINVAL;
 }
 
 long long all_tiles(const void* const* g, const int64_t* numel, int count, int dtype) {
@@ -235,6 +293,8 @@ extern "C" int ccnet_clip_grad_norm(const void* const* grads, void* const* out, 
     if ((dtype != 0 && dtype != 1) || !norm || !(max_norm >= 0.f) || !list_ok(grads, numel, count, esz) ||
         !list_ok((const void* const*)out, numel, count, esz))
         return CCNET_EINVAL;
+    int rc = aliases_ok(grads, out, numel, count, esz);
+    if (rc != CCNET_OK) return rc;
     const long long tiles = all_tiles(grads, numel, count, dtype);
     if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
     if (!workspace || ((uintptr_t)workspace & 7)) return CCNET_EINVAL;
@@ -242,7 +302,7 @@ extern "C" int ccnet_clip_grad_norm(const void* const* grads, void* const* out, 
     hipStream_t st = (hipStream_t)stream;
     double* ws = (double*)workspace;
     float* factor = (float*)workspace;  // the workspace's first 8 bytes
-    int rc = dtype == 0 ? norm_launches<float>(grads, numel, count, ws, st) : norm_launches<unsigned short>(grads, numel, count, ws, st);
+    rc = dtype == 0 ? norm_launches<float>(grads, numel, count, ws, st) : norm_launches<unsigned short>(grads, numel, count, ws, st);
     if (rc != CCNET_OK) return rc;
     hipLaunchKernelGGL(norm_final_kernel, dim3(1), dim3(1024), 0, st, ws + 1, (int)tiles, max_norm, norm, factor);
     CCNET_LAUNCH_CHECK();
@@ -256,6 +316,8 @@ extern "C" int ccnet_clip_grad_value(const void* const* grads, void* const* out,
     if ((dtype != 0 && dtype != 1) || !(limit >= 0.f) || !list_ok(grads, numel, count, esz) ||
         !list_ok((const void* const*)out, numel, count, esz))
         return CCNET_EINVAL;
+    const int rc = aliases_ok(grads, out, numel, count, esz);
+    if (rc != CCNET_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
     return dtype == 0 ? clip_launches<float, true>(grads, out, numel, count, nullptr, limit, st)
                       : clip_launches<unsigned short, true>(grads, out, numel, count, nullptr, limit, st);

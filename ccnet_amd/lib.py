@@ -31,7 +31,7 @@ EXPORTS = [
     "ccnet_xattn_fused_bf16", "ccnet_xattn_packed_bytes", "ccnet_xattn_kv_image_bytes",
     # token lookup, packed causal attention, gradient clipping
     "ccnet_embedding", "ccnet_embedding_grad_workspace_bytes", "ccnet_embedding_grad", "ccnet_attention_packed_bf16",
-    "ccnet_attention_packed_bwd_bf16", "ccnet_grad_norm_workspace_bytes", "ccnet_grad_norm", "ccnet_clip_grad_norm",
+    "ccnet_attention_packed_bwd_workspace_bytes", "ccnet_attention_packed_bwd_bf16", "ccnet_grad_norm_workspace_bytes", "ccnet_grad_norm", "ccnet_clip_grad_norm",
     "ccnet_clip_grad_value",
 ]
 
@@ -134,12 +134,14 @@ def load() -> C.CDLL:
     lib.ccnet_xattn_kv_image_bytes.argtypes = [i, i]
     lib.ccnet_xattn_kv_image_bytes.restype = C.c_int64
     lib.ccnet_embedding.argtypes = [vp, i, i, i, vp, i, i, i, f, vp, i, i, vp]
-    lib.ccnet_embedding_grad_workspace_bytes.argtypes = [i, i]
+    lib.ccnet_embedding_grad_workspace_bytes.argtypes = [i, i, i]
     lib.ccnet_embedding_grad_workspace_bytes.restype = sz
     lib.ccnet_embedding_grad.argtypes = [vp, i, i, i, vp, i, i, i, f, i64, vp, i, i, vp, sz, vp]
-    lib.ccnet_attention_packed_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, i, vp, vp]
-    lib.ccnet_attention_packed_bwd_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, vp, vp, vp, i, vp, i, vp, i, vp, i, i, i, i, i,
-                                                    f, i, vp]
+    lib.ccnet_attention_packed_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, i, vp, vp, vp]
+    lib.ccnet_attention_packed_bwd_workspace_bytes.argtypes = [i, i, i, i, i]
+    lib.ccnet_attention_packed_bwd_workspace_bytes.restype = sz
+    lib.ccnet_attention_packed_bwd_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, vp, i, vp, vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, i,
+                                                    vp, sz, vp]
     pp, pi64 = C.POINTER(vp), C.POINTER(i64)
     lib.ccnet_grad_norm_workspace_bytes.argtypes = [pp, pi64, i, i]
     lib.ccnet_grad_norm_workspace_bytes.restype = sz

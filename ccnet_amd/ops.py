@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -594,36 +594,26 @@ def axpy_f32(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
 _F32_BF16 = {torch.float32: 0, BF16: 1}
 
 
-class _on_device_of:
-    """Makes the tensors' device current for the launch (a no-op where it is): the stream is that device's current one."""
-
-    def __init__(self, *ts: Optional[torch.Tensor]):
-        ts = [t for t in ts if t is not None]
+def _elsewhere(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether the operands live on another device than the current one (the op then runs with that device made current); raises
+    where they are on the CPU or on different devices."""
+    dev = {t.get_device() for t in ts if t is not None}
+    if len(dev) != 1 or -1 in dev:
         _need_cuda(*ts)
-        if any(t.device != ts[0].device for t in ts):
-            raise _l.CcnetError("operands are on different devices: " + ", ".join(str(t.device) for t in ts))
-        self.device = ts[0].device
-        self.guard = None
-
-    def __enter__(self) -> int:
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return _stream()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+        raise _l.CcnetError(f"operands are on different devices: {sorted(dev)}")
+    return dev.pop() != torch.cuda.current_device()
 
 
 def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
     """Row stride of a 2-D operand [rows, width] whose rows are contiguous; raises on anything else."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype not in dtypes:
+    if t.shape != (rows, width) or t.dtype not in dtypes:
         raise _l.CcnetError(f"{what}: expected {' or '.join(str(d) for d in dtypes)} [{rows}, {width}], got {t.dtype} {list(t.shape)}")
-    if width > 1 and t.stride(1) != 1:
-        raise _l.CcnetError(f"{what}: rows must be contiguous (column stride {t.stride(1)})")
-    ld = t.stride(0) if rows > 1 else max(t.stride(0), (width + 7) // 8 * 8)
-    if max(rows, ld) > 0x7fffffff:
+    ld, step = t.stride()
+    if step != 1 and width > 1:
+        raise _l.CcnetError(f"{what}: rows must be contiguous (column stride {step})")
+    if rows <= 1:  # the stride of a single row says nothing
+        ld = max(ld, (width + 7) // 8 * 8)
+    if ld > 0x7fffffff or rows > 0x7fffffff:
         raise _l.CcnetError(f"{what}: {rows} rows of stride {ld} pass the 32 bits of the C ABI")
     return ld
 
@@ -641,15 +631,17 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype:
     lib = _l.load()
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise _l.CcnetError(f"table must be [vocab, C], got {list(table.shape)}")
-    ldt = _rows_ld(table, "table", table.shape[0], table.shape[1], tuple(_F32_BF16))
-    with _on_device_of(ids, table, out) as st:
-        flat = _ids(ids)
-        T, Cc = flat.numel(), table.shape[1]
-        if out is None:
-            out = torch.empty((T, Cc), dtype=dtype, device=ids.device)
-        ldo = _rows_ld(out, "out", T, Cc, tuple(_F32_BF16))
-        _l.check(lib.ccnet_embedding(flat.data_ptr(), flat.element_size(), T, table.shape[0], table.data_ptr(), _F32_BF16[table.dtype],
-                                     ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, st), "embedding")
+    ldt = _rows_ld(table, "table", table.shape[0], table.shape[1], _F32_BF16)
+    if _elsewhere(ids, table, out):
+        with torch.cuda.device(table.device):
+            return embedding(ids, table, scale, dtype, out)
+    flat = _ids(ids)
+    T, Cc = flat.numel(), table.shape[1]
+    if out is None:
+        out = torch.empty((T, Cc), dtype=dtype, device=table.device)
+    ldo = _rows_ld(out, "out", T, Cc, _F32_BF16)
+    _l.check(lib.ccnet_embedding(flat.data_ptr(), flat.element_size(), T, table.shape[0], table.data_ptr(), _F32_BF16[table.dtype],
+                                 ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, _stream()), "embedding")
     return out
 
 
@@ -665,21 +657,23 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float
         raise _l.CcnetError(f"embedding_grad: vocab {vocab}")
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise _l.CcnetError(f"embedding_grad: padding_idx {padding_idx} outside the table of {vocab}")
-    with _on_device_of(ids, dy, out) as st:
-        flat = _ids(ids)
-        T = flat.numel()
-        if dy.dim() != 2 or dy.shape[1] < 1:
-            raise _l.CcnetError(f"dy must be [T, C], got {list(dy.shape)}")
-        Cc = dy.shape[1]
-        lddy = _rows_ld(dy, "dy", T, Cc, tuple(_F32_BF16))
-        if out is None:
-            out = torch.empty((vocab, Cc), dtype=torch.float32, device=dy.device)
-        ldg = _rows_ld(out, "out", vocab, Cc, (torch.float32,))
-        wsb = lib.ccnet_embedding_grad_workspace_bytes(T, Cc)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device)
-        _l.check(lib.ccnet_embedding_grad(flat.data_ptr(), flat.element_size(), T, vocab, dy.data_ptr(), _F32_BF16[dy.dtype], lddy, Cc,
-                                          scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ldg, int(accumulate),
-                                          ws.data_ptr(), wsb, st), "embedding_grad")
+    if _elsewhere(ids, dy, out):
+        with torch.cuda.device(dy.device):
+            return embedding_grad(ids, dy, vocab, scale, padding_idx, out, accumulate)
+    flat = _ids(ids)
+    T = flat.numel()
+    if dy.dim() != 2 or dy.shape[1] < 1:
+        raise _l.CcnetError(f"dy must be [T, C], got {list(dy.shape)}")
+    Cc = dy.shape[1]
+    lddy = _rows_ld(dy, "dy", T, Cc, _F32_BF16)
+    if out is None:
+        out = torch.empty((vocab, Cc), dtype=torch.float32, device=dy.device)
+    ldg = _rows_ld(out, "out", vocab, Cc, (torch.float32,))
+    wsb = lib.ccnet_embedding_grad_workspace_bytes(T, vocab, Cc)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device)
+    _l.check(lib.ccnet_embedding_grad(flat.data_ptr(), flat.element_size(), T, vocab, dy.data_ptr(), _F32_BF16[dy.dtype], lddy, Cc,
+                                      scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ldg, int(accumulate),
+                                      ws.data_ptr(), wsb, _stream()), "embedding_grad")
     return out
 
 
@@ -693,48 +687,66 @@ def _packed_operands(q, k, v, cu_seqlens, H: int, Hkv: int, d: int):
                   _rows_ld(v, "v", rows, Hkv * d, (BF16,)))
 
 
+class PackedStats(NamedTuple):
+    """What `attention_packed` leaves for its backward: the rows' log-sum-exp in base 2, fp32 [H, rows], and what the rounding
+    of o to bf16 took away, bf16 [rows, H*d] (with it dO . o is known to fp32 in the backward; o alone is off by 2^-8)."""
+    lse: torch.Tensor
+    o_low: torch.Tensor
+
+
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, H: int, Hkv: int, d: int,
                      scale: float, with_lse: bool = False, out: Optional[torch.Tensor] = None):
     """Causal self-attention over sequences that lie end to end in the rows: q [rows, H*d], k / v [rows, Hkv*d] bf16 (column
     slices of one matrix allowed), query head h on key head h // (H // Hkv), d 64 or 128, sequence i = rows
-    cu_seqlens[i] .. cu_seqlens[i+1] (int32 on the GPU, never copied to the host).  Returns o [rows, H*d], with_lse: (o, lse) for
+    cu_seqlens[i] .. cu_seqlens[i+1] (int32 on the GPU, never copied to the host).  Returns o [rows, H*d], with_lse: (o, stats) for
     `attention_packed_bwd`.  Rows behind the last sequence are zeros, or with `out` (which must not overlap k or v) left as
     they are."""
     lib = _l.load()
-    with _on_device_of(q, k, v, cu_seqlens, out) as st:
-        rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
-        o = torch.empty((rows, H * d), dtype=BF16, device=q.device) if out is None else out
-        lse = torch.empty((H, rows), dtype=torch.float32, device=q.device) if with_lse else None
-        _l.check(lib.ccnet_attention_packed_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(),
-                                                 _rows_ld(o, "out", rows, H * d, (BF16,)), cu_seqlens.data_ptr(),
-                                                 cu_seqlens.numel() - 1, rows, H, Hkv, d, scale, int(out is None), _ptr(lse), st),
-                 "attention_packed")
-    return (o, lse) if with_lse else o
+    if _elsewhere(q, k, v, cu_seqlens, out):
+        with torch.cuda.device(q.device):
+            return attention_packed(q, k, v, cu_seqlens, H, Hkv, d, scale, with_lse, out)
+    rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
+    o = torch.empty((rows, H * d), dtype=BF16, device=q.device) if out is None else out
+    stats = None
+    if with_lse:
+        stats = PackedStats(torch.empty((H, rows), dtype=torch.float32, device=q.device),
+                            torch.empty((rows, H * d), dtype=BF16, device=q.device))
+    _l.check(lib.ccnet_attention_packed_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(),
+                                             _rows_ld(o, "out", rows, H * d, (BF16,)), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1,
+                                             rows, H, Hkv, d, scale, int(out is None), stats.lse.data_ptr() if with_lse else None,
+                                             stats.o_low.data_ptr() if with_lse else None, _stream()), "attention_packed")
+    return (o, stats) if with_lse else o
 
 
-def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, lse: torch.Tensor,
+def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor, stats: PackedStats,
                          cu_seqlens: torch.Tensor, H: int, Hkv: int, d: int, scale: float, dq: Optional[torch.Tensor] = None,
                          dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
-    """(dq, dk, dv) of `attention_packed` from its o, lse and the gradient `do` of o; dk / dv hold the sum over the query heads of
-    a key head.  The results overwrite dq / dk / dv where given (all three, e.g. column slices of one matrix; rows behind the
+    """(dq, dk, dv) of `attention_packed` from its (o, stats) and the gradient `do` of o; dk / dv hold the sum over the query heads
+    of a key head.  The results overwrite dq / dk / dv where given (all three, e.g. column slices of one matrix; rows behind the
     last sequence are then left as they are) or are new tensors (those rows zeros)."""
     lib = _l.load()
-    given = [g is not None for g in (dq, dk, dv)]
-    if any(given) and not all(given):
+    given = dq is not None
+    if given != (dk is not None) or given != (dv is not None):
         raise _l.CcnetError("attention_packed_bwd: give all of dq, dk, dv or none")
-    with _on_device_of(q, k, v, o, do, lse, cu_seqlens, dq, dk, dv) as st:
-        rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
-        if lse.dtype != torch.float32 or tuple(lse.shape) != (H, rows) or not lse.is_contiguous():
-            raise _l.CcnetError(f"attention_packed_bwd: lse must be the forward's fp32 [{H}, {rows}]")
-        if not given[0]:
-            dq, dk, dv = (torch.empty((rows, n * d), dtype=BF16, device=q.device) for n in (H, Hkv, Hkv))
-        delta = torch.empty((H, rows), dtype=torch.float32, device=q.device)
-        _l.check(lib.ccnet_attention_packed_bwd_bf16(
-            q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), _rows_ld(o, "o", rows, H * d, (BF16,)),
-            do.data_ptr(), _rows_ld(do, "do", rows, H * d, (BF16,)), lse.data_ptr(), delta.data_ptr(),
-            dq.data_ptr(), _rows_ld(dq, "dq", rows, H * d, (BF16,)), dk.data_ptr(), _rows_ld(dk, "dk", rows, Hkv * d, (BF16,)),
-            dv.data_ptr(), _rows_ld(dv, "dv", rows, Hkv * d, (BF16,)), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, rows, H, Hkv, d,
-            scale, int(not given[0]), st), "attention_packed_bwd")
+    lse, o_low = stats
+    if _elsewhere(q, k, v, o, do, lse, o_low, cu_seqlens, dq, dk, dv):
+        with torch.cuda.device(q.device):
+            return attention_packed_bwd(q, k, v, o, do, stats, cu_seqlens, H, Hkv, d, scale, dq, dk, dv)
+    rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
+    if lse.dtype != torch.float32 or lse.shape != (H, rows) or not lse.is_contiguous() or o_low.dtype != BF16 \
+            or o_low.shape != (rows, H * d) or not o_low.is_contiguous():
+        raise _l.CcnetError(f"attention_packed_bwd: stats must be the forward's, fp32 [{H}, {rows}] and bf16 [{rows}, {H * d}]")
+    if not given:
+        dq = torch.empty((rows, H * d), dtype=BF16, device=q.device)
+        dk, dv = (torch.empty((rows, Hkv * d), dtype=BF16, device=q.device) for _ in range(2))
+    n_seq = cu_seqlens.numel() - 1
+    wsb = lib.ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
+    _l.check(lib.ccnet_attention_packed_bwd_bf16(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), _rows_ld(o, "o", rows, H * d, (BF16,)), o_low.data_ptr(),
+        do.data_ptr(), _rows_ld(do, "do", rows, H * d, (BF16,)), lse.data_ptr(), dq.data_ptr(), _rows_ld(dq, "dq", rows, H * d, (BF16,)),
+        dk.data_ptr(), _rows_ld(dk, "dk", rows, Hkv * d, (BF16,)), dv.data_ptr(), _rows_ld(dv, "dv", rows, Hkv * d, (BF16,)),
+        cu_seqlens.data_ptr(), n_seq, rows, H, Hkv, d, scale, int(not given), ws.data_ptr(), wsb, _stream()), "attention_packed_bwd")
     return dq, dk, dv
 
 
@@ -754,55 +766,46 @@ def _grad_list(grads, what: str):
     grads = list(grads)
     if not grads:
         raise _l.CcnetError(f"{what}: no gradients")
-    dt = grads[0].dtype
-    if dt not in _F32_BF16 or any(g.dtype != dt for g in grads):
-        raise _l.CcnetError(f"{what}: gradients must all be fp32 or all bf16, got {sorted({str(g.dtype) for g in grads})}")
-    if not all(_dense(g) for g in grads):
+    dts = {g.dtype for g in grads}
+    if len(dts) != 1 or not dts <= _F32_BF16.keys():
+        raise _l.CcnetError(f"{what}: gradients must all be fp32 or all bf16, got {sorted(str(d) for d in dts)}")
+    plain = all(map(torch.Tensor.is_contiguous, grads))
+    if not plain and not all(map(_dense, grads)):
         raise _l.CcnetError(f"{what}: a gradient's elements must fill one range of memory (expanded or strided views do not)")
     n = len(grads)
-    return grads, (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads]), n, _F32_BF16[dt]
+    sizes = list(map(torch.Tensor.numel, grads))
+    return (grads, (C.c_void_p * n)(*map(torch.Tensor.data_ptr, grads)), (C.c_int64 * n)(*sizes), n, _F32_BF16[grads[0].dtype],
+            sizes if plain else None)
 
 
-def _clip_outputs(grads, ptrs, out, what: str):
-    """(pointers to write to, the tensors written): in place, or `out` with the same shapes, strides and type."""
+def _clip_outputs(grads, ptrs, sizes, out, what: str):
+    """(pointers to write to, the tensors written): in place, or `out` with the same shapes, strides and type.  That they do not
+    overlap is the library's check."""
     if out is None:
-        outs, optrs = grads, ptrs
-    else:
-        outs = list(out)
-        if len(outs) != len(grads) or any(o.shape != g.shape or o.stride() != g.stride() or o.dtype != g.dtype
-                                          for o, g in zip(outs, grads)):
-            raise _l.CcnetError(f"{what}: out must match the gradients' shapes, strides and type")
-        optrs = (C.c_void_p * len(outs))(*[o.data_ptr() for o in outs])
-    esz = grads[0].element_size()
-    spans = sorted((o.data_ptr(), o.data_ptr() + o.numel() * esz, i) for i, o in enumerate(outs) if o.numel())
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
-        raise _l.CcnetError(f"{what}: the tensors written overlap (one tensor given twice?)")
-    if out is not None:  # a gradient read by one tile while another writes there
-        reads = sorted((g.data_ptr(), g.data_ptr() + g.numel() * esz, i) for i, g in enumerate(grads) if g.numel())
-        j = 0
-        for lo, hi, i in reads:
-            while j > 0 and spans[j - 1][1] > lo:
-                j -= 1
-            while j < len(spans) and spans[j][1] <= lo:
-                j += 1
-            m = j
-            while m < len(spans) and spans[m][0] < hi:
-                if not (spans[m][2] == i and spans[m][0] == lo):
-                    raise _l.CcnetError(f"{what}: out overlaps a gradient other than its own")
-                m += 1
-    return optrs, outs
+        return ptrs, grads
+    outs = list(out)
+    same = len(outs) == len(grads) and {o.dtype for o in outs} == {grads[0].dtype}
+    if same and sizes is not None and all(map(torch.Tensor.is_contiguous, outs)):
+        same = list(map(torch.Tensor.numel, outs)) == sizes
+    elif same:
+        same = all(o.shape == g.shape and o.stride() == g.stride() for o, g in zip(outs, grads))
+    if not same:
+        raise _l.CcnetError(f"{what}: out must match the gradients' shapes, strides and type")
+    return (C.c_void_p * len(outs))(*map(torch.Tensor.data_ptr, outs)), outs
 
 
 def grad_norm(grads) -> torch.Tensor:
     """The L2 norm over all elements of all tensors (fp32 or bf16, contiguous in any order of their dimensions), summed in fp64:
     an fp32 scalar on the GPU."""
     lib = _l.load()
-    grads, ptrs, numel, n, dt = _grad_list(grads, "grad_norm")
-    with _on_device_of(*grads) as st:
-        wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
-        ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
-        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), st), "grad_norm")
+    grads, ptrs, numel, n, dt, _ = _grad_list(grads, "grad_norm")
+    if _elsewhere(*grads):
+        with torch.cuda.device(grads[0].device):
+            return grad_norm(grads)
+    wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
+    ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), _stream()), "grad_norm")
     return norm
 
 
@@ -811,28 +814,32 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     synchronisation: returns the norm before clipping as an fp32 scalar on the GPU.  A norm that is not finite scales nothing.
     out: tensors of the same shapes that receive the clipped values instead; the tensors written must not overlap."""
     lib = _l.load()
-    grads, ptrs, numel, n, dt = _grad_list(grads, "clip_grad_norm")
+    grads, ptrs, numel, n, dt, sizes = _grad_list(grads, "clip_grad_norm")
     if not max_norm >= 0:
         raise _l.CcnetError(f"clip_grad_norm: max_norm {max_norm}")
-    optrs, outs = _clip_outputs(grads, ptrs, out, "clip_grad_norm")
-    with _on_device_of(*grads, *(outs if out is not None else ())) as st:
-        wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
-        ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
-        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), st),
-                 "clip_grad_norm")
+    optrs, outs = _clip_outputs(grads, ptrs, sizes, out, "clip_grad_norm")
+    if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
+        with torch.cuda.device(grads[0].device):
+            return clip_grad_norm(grads, max_norm, None if out is None else outs)
+    wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
+    ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _stream()),
+             "clip_grad_norm")
     return norm
 
 
 def clip_grad_value(grads, limit: float, out=None) -> None:
     """Every element clamped to [-limit, limit] in place (clip_grad_value_), or into `out` as in `clip_grad_norm`."""
     lib = _l.load()
-    grads, ptrs, numel, n, dt = _grad_list(grads, "clip_grad_value")
+    grads, ptrs, numel, n, dt, sizes = _grad_list(grads, "clip_grad_value")
     if not limit >= 0:
         raise _l.CcnetError(f"clip_grad_value: limit {limit}")
-    optrs, outs = _clip_outputs(grads, ptrs, out, "clip_grad_value")
-    with _on_device_of(*grads, *(outs if out is not None else ())) as st:
-        _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, st), "clip_grad_value")
+    optrs, outs = _clip_outputs(grads, ptrs, sizes, out, "clip_grad_value")
+    if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
+        with torch.cuda.device(grads[0].device):
+            return clip_grad_value(grads, limit, None if out is None else outs)
+    _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _stream()), "clip_grad_value")
 
 
 _prof_on = False

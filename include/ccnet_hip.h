@@ -394,8 +394,8 @@ int ccnet_embedding(const void* ids, int id_bytes, int T, int vocab, const void*
 /* grad[v] (fp32) = scale * sum of dy[t] over the positions with ids[t] = v; every row is written, rows without a position as
  * zeros.  accumulate != 0: added to what is there, rows without a position are not touched.  Positions whose id is outside
  * [0, vocab) or equal to padding_idx (-1: none) take no part.  T <= 2^30; workspace (16-byte aligned):
- * ccnet_embedding_grad_workspace_bytes(T, C) bytes. */
-size_t ccnet_embedding_grad_workspace_bytes(int T, int C);
+ * ccnet_embedding_grad_workspace_bytes(T, vocab, C) bytes. */
+size_t ccnet_embedding_grad_workspace_bytes(int T, int vocab, int C);
 int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const void* dy, int dy_dtype, int lddy, int C, float scale,
                          int64_t padding_idx, float* grad, int ldg, int accumulate, void* workspace, size_t workspace_bytes,
                          void* stream);
@@ -403,20 +403,23 @@ int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const 
 /* Causal self-attention over n_seq sequences that lie end to end in the rows of q / k / v: sequence i is rows
  * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (device memory, n_seq + 1 values, the first 0, rising; empty sequences are allowed).
  * H query heads of width d (64 or 128) in columns h d ..; query head h reads key head h / (H / Hkv).  Key <= query.
- *   out = softmax(scale q k^T) v;   lse[h][row] (may be NULL) = log2 of the sum of 2^(scale log2(e) q k^T)
+ *   out = softmax(scale q k^T) v;   lse[h][row] (may be NULL) = log2 of the sum of 2^(scale log2(e) q k^T);
+ *   o_low [rows][H d] (may be NULL) = what the rounding of out to bf16 took away, itself rounded to bf16
  * Rows behind the last sequence: left as they are, or with zero_tail != 0 written as zeros (lse: -inf).  A key or value that is
  * not finite reaches only the queries of its sequence that see it.  16-byte aligned rows (ld % 8 == 0); out must not overlap
  * k or v.  Grids follow from rows and n_seq alone: a captured graph serves other lengths with the same totals. */
 int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo,
                                 const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale, int zero_tail,
-                                float* lse, void* stream);
-/* Its backward: dQ, and dK / dV summed over the query heads of a key head, from the forward's out and lse.  delta: scratch
- * [H][rows] fp32.  The gradients overwrite; rows behind the last sequence as above.  dO, lse and the operands must be finite for
- * the gradients of a sequence to be (a value that is not spreads inside its sequence, never to another one). */
+                                float* lse, void* o_low, void* stream);
+/* Its backward: dQ, and dK / dV summed over the query heads of a key head, from the forward's out, o_low (NULL: out alone, whose
+ * rounding then enters dQ and dK) and lse.  The gradients overwrite; rows behind the last sequence as above.  dO, lse and the
+ * operands must be finite for the gradients of a sequence to be (a value that is not spreads inside its sequence, never to
+ * another one).  workspace (16-byte aligned): ccnet_attention_packed_bwd_workspace_bytes of the same sizes. */
+size_t ccnet_attention_packed_bwd_workspace_bytes(int n_seq, int rows, int H, int Hkv, int d);
 int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, const void* O, int ldo,
-                                    const void* dO, int lddo, const float* lse, float* delta, void* dQ, int lddq, void* dK, int lddk,
-                                    void* dV, int lddv, const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d,
-                                    float scale, int zero_tail, void* stream);
+                                    const void* o_low, const void* dO, int lddo, const float* lse, void* dQ, int lddq, void* dK,
+                                    int lddk, void* dV, int lddv, const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv,
+                                    int d, float scale, int zero_tail, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Global gradient norm over `count` tensors (host arrays of device pointers and element counts, read before the call returns;
  * elements contiguous in memory, any alignment of at least the element's): norm[0] = sqrt(sum of squares), fp64 inside, so that
@@ -425,8 +428,8 @@ size_t ccnet_grad_norm_workspace_bytes(const void* const* grads /*host*/, const 
 int ccnet_grad_norm(const void* const* grads /*host*/, const int64_t* numel /*host*/, int count, int dtype, void* workspace,
                     size_t workspace_bytes, float* norm /*device*/, void* stream);
 /* out[i] = min(1, max_norm / (norm + 1e-6)) * grads[i]  (util.py:1176-1206, clip_grad_norm_); out[i] == grads[i]: in place, and
- * then nothing is written where the factor is 1.  A norm that is not finite leaves the values as they are (factor 1).  The
- * tensors of `out` must not overlap each other, nor any of `grads` other than their own whole. */
+ * then nothing is written where the factor is 1.  A norm that is not finite leaves the values as they are (factor 1).
+ * CCNET_EINVAL where tensors of `out` overlap each other, or any of `grads` other than their own whole. */
 int ccnet_clip_grad_norm(const void* const* grads /*host*/, void* const* out /*host*/, const int64_t* numel /*host*/, int count,
                          int dtype, float max_norm, void* workspace, size_t workspace_bytes, float* norm /*device*/, void* stream);
 /* out[i] = grads[i] clamped to [-limit, limit] (clip_grad_value_; a NaN stays one).  Aliasing as above. */

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 BF16 = torch.bfloat16
+EINVAL, EUNSUP, EWS = -1, -2, -4
 
 
 def _err():
@@ -23,7 +24,7 @@ def test_cpu_tensors_are_refused():
     cu = torch.tensor([0, 4], dtype=torch.int32)
     b = x.to(BF16)
     for call in (lambda: ops.embedding(ids, x), lambda: ops.embedding_grad(ids, x, 9), lambda: ops.attention_packed(b, b, b, cu, 1, 1, 64, 1.0),
-                 lambda: ops.attention_packed_bwd(b, b, b, b, b, x[:1, :4], cu, 1, 1, 64, 1.0), lambda: ops.grad_norm([x]),
+                 lambda: ops.attention_packed_bwd(b, b, b, b, b, ops.PackedStats(x[:1, :4], b), cu, 1, 1, 64, 1.0), lambda: ops.grad_norm([x]),
                  lambda: ops.clip_grad_norm([x], 1.0), lambda: ops.clip_grad_value([x], 1.0)):
         with pytest.raises(_err(), match="GPU only"):
             call()
@@ -38,34 +39,32 @@ def test_wrapper_refusals_before_any_launch():
                  lambda: ops.embedding_grad(ids, x, 9, padding_idx=9), lambda: ops.grad_norm([]), lambda: ops.grad_norm([x, x.to(BF16)]),
                  lambda: ops.grad_norm([x.half()]), lambda: ops.grad_norm([x[:, :3]]), lambda: ops.grad_norm([x[:1].expand(4, 64)]),
                  lambda: ops.clip_grad_norm([x], -1.0), lambda: ops.clip_grad_norm([x], float("nan")),
-                 lambda: ops.clip_grad_value([x], -1.0), lambda: ops.clip_grad_norm([x, x], 1.0),
-                 lambda: ops.clip_grad_norm([x, x[1]], 1.0), lambda: ops.clip_grad_norm([x], 1.0, out=[]),
+                 lambda: ops.clip_grad_value([x], -1.0), lambda: ops.clip_grad_norm([x], 1.0, out=[]),
                  lambda: ops.clip_grad_norm([x], 1.0, out=[x.t()]), lambda: ops.clip_grad_norm([x], 1.0, out=[x.to(BF16)])):
         with pytest.raises(_err()):
             call()
 
 
 def test_clip_outputs_must_not_overlap_other_gradients():
-    """The aliasing rules by themselves (they are checked before the device): in place and apart are fine, shifted is not."""
-    from ccnet_amd import ops
+    """The aliasing rules of the C entry points, on host addresses that are never dereferenced: the calls that break one return
+    CCNET_EINVAL before a launch; the ones that keep them get as far as the next check, a workspace that is too small."""
+    l = _lib()
+    base = 1 << 20
 
-    def go(grads, out):
-        grads, ptrs, *_ = ops._grad_list(grads, "t")
-        return ops._clip_outputs(grads, ptrs, out, "t")
+    def go(grads, outs):
+        n = len(grads)
+        mk = lambda v: (C.c_void_p * n)(*[base + 4 * lo for lo, _ in v])  # noqa: E731
+        num = (C.c_int64 * n)(*[hi - lo for lo, hi in grads])
+        out = mk(outs)
+        return l.ccnet_clip_grad_norm(mk(grads), out, num, n, 0, 1.0, C.c_void_p(base), 0, C.c_void_p(base), None)
 
-    f = torch.zeros(100)
-    a, b, c = f[:10], f[10:20], f[20:30]
-    go([a, b, c], None)
-    go([a, b], [a, b])
-    go([a, b], [c, f[40:50]])
-    go([a, b], [a, c])
-    go([c, a], [f[50:60], a])
-    go([a, a[:0], b], [c, a[:0], f[40:50]])
-    go([a, a], [b, c])  # reading one twice is fine
-    for grads, out in (([a, b], [b, a]), ([a, b], [f[5:15], c]), ([a], [f[1:11]]), ([a, b, c], [f[50:60], f[12:22], f[70:80]]),
-                       ([a, b], [c, c]), ([a, b], [f[60:70], f[65:75]]), ([f[:50], c], [f[50:], f[30:40]])):
-        with pytest.raises(_err()):
-            go(grads, out)
+    a, b, c, d = (0, 10), (10, 20), (20, 30), (40, 50)
+    e = (0, 0)
+    for grads, outs in (([a, b, c], [a, b, c]), ([a, b], [c, d]), ([a, b], [a, c]), ([c, a], [(50, 60), a]), ([a, e, b], [c, e, d]), ([a, a], [b, c])):
+        assert go(grads, outs) == EWS, (grads, outs)
+    for grads, outs in (([a, b], [b, a]), ([a, b], [(5, 15), c]), ([a], [(1, 11)]), ([a, b, c], [(50, 60), (12, 22), (70, 80)]), ([a, b], [c, c]),
+                        ([a, b], [(60, 70), (65, 75)]), ([(0, 50), (60, 70)], [(50, 100), (30, 40)]), ([a, a], [a, a]), ([a, a], [a, b])):
+        assert go(grads, outs) == EINVAL, (grads, outs)
 
 
 def test_dense_layouts():
@@ -73,9 +72,6 @@ def test_dense_layouts():
     x = torch.zeros(4, 6, 5)
     assert all(ops._dense(t) for t in (x, x.permute(2, 0, 1), x.transpose(0, 1), x[1], x[:1], torch.zeros(0), x[1, 1, 1]))
     assert not any(ops._dense(t) for t in (x[:, ::2], x[:, :3], x[..., 1], x[:1].expand(4, 6, 5)))
-
-
-EINVAL, EUNSUP, EWS = -1, -2, -4
 
 
 def test_c_abi_refusals():
@@ -92,8 +88,8 @@ def test_c_abi_refusals():
     a[2] = 0
     assert E(*a) == 0  # no rows: nothing to do
     G = l.ccnet_embedding_grad
-    need = l.ccnet_embedding_grad_workspace_bytes(1000, 64)
-    assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 64) == 0
+    need = l.ccnet_embedding_grad_workspace_bytes(1000, 10, 64)
+    assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 10, 64) == 0
     ok = [p, 8, 1000, 10, p, 1, 64, 64, 1.0, -1, p, 64, 0, p, need, None]
     for i, v, rc in ((1, 3, EINVAL), (2, -1, EINVAL), (3, 0, EINVAL), (3, 0x7fffffff, EINVAL), (4, None, EINVAL), (5, 2, EINVAL), (6, 8, EINVAL),
                      (7, 0, EINVAL), (10, None, EINVAL), (10, C.c_void_p(1026), EINVAL), (11, 63, EINVAL), (13, None, EINVAL),
@@ -102,12 +98,12 @@ def test_c_abi_refusals():
         a[i] = v
         assert G(*a) == rc, (i, v)
     F = l.ccnet_attention_packed_bf16
-    ok = [p, 256, p, 128, p, 128, p, 256, p, 3, 100, 4, 2, 64, 0.125, 1, None, None]
+    ok = [p, 256, p, 128, p, 128, p, 256, p, 3, 100, 4, 2, 64, 0.125, 1, None, None, None]
     odd = C.c_void_p(1 << 20 | 8)
     for i, v, rc in ((0, None, EINVAL), (0, odd, EINVAL), (1, 255, EINVAL), (1, 248, EINVAL), (2, None, EINVAL), (3, 64, EINVAL), (4, odd, EINVAL),
                      (5, 132, EINVAL), (6, None, EINVAL), (7, 192, EINVAL), (8, None, EINVAL), (9, -1, EINVAL), (10, -1, EINVAL), (11, 0, EINVAL),
                      (11, 3, EINVAL), (12, 0, EINVAL), (13, 96, EUNSUP), (13, 32, EUNSUP), (14, 0.0, EINVAL), (14, -1.0, EINVAL),
-                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP)):
+                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP), (17, odd, EINVAL)):
         a = list(ok)
         a[i] = v
         assert F(*a) == rc, (i, v)
@@ -115,16 +111,19 @@ def test_c_abi_refusals():
     a[10] = 0
     assert F(*a) == 0
     B = l.ccnet_attention_packed_bwd_bf16
-    ok = [p, 256, p, 128, p, 128, p, 256, p, 256, p, p, p, 256, p, 128, p, 128, p, 3, 100, 4, 2, 64, 0.125, 1, None]
-    for i in (0, 2, 4, 6, 8, 10, 11, 12, 14, 16, 18):
+    size = l.ccnet_attention_packed_bwd_workspace_bytes
+    need = size(3, 100, 4, 2, 64)
+    assert need >= 100 * 4 * 4 and size(1, 4096, 16, 4, 64) >= 4096 * 16 * 4 + 2 * 2 * 4096 * 4 * 64 * 4  # (long walks of few key heads are cut)
+    ok = [p, 256, p, 128, p, 128, p, 256, p, p, 256, p, p, 256, p, 128, p, 128, p, 3, 100, 4, 2, 64, 0.125, 1, p, need, None]
+    for i in (0, 2, 4, 6, 9, 11, 12, 14, 16, 18, 26):
         a = list(ok)
         a[i] = None
         assert B(*a) == EINVAL, i
-    for i in (1, 3, 5, 7, 9, 13, 15, 17):
+    for i in (1, 3, 5, 7, 10, 13, 15, 17):
         a = list(ok)
         a[i] = 100
         assert B(*a) == EINVAL, i
-    for i, v, rc in ((21, 3, EINVAL), (23, 80, EUNSUP), (24, 0.0, EINVAL), (20, 0, 0)):
+    for i, v, rc in ((8, odd, EINVAL), (26, odd, EINVAL), (21, 3, EINVAL), (23, 80, EUNSUP), (24, 0.0, EINVAL), (20, 0, 0), (27, need - 1, EWS)):
         a = list(ok)
         a[i] = v
         assert B(*a) == rc, (i, v)
@@ -161,4 +160,4 @@ def test_packed_attention_wrapper_refusals():
         with pytest.raises(_err()):
             ops._packed_operands(q, k, v, cu, 4, 4, 64)
     with pytest.raises(_err(), match="all of dq"):
-        ops.attention_packed_bwd(b, b, b, b, b, b, cu, 4, 4, 64, 1.0, dq=b)
+        ops.attention_packed_bwd(b, b, b, b, b, ops.PackedStats(b, b), cu, 4, 4, 64, 1.0, dq=b)

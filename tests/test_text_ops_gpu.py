@@ -179,7 +179,7 @@ def _packed_inputs(lens, H, Hkv, d, pad=0, seed=0, gap=0):
 
 def _attention_ref(q, k, v, do, lens, H, Hkv, d, scale):
     """Outputs, log2-sum-exp and gradients by the formulas in 64 bits, each with its bound.  Roundings: P (2^-8 relative), the
-    output; in the backward P, dS, the forward's output inside delta, and the result.  2^-10 covers the fp32 scores and
+    output; in the backward P, dS, the forward's P inside delta, and the result.  2^-10 covers the fp32 scores and
     exponentials (128 products of at most 2^-24 of the sum of magnitudes, which is below 2^9 here)."""
     rows, G = q.shape[0], H // Hkv
     z = lambda h: torch.zeros(rows, h * d, dtype=F64, device="cuda")  # noqa: E731
@@ -203,7 +203,9 @@ def _attention_ref(q, k, v, do, lens, H, Hkv, d, scale):
             dp = D @ V.T
             delta = (D * O).sum(1, keepdim=True)
             ds = p * (dp - delta)
-            eds = (H16 + 2.0 ** -10) * ds.abs() + p * (D.abs() * to[r, a]).sum(1, keepdim=True) + 2.0 ** -10 * p * (dp.abs() + delta.abs())
+            # delta: the output as the kernel has it, before its rounding (and 2^-17 of that for the part kept beside it)
+            eds = (H16 + 2.0 ** -10) * ds.abs() + p * (D.abs() * (near + 2.0 ** -16 * O.abs())).sum(1, keepdim=True) \
+                + 2.0 ** -10 * p * (dp.abs() + delta.abs())
             dq[r, a] = scale * ds @ K
             tq[r, a] = scale * eds @ K.abs()
             dk[r, b] += scale * ds.T @ Q
@@ -230,11 +232,14 @@ def _check_attention(got, ref, what):
     _within(got["lse"][fin], ref["lse"][0][fin], 2.0 ** -10 + 2.0 ** -20 * ref["lse"][0][fin].abs(), f"{what} lse")
 
 
+NAMES = ("o", "lse", "dq", "dk", "dv")
+
+
 def _run_attention(q, k, v, do, cu, H, Hkv, d, scale):
     ops = _ops()
-    o, lse = ops.attention_packed(q, k, v, cu, H, Hkv, d, scale, with_lse=True)
-    dq, dk, dv = ops.attention_packed_bwd(q, k, v, o, do, lse, cu, H, Hkv, d, scale)
-    return {"o": o, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+    o, stats = ops.attention_packed(q, k, v, cu, H, Hkv, d, scale, with_lse=True)
+    dq, dk, dv = ops.attention_packed_bwd(q, k, v, o, do, stats, cu, H, Hkv, d, scale)
+    return {"o": o, "lse": stats.lse, "stats": stats, "dq": dq, "dk": dk, "dv": dv}
 
 
 LENS = [(1,), (2,), (31,), (32,), (33,), (77,), (63, 64, 65), (127, 128, 129), (0, 5, 0, 0, 77, 0), (256,), (257, 300), (511, 3, 640),
@@ -260,6 +265,21 @@ def test_packed_attention_head_layouts(cuda, H, Hkv, d):
     _check_attention(got, _attention_ref(q, k, v, do, lens, H, Hkv, d, 0.2), f"{H}/{Hkv}")
     for name in ("o", "dq", "dk", "dv"):
         assert (got[name][sum(lens):] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(4, 1), (6, 1), (8, 2), (6, 3)])
+def test_packed_attention_long_walks_of_few_key_heads(cuda, H, Hkv, d):
+    """Mean length of 512 and more: the walk over a group's query heads is cut into parts that are summed afterwards."""
+    lens = (700, 1200, 0, 513)
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, pad=77, seed=H + d)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, d ** -0.5)
+    _check_attention(got, _attention_ref(q, k, v, do, lens, H, Hkv, d, d ** -0.5), f"{H}/{Hkv}")
+    dq, dk, dv = (torch.full_like(got[x], 7.0) for x in ("dq", "dk", "dv"))
+    _ops().attention_packed_bwd(q, k, v, got["o"], do, got["stats"], cu, H, Hkv, d, d ** -0.5, dq=dq, dk=dk, dv=dv)
+    n = sum(lens)
+    for x, name in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
+        assert (got[name][n:] == 0).all() and (x[n:] == 7).all() and torch.equal(x[:n], got[name][:n])
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -289,7 +309,7 @@ def test_rows_behind_the_last_sequence(cuda, d):
     both = torch.full((n + 141, (H + 2 * Hkv) * d), 7.0, dtype=BF16, device="cuda")
     ops.attention_packed(q, k, v, cu, H, Hkv, d, 0.1, out=o)
     dq, dk, dv = both[:, :H * d], both[:, H * d:(H + Hkv) * d], both[:, (H + Hkv) * d:]
-    ops.attention_packed_bwd(q, k, v, got["o"], do, got["lse"], cu, H, Hkv, d, 0.1, dq=dq, dk=dk, dv=dv)
+    ops.attention_packed_bwd(q, k, v, got["o"], do, got["stats"], cu, H, Hkv, d, 0.1, dq=dq, dk=dk, dv=dv)
     for t, name in ((o, "o"), (dq, "dq"), (dk, "dk"), (dv, "dv")):
         assert torch.equal(t[:n], clean[name]) and (t[n:] == 7).all(), name
 
@@ -370,7 +390,7 @@ def test_packed_attention_repeats_bit_for_bit(cuda):
     lens = (300, 7, 129, 64)
     q, k, v, do, cu = _packed_inputs(lens, 8, 2, 64, seed=5)
     a, b = (_run_attention(q, k, v, do, cu, 8, 2, 64, 0.1) for _ in range(2))
-    assert all(torch.equal(a[x], b[x]) for x in a)
+    assert all(torch.equal(a[x], b[x]) for x in NAMES)
 
 
 def test_packed_attention_rows_past_two_gigabytes(cuda):
@@ -398,7 +418,7 @@ def test_packed_attention_offsets_that_are_wrong_stay_inside(cuda):
     q, k, v, do, _ = _packed_inputs((100,), 2, 2, 64, seed=1)
     ref = _run_attention(q, k, v, do, torch.tensor([0, 100], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
     got = _run_attention(q, k, v, do, torch.tensor([0, 5000], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
-    assert all(torch.equal(got[x], ref[x]) for x in ref)
+    assert all(torch.equal(got[x], ref[x]) for x in NAMES)
     got = _run_attention(q, k, v, do, torch.tensor([0, 100, 40], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
     assert torch.isfinite(got["o"]).all()
 
@@ -417,7 +437,7 @@ def test_packed_attention_in_a_graph_serves_other_lengths(cuda):
         graph.replay()
         torch.cuda.synchronize()
         ref = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
-        assert all(torch.equal(got[x], ref[x]) for x in ref), lens
+        assert all(torch.equal(got[x], ref[x]) for x in NAMES), lens
 
 
 # ------------------------------------------------------------------ gradient norm and clipping
@@ -556,4 +576,4 @@ def test_text_ops_on_another_stream(cuda):
                 got.append((ops.embedding_grad(ids, dy, 500), _run_attention(q, k, v, do, cu, 4, 4, 64, 0.1), ops.grad_norm(grads)))
     torch.cuda.synchronize()
     for g in got:
-        assert torch.equal(g[0], want[0]) and all(torch.equal(g[1][x], want[1][x]) for x in want[1]) and torch.equal(g[2], want[2])
+        assert torch.equal(g[0], want[0]) and all(torch.equal(g[1][x], want[1][x]) for x in NAMES) and torch.equal(g[2], want[2])

@@ -290,11 +290,16 @@ __device__ __forceinline__ float half_sum(float v) {
 }
 
 // ------------------------------------------------------------------ forward
-// A wave owns QB blocks of 32 queries; the workgroup's four waves walk the keys in tiles of 64 through a double-buffered stage.
+// A wave owns QB blocks of 32 queries and walks the keys in blocks of 32, staged as tiles of 64.  Step j of the walk takes the
+// scores of key block j, which the step before has left, through the softmax and into O, and computes the scores of block
+// j + 1 beside it: the two products of a step and its exponentials are independent, so that the matrix pipe and the vector
+// pipe, which need about 512 cycles a step each at d = 128, run at once.  Half way through a tile's two steps lies the fence at
+// which the next tile has landed (its keys are needed by the second step) and the tile after it is sent for: K in a ring of
+// two, V, which is needed a step longer, in a ring of three.
 template <int D, int QB>
 __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedArgs a) {
-    constexpr int BM = 128 * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TILEB];  // per stage: K, V
+    constexpr int BM = 128 * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[5 * TILEB];  // K 0, K 1, V 0, V 1, V 2
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
@@ -327,11 +332,10 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
         kd.init(wave, lane, ldkb);
         vd.init(wave, lane, ldvb);
         const unsigned lds0 = lds_addr(smem);
-        auto issue = [&](int t) {
-            const int left = tl.len - t * PA_TILE;
-            const unsigned st = lds0 + (t & 1) * 2 * TILEB;
-            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, min(left, PA_TILE), ldkb, ROWB), st);
-            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, min(left, PA_TILE), ldvb, ROWB), st + TILEB);
+        auto issue = [&](int t, int vslot) {
+            const int left = min(tl.len - t * PA_TILE, PA_TILE);
+            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, left, ldkb, ROWB), lds0 + (t & 1) * TILEB);
+            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, left, ldvb, ROWB), lds0 + (2 + vslot) * TILEB);
         };
         int kread[NK], vlo[ND], vhi[ND];
 #pragma unroll
@@ -339,59 +343,44 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, vlo[d], vhi[d]);
 
+        f32x16 s[QB];
+        auto scores = [&](f32x16 (&r)[QB], const char* kb, int X0) {  // of query blocks X0 .. with the key block at kb
+#pragma unroll
+            for (int X = X0; X < QB; ++X)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) r[X][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                const bf16x8 kf = *(const bf16x8*)(kb + kread[ks]);
+#pragma unroll
+                for (int X = X0; X < QB; ++X) r[X] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[X][ks], r[X], 0, 0, 0);
+            }
+        };
         bool bad = false;  // a value on this wave's diagonal that is not finite
-        // keys that the workgroup sees: up to its last query
-        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
-        // one 64-key tile: NB blocks of 32 keys of it are seen by some query of the wave; DIAG: block 32 X' on the diagonal
-        auto body = [&](int t, auto nb_c, auto diag_c) {
-            constexpr int NB = decltype(nb_c)::value;
-            constexpr bool DIAG = decltype(diag_c)::value;
-            const char* kb = smem + (t & 1) * 2 * TILEB;
-            const char* vb = kb + TILEB;
-            // block kbk against query block X: above the diagonal (skipped) or on it, where DIAG
-            auto hidden = [](int kbk, int X) { return DIAG && (QB == 1 ? false : kbk > X); };
-            auto ondiag = [](int kbk, int X) { return DIAG && (QB == 1 ? kbk == NB - 1 : kbk == X); };
-            f32x16 s[QB][NB];
+        // One step: vb = V of this key block, kn = K of the next.  X0: first query block that sees this key block; diag: the query
+        // block on the diagonal (-1: none); XN: first query block that sees the next one (QB: there is no next).
+        auto step = [&](const char* vb, const char* kn, auto x0_c, auto diag_c, auto xn_c) {
+            constexpr int X0 = decltype(x0_c)::value, DIAG = decltype(diag_c)::value, XN = decltype(xn_c)::value;
+            if constexpr (DIAG >= 0) {
 #pragma unroll
-            for (int kbk = 0; kbk < NB; ++kbk) {
-#pragma unroll
-                for (int X = 0; X < QB; ++X)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[X][kbk][e] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    const bf16x8 kf = *(const bf16x8*)(kb + kbk * 32 * ROWB + kread[ks]);
-#pragma unroll
-                    for (int X = 0; X < QB; ++X)
-                        if (!hidden(kbk, X)) s[X][kbk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[X][ks], s[X][kbk], 0, 0, 0);
-                }
-#pragma unroll
-                for (int X = 0; X < QB; ++X)
-                    if (ondiag(kbk, X)) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if ((e & 3) + 8 * (e >> 2) + 4 * hh > l31) s[X][kbk][e] = -INFINITY;
-                    }
+                for (int e = 0; e < 16; ++e)
+                    if ((e & 3) + 8 * (e >> 2) + 4 * hh > l31) s[DIAG][e] = -INFINITY;
             }
             // running maximum in the scaled log2 domain; kept while no row of the wave outgrows it by more than 2^6, so that the
             // rescaling of O and l is rare (P <= 64 stays exact in fp32, and its rounding to bf16 is relative)
             float mx[QB];
             bool grew = false;
 #pragma unroll
-            for (int X = 0; X < QB; ++X) {
+            for (int X = X0; X < QB; ++X) {
                 float m = -INFINITY;
 #pragma unroll
-                for (int kbk = 0; kbk < NB; ++kbk)
-                    if (!hidden(kbk, X)) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) m = fmaxf(m, s[X][kbk][e]);
-                    }
+                for (int e = 0; e < 16; ++e) m = fmaxf(m, s[X][e]);
                 mx[X] = half_max(m) * a.scale_log2e;
                 grew |= !(mx[X] - m_run[X] <= 6.0f);
             }
             if (__any(grew)) {
 #pragma unroll
-                for (int X = 0; X < QB; ++X) {
+                for (int X = X0; X < QB; ++X) {
                     const float m_new = fmaxf(m_run[X], mx[X]);
                     // a row that has seen only -inf scores keeps -inf as its maximum; its l stays 0 and its result 0 / 0
                     const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run[X] - m_new);
@@ -403,69 +392,100 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
                         for (int e = 0; e < 16; ++e) o[X][d][e] *= alpha;
                 }
             }
-            u32x4 pf[QB][NB][2];
+            f32x16 sn[QB];
+            if constexpr (XN < QB) scores(sn, kn, XN);
+            u32x4 pf[QB][2];
 #pragma unroll
-            for (int X = 0; X < QB; ++X) {
+            for (int X = X0; X < QB; ++X) {
                 const float m = m_run[X] == -INFINITY ? 0.f : m_run[X];
 #pragma unroll
-                for (int kbk = 0; kbk < NB; ++kbk)
-                    if (!hidden(kbk, X)) {
+                for (int sI = 0; sI < 2; ++sI) {
+                    float p[8];
 #pragma unroll
-                        for (int sI = 0; sI < 2; ++sI) {
-                            float p[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[X][kbk][8 * sI + j], a.scale_log2e, -m));
-                            l_run[X] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                            pf[X][kbk][sI] = pack8(p);
-                        }
-                    }
+                    for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[X][8 * sI + j], a.scale_log2e, -m));
+                    l_run[X] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    pf[X][sI] = pack8(p);
+                }
             }
+            u32x4 vf[ND][2];
 #pragma unroll
-            for (int kbk = 0; kbk < NB; ++kbk) {
-                u32x4 vf[ND][2];
+            for (int sI = 0; sI < 2; ++sI)
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+                    vf[d][sI] = __builtin_bit_cast(u32x4, tr_pair(vb + sI * 16 * ROWB + vlo[d], vb + sI * 16 * ROWB + vhi[d]));
+            auto pv = [&](int X) {
+#pragma unroll
+                for (int sI = 0; sI < 2; ++sI)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        o[X][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d][sI]), __builtin_bit_cast(bf16x8, pf[X][sI]),
+                                                                         o[X][d], 0, 0, 0);
+            };
+#pragma unroll
+            for (int X = X0; X < QB; ++X)
+                if (X != DIAG) pv(X);
+            if constexpr (DIAG >= 0) {
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int sI = 0; sI < 2; ++sI)
-                        vf[d][sI] = __builtin_bit_cast(u32x4, tr_pair(vb + (kbk * 32 + sI * 16) * ROWB + vlo[d], vb + (kbk * 32 + sI * 16) * ROWB + vhi[d]));
-                auto pv = [&](int X) {
+                    for (int sI = 0; sI < 2; ++sI) vf[d][sI] = finite_part(vf[d][sI], bad);
+                pv(DIAG);
+            }
+            if constexpr (XN < QB) {
 #pragma unroll
-                    for (int sI = 0; sI < 2; ++sI)
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-                            o[X][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d][sI]),
-                                                                             __builtin_bit_cast(bf16x8, pf[X][kbk][sI]), o[X][d], 0, 0, 0);
-                };
-#pragma unroll
-                for (int X = 0; X < QB; ++X)
-                    if (!hidden(kbk, X) && !ondiag(kbk, X)) pv(X);
-#pragma unroll
-                for (int X = 0; X < QB; ++X)
-                    if (ondiag(kbk, X)) {
-#pragma unroll
-                        for (int d = 0; d < ND; ++d)
-#pragma unroll
-                            for (int sI = 0; sI < 2; ++sI) vf[d][sI] = finite_part(vf[d][sI], bad);
-                        pv(X);
-                    }
+                for (int X = XN; X < QB; ++X) s[X] = sn[X];
             }
         };
+        using zero = std::integral_constant<int, 0>;
         using one = std::integral_constant<int, 1>;
-        using two = std::integral_constant<int, 2>;
-        const int dt = q0 / PA_TILE;  // the tile that holds the wave's diagonal
+        using none = std::integral_constant<int, -1>;
+        using end = std::integral_constant<int, QB>;
+        // keys that the workgroup sees: up to its last query; the wave's diagonal lies in key block jd
+        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
+        const int jd = q0 / 32, walk = q0 < tl.len ? jd / 2 : 0;  // tiles that the wave takes whole
 #pragma unroll
         for (int X = 0; X < QB; ++X) settle(qf[X]);
-        issue(0);
-        stage_fence();
-        for (int t = 0; t < ntiles; ++t) {
-            if (t + 1 < ntiles) issue(t + 1);
-            if (t < dt) body(t, two{}, std::false_type{});
-            else if (t == dt && q0 < tl.len) {
-                if (QB == 1 && !(q0 & 32)) body(t, one{}, std::true_type{});
-                else body(t, two{}, std::true_type{});
-            }
-            stage_fence();
+        issue(0, 0);
+        if (ntiles > 1) {
+            issue(1, 1);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        int v = 0, t = 0;  // ring slot of the tile's values, tile
+        auto fence = [&]() {  // tile t + 1 has landed, and what tile t + 2 overwrites is no longer read
+            stage_fence();
+            if (t + 2 < ntiles) issue(t + 2, v == 0 ? 2 : v - 1);
+        };
+        if (q0 < tl.len) scores(s, smem, 0);
+        for (; t < walk; ++t) {
+            const char* vb = smem + (2 + v) * TILEB;
+            step(vb, smem + (t & 1) * TILEB + BLOCKB, zero{}, none{}, zero{});
+            fence();
+            step(vb + BLOCKB, smem + ((t + 1) & 1) * TILEB, zero{}, none{}, zero{});
+            v = v == 2 ? 0 : v + 1;
+        }
+        if (q0 < tl.len) {  // the tile that holds the diagonal, in its first block or (QB 1, every other wave) its second
+            const char* vb = smem + (2 + v) * TILEB;
+            const char* kn = smem + (t & 1) * TILEB + BLOCKB;
+            if constexpr (QB == 2) {
+                step(vb, kn, zero{}, zero{}, one{});
+                fence();
+                step(vb + BLOCKB, kn, one{}, one{}, end{});
+            } else if (jd & 1) {
+                step(vb, kn, zero{}, none{}, zero{});
+                fence();
+                step(vb + BLOCKB, kn, zero{}, zero{}, end{});
+            } else {
+                step(vb, kn, zero{}, zero{}, end{});
+                fence();
+            }
+            v = v == 2 ? 0 : v + 1;
+            ++t;
+        }
+        for (; t < ntiles; ++t, v = v == 2 ? 0 : v + 1) fence();
         if (__any(bad)) {
 #pragma unroll
             for (int X = 0; X < QB; ++X) {

@@ -594,6 +594,11 @@ def axpy_f32(a: torch.Tensor, b: torch.Tensor, c: torch.Tensor) -> torch.Tensor:
 _F32_BF16 = {torch.float32: 0, BF16: 1}
 
 
+def _raw_stream() -> int:
+    """The current device's current stream, without the 2.5 us that building a torch.cuda.Stream object costs."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
 def _elsewhere(*ts: Optional[torch.Tensor]) -> bool:
     """Whether the operands live on another device than the current one (the op then runs with that device made current); raises
     where they are on the CPU or on different devices."""
@@ -641,7 +646,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype:
         out = torch.empty((T, Cc), dtype=dtype, device=table.device)
     ldo = _rows_ld(out, "out", T, Cc, _F32_BF16)
     _l.check(lib.ccnet_embedding(flat.data_ptr(), flat.element_size(), T, table.shape[0], table.data_ptr(), _F32_BF16[table.dtype],
-                                 ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, _stream()), "embedding")
+                                 ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, _raw_stream()), "embedding")
     return out
 
 
@@ -673,7 +678,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float
     ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device)
     _l.check(lib.ccnet_embedding_grad(flat.data_ptr(), flat.element_size(), T, vocab, dy.data_ptr(), _F32_BF16[dy.dtype], lddy, Cc,
                                       scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ldg, int(accumulate),
-                                      ws.data_ptr(), wsb, _stream()), "embedding_grad")
+                                      ws.data_ptr(), wsb, _raw_stream()), "embedding_grad")
     return out
 
 
@@ -706,7 +711,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         with torch.cuda.device(q.device):
             return attention_packed(q, k, v, cu_seqlens, H, Hkv, d, scale, with_lse, out)
     rows, (ldq, ldk, ldv) = _packed_operands(q, k, v, cu_seqlens, H, Hkv, d)
-    o = torch.empty((rows, H * d), dtype=BF16, device=q.device) if out is None else out
+    o = q.new_empty((rows, H * d)) if out is None else out
     stats = None
     if with_lse:
         stats = PackedStats(torch.empty((H, rows), dtype=torch.float32, device=q.device),
@@ -714,7 +719,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     _l.check(lib.ccnet_attention_packed_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(),
                                              _rows_ld(o, "out", rows, H * d, (BF16,)), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1,
                                              rows, H, Hkv, d, scale, int(out is None), stats.lse.data_ptr() if with_lse else None,
-                                             stats.o_low.data_ptr() if with_lse else None, _stream()), "attention_packed")
+                                             stats.o_low.data_ptr() if with_lse else None, _raw_stream()), "attention_packed")
     return (o, stats) if with_lse else o
 
 
@@ -746,7 +751,7 @@ def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
         q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), _rows_ld(o, "o", rows, H * d, (BF16,)), o_low.data_ptr(),
         do.data_ptr(), _rows_ld(do, "do", rows, H * d, (BF16,)), lse.data_ptr(), dq.data_ptr(), _rows_ld(dq, "dq", rows, H * d, (BF16,)),
         dk.data_ptr(), _rows_ld(dk, "dk", rows, Hkv * d, (BF16,)), dv.data_ptr(), _rows_ld(dv, "dv", rows, Hkv * d, (BF16,)),
-        cu_seqlens.data_ptr(), n_seq, rows, H, Hkv, d, scale, int(not given), ws.data_ptr(), wsb, _stream()), "attention_packed_bwd")
+        cu_seqlens.data_ptr(), n_seq, rows, H, Hkv, d, scale, int(not given), ws.data_ptr(), wsb, _raw_stream()), "attention_packed_bwd")
     return dq, dk, dv
 
 
@@ -805,7 +810,7 @@ def grad_norm(grads) -> torch.Tensor:
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
     ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), _stream()), "grad_norm")
+    _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()), "grad_norm")
     return norm
 
 
@@ -824,7 +829,7 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
     ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _stream()),
+    _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()),
              "clip_grad_norm")
     return norm
 
@@ -839,7 +844,7 @@ def clip_grad_value(grads, limit: float, out=None) -> None:
     if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
         with torch.cuda.device(grads[0].device):
             return clip_grad_value(grads, limit, None if out is None else outs)
-    _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _stream()), "clip_grad_value")
+    _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _raw_stream()), "clip_grad_value")
 
 
 _prof_on = False

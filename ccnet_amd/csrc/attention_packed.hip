@@ -508,12 +508,13 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
 }
 
 // ------------------------------------------------------------------ backward: dQ (and delta)
-// The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, dQ^T += K^T dS^T from transposed
-// reads of the same K tile.  delta is taken from the wave's own dO and O rows and left for the dK / dV kernel.
+// The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
+// from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
+// and left for the dK / dV kernel.
 template <int D>
 __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
-    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * TILEB];  // per stage: K, V
+    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+    __shared__ __attribute__((aligned(1024))) char smem[5 * TILEB];  // V 0, V 1, K 0, K 1, K 2
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
@@ -534,9 +535,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         float dlt = 0.f;
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) {
-            u32x4 ov = {0u, 0u, 0u, 0u};
+            u32x4 ov = {0u, 0u, 0u, 0u}, lv = {0u, 0u, 0u, 0u};
             if (qok) ov = *(const u32x4*)(a.O + row * a.ldo + h * D + ks * 16 + hh * 8);
-            u32x4 lv = {0u, 0u, 0u, 0u};
             if (qok && a.o_low) lv = *(const u32x4*)(a.o_low + (row * a.H + h) * D + ks * 16 + hh * 8);
             float x[8], l[8], y[8];
             unpack8(ov, x);
@@ -556,28 +556,32 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         kd.init(wave, lane, ldkb);
         vd.init(wave, lane, ldvb);
         const unsigned lds0 = lds_addr(smem);
-        auto issue = [&](int t) {
-            const int left = tl.len - t * PA_TILE;
-            const unsigned st = lds0 + (t & 1) * 2 * TILEB;
-            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, min(left, PA_TILE), ldkb, ROWB), st);
-            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, min(left, PA_TILE), ldvb, ROWB), st + TILEB);
+        auto issue = [&](int t, int kslot) {
+            const int left = min(tl.len - t * PA_TILE, PA_TILE);
+            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, left, ldkb, ROWB), lds0 + (2 + kslot) * TILEB);
+            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, left, ldvb, ROWB), lds0 + (t & 1) * TILEB);
         };
         int rread[NK], klo[ND], khi[ND];
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, klo[d], khi[d]);
-        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
-        auto block = [&](const char* kb, const char* vb, auto diag_c) {
-            constexpr bool DIAG = decltype(diag_c)::value;
-            f32x16 s, dp;
+        f32x16 s, dp;
+        auto scores = [&](f32x16& sr, f32x16& dr, const char* kb, const char* vb) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = 0.f; }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kb + rread[ks]), qf[ks], s, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vb + rread[ks]), dof[ks], dp, 0, 0, 0);
+                sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kb + rread[ks]), qf[ks], sr, 0, 0, 0);
+                dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vb + rread[ks]), dof[ks], dr, 0, 0, 0);
             }
+        };
+        // kb: K of this key block; kn, vn: K and V of the next
+        auto step = [&](const char* kb, const char* kn, const char* vn, auto diag_c, auto next_c) {
+            constexpr bool DIAG = decltype(diag_c)::value, NEXT = decltype(next_c)::value;
+            f32x16 sn, dpn;
+            if constexpr (NEXT) scores(sn, dpn, kn, vn);
+            bf16x8 dsf[2];
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI) {
                 float ds[8];
@@ -587,42 +591,70 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
                     ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dlt);
                     if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > l31) ds[j] = 0.f;
                 }
-                const bf16x8 dsf = __builtin_bit_cast(bf16x8, pack8(ds));
+                dsf[sI] = __builtin_bit_cast(bf16x8, pack8(ds));
+            }
+#pragma unroll
+            for (int sI = 0; sI < 2; ++sI)
 #pragma unroll
                 for (int d = 0; d < ND; ++d)
-                    dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(kb + sI * 16 * ROWB + klo[d], kb + sI * 16 * ROWB + khi[d]), dsf, dq[d], 0, 0, 0);
-            }
+                    dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(kb + sI * 16 * ROWB + klo[d], kb + sI * 16 * ROWB + khi[d]), dsf[sI], dq[d], 0, 0, 0);
+            if constexpr (NEXT) { s = sn; dp = dpn; }
         };
+        const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
+        const int jd = q0 / 32, walk = q0 < tl.len ? jd / 2 : 0;
         settle(qf);
         settle(dof);
         asm volatile("" : "+v"(lse), "+v"(dlt));
-        issue(0);
-        stage_fence();
-        for (int t = 0; t < ntiles; ++t) {
-            if (t + 1 < ntiles) issue(t + 1);
-            const char* kb = smem + (t & 1) * 2 * TILEB;
-            const char* vb = kb + TILEB;
-            if (q0 < tl.len) {
-#pragma unroll 1
-                for (int kbk = 0; kbk < 2; ++kbk) {
-                    const int k0 = t * PA_TILE + kbk * 32;
-                    if (k0 < q0) block(kb + kbk * 32 * ROWB, vb + kbk * 32 * ROWB, std::false_type{});
-                    else if (k0 == q0) block(kb + kbk * 32 * ROWB, vb + kbk * 32 * ROWB, std::true_type{});
-                }
-            }
-            stage_fence();
+        issue(0, 0);
+        if (ntiles > 1) {
+            issue(1, 1);
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        int kslot = 0, t = 0;
+        auto next_slot = [&]() { return kslot == 2 ? 0 : kslot + 1; };
+        auto fence = [&]() {  // tile t + 1 has landed, and what tile t + 2 overwrites is no longer read
+            stage_fence();
+            if (t + 2 < ntiles) issue(t + 2, kslot == 0 ? 2 : kslot - 1);
+        };
+        if (q0 < tl.len) scores(s, dp, smem + 2 * TILEB, smem);
+        for (; t < walk; ++t) {
+            const char* kb = smem + (2 + kslot) * TILEB;
+            step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{});
+            fence();
+            step(kb + BLOCKB, smem + (2 + next_slot()) * TILEB, smem + ((t + 1) & 1) * TILEB, std::false_type{}, std::true_type{});
+            kslot = next_slot();
+        }
+        if (q0 < tl.len) {
+            const char* kb = smem + (2 + kslot) * TILEB;
+            if (jd & 1) {
+                step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{});
+                fence();
+                step(kb + BLOCKB, nullptr, nullptr, std::true_type{}, std::false_type{});
+            } else {
+                step(kb, nullptr, nullptr, std::true_type{}, std::false_type{});
+                fence();
+            }
+            kslot = next_slot();
+            ++t;
+        }
+        for (; t < ntiles; ++t, kslot = next_slot()) fence();
     }
     store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, qok);
 }
 
 // ------------------------------------------------------------------ backward: dK, dV
-// A wave owns 32 keys of a key head; the workgroup walks the query tiles from its own diagonal on, for every query head of the
-// group in turn, so the group's sum is taken in the accumulators, in a fixed order.
+// A wave owns 32 keys of a key head; the workgroup walks the query tiles from its own diagonal on, for the query heads of the
+// group (or of its part of it) in turn, so the group's sum is taken in the accumulators, in a fixed order.  As above the scores
+// of the next query block are computed beside the exponentials of this one; Q and dO are both needed a step longer (rings of
+// three).  Query blocks in front of a wave's own keys (in the first two tiles of a head) are masked whole.
 template <int D>
 __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
-    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, STAGEB = 2 * TILEB + 512;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * STAGEB];  // per stage: Q, dO, lse and delta of the 64 queries
+    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, STAGEB = 2 * TILEB + 512;
+    __shared__ __attribute__((aligned(1024))) char smem[3 * STAGEB];  // per stage: Q, dO, lse and delta of the 64 queries
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
@@ -647,34 +679,49 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
         qd.init(wave, lane, ldqb);
         dd.init(wave, lane, lddob);
         const unsigned lds0 = lds_addr(smem);
-        const int t0 = tl.tile * BM / PA_TILE, per_head = (tl.len + PA_TILE - 1) / PA_TILE - t0;
-        auto issue = [&](int i) {  // step i of the walk: head i / per_head of the group, query tile t0 + i % per_head
-            const int g = i / per_head, t = t0 + i - g * per_head, h = h0 + g;
+        const int t0 = tl.tile * BM / PA_TILE, per_head = (tl.len + PA_TILE - 1) / PA_TILE - t0, steps = per_head * G;
+        int ig = 0, it = 0, islot = 0, issued = 0;  // next tile to send for: head of the part, tile behind t0, ring slot
+        auto issue = [&]() {
+            if (issued == steps) return;
+            const int h = h0 + ig, t = t0 + it, left = min(tl.len - t * PA_TILE, PA_TILE);
             const long long r0 = (long long)tl.start + t * PA_TILE;
-            const int left = min(tl.len - t * PA_TILE, PA_TILE);
-            const unsigned st = lds0 + (i & 1) * STAGEB;
+            const unsigned st = lds0 + islot * STAGEB;
             qd.issue(row_rsrc((const char*)(a.Q + r0 * a.ldq + h * D), left, ldqb, ROWB), st);
             dd.issue(row_rsrc((const char*)(a.dO + r0 * a.lddo + h * D), left, lddob, ROWB), st + TILEB);
             if (wave < 2) {  // queries behind the end read as lse = delta = 0, q = dO = 0: P = 1 meets only zeros
                 const float* p = (wave == 0 ? a.lse : a.delta) + (long long)h * a.rows + r0;
                 dma4(row_rsrc((const char*)p, left, 4, 4), st + 2 * TILEB + wave * 256, lane * 4);
             }
+            ++issued;
+            islot = islot == 2 ? 0 : islot + 1;
+            if (++it == per_head) { it = 0; ++ig; }
         };
         int rread[NK], tlo[ND], thi[ND];
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, tlo[d], thi[d]);
-        auto block = [&](const char* qb, const char* db, const float* stat, auto diag_c) {
-            constexpr bool DIAG = decltype(diag_c)::value;
-            f32x16 s, dp;
+        f32x16 s, dp;
+        auto scores = [&](f32x16& sr, f32x16& dr, const char* qb) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { s[e] = 0.f; dp[e] = 0.f; }
+            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = 0.f; }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], s, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(db + rread[ks]), vf[ks], dp, 0, 0, 0);
+                sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], sr, 0, 0, 0);
+                dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + TILEB + rread[ks]), vf[ks], dr, 0, 0, 0);
             }
+        };
+        // qb: Q of this query block (dO a tile behind it), stat: its lse and delta, rel: its index counted from the wave's diagonal,
+        // qn: Q of the next block
+        auto step = [&](const char* qb, const float* stat, int rel, const char* qn) {
+            if (rel <= 0) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (rel * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
+            }
+            f32x16 sn, dpn;
+            scores(sn, dpn, qn);
+            bf16x8 pfr[2], dsf[2];
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI) {
                 float p[8], ds[8];
@@ -685,40 +732,42 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int e = 8 * sI + 4 * g + j;
-                        float pe = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -l4[j]));
-                        float de = pe * (dp[e] - d4[j]);
-                        if (DIAG && qo + j < l31) { pe = 0.f; de = 0.f; }
-                        p[4 * g + j] = pe;
-                        ds[4 * g + j] = de;
+                        p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -l4[j]));
+                        ds[4 * g + j] = p[4 * g + j] * (dp[e] - d4[j]);
                     }
                 }
-                const bf16x8 pfr = __builtin_bit_cast(bf16x8, pack8(p)), dsf = __builtin_bit_cast(bf16x8, pack8(ds));
+                pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
+                dsf[sI] = __builtin_bit_cast(bf16x8, pack8(ds));
+            }
+#pragma unroll
+            for (int sI = 0; sI < 2; ++sI)
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(db + sI * 16 * ROWB + tlo[d], db + sI * 16 * ROWB + thi[d]), pfr, dv[d], 0, 0, 0);
-                    dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(qb + sI * 16 * ROWB + tlo[d], qb + sI * 16 * ROWB + thi[d]), dsf, dk[d], 0, 0, 0);
+                    const char* x = qb + sI * 16 * ROWB;
+                    dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + TILEB + tlo[d], x + TILEB + thi[d]), pfr[sI], dv[d], 0, 0, 0);
+                    dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + tlo[d], x + thi[d]), dsf[sI], dk[d], 0, 0, 0);
                 }
-            }
+            s = sn;
+            dp = dpn;
         };
-        const int steps = per_head * G;
         settle(kf);
         settle(vf);
-        issue(0);
+        issue();
         stage_fence();
-        for (int i = 0, t = t0; i < steps; ++i, t = t + 1 == t0 + per_head ? t0 : t + 1) {
-            if (i + 1 < steps) issue(i + 1);
-            const char* qb = smem + (i & 1) * STAGEB;
-            const char* db = qb + TILEB;
-            const float* stat = (const float*)(db + TILEB);
-            if (k0 < tl.len) {
-#pragma unroll
-                for (int qbk = 0; qbk < 2; ++qbk) {
-                    const int q0 = t * PA_TILE + qbk * 32;
-                    if (q0 > k0) block(qb + qbk * 32 * ROWB, db + qbk * 32 * ROWB, stat + qbk * 32, std::false_type{});
-                    else if (q0 == k0) block(qb + qbk * 32 * ROWB, db + qbk * 32 * ROWB, stat + qbk * 32, std::true_type{});
-                }
-            }
-            stage_fence();
+        issue();  // (the first fence of the walk waits for it)
+        scores(s, dp, smem);
+        int slot = 0, rel = -wave;
+        for (int i = 0, it2 = 0; i < steps; ++i) {
+            const char* qb = smem + slot * STAGEB;
+            const float* stat = (const float*)(qb + 2 * TILEB);
+            slot = slot == 2 ? 0 : slot + 1;
+            step(qb, stat, rel, qb + BLOCKB);
+            stage_fence();  // tile i + 1 has landed; tile i + 2 may overwrite tile i - 1
+            issue();
+            // (behind the last tile: the slot that was read two tiles ago, or nothing yet; its scores are not used)
+            step(qb + BLOCKB, stat + 32, rel + 1, smem + slot * STAGEB);
+            rel += 2;
+            if (++it2 == per_head) { it2 = 0; rel = -wave; }
         }
     }
     if (a.parts > 1) {

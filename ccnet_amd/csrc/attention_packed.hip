@@ -87,10 +87,27 @@ __device__ __forceinline__ u32x4 row_rsrc(const char* base, int rows, long long 
 
 struct Tile { int start, len, tile, ntiles; bool tail; };
 
+// sum and maximum over the wave by row shifts and broadcasts (six vector instructions; a shuffle through LDS takes as long as
+// all of them); values are not negative
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true); }
 __device__ __forceinline__ int wave_isum(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return __builtin_amdgcn_readfirstlane(v);
+    v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ int wave_imax(int v) {
+    v = max(v, dpp<0x111, 0xf>(v));
+    v = max(v, dpp<0x112, 0xf>(v));
+    v = max(v, dpp<0x114, 0xf>(v));
+    v = max(v, dpp<0x118, 0xf>(v));
+    v = max(v, dpp<0x142, 0xa>(v));
+    v = max(v, dpp<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // Tile `idx` of the tiles of `step` rows that the sequences have together, ordered by level: first every sequence's tile with
@@ -98,7 +115,8 @@ __device__ __forceinline__ int wave_isum(int v) {
 // f(L) = sum_i max(0, ntiles_i - L), falling in L, so a bisection finds the level and a ballot the sequence.  Sequence n_seq
 // stands for the rows behind the last one (when they are to be written).  Offsets are clamped to [0, rows] and to rising
 // order: wrong ones give wrong results but no access outside.  False: there is no such tile.
-__device__ bool find_tile(const PackedArgs& a, int idx, int step, bool from_end, Tile& t) {
+template <int step>
+__device__ __forceinline__ bool find_tile(const PackedArgs& a, int idx, bool from_end, Tile& t) {
     const int lane = threadIdx.x & 63, n = a.n_seq + 1;
     auto span = [&](int i, int& s) {
         if (i >= n) { s = 0; return 0; }
@@ -107,7 +125,7 @@ __device__ bool find_tile(const PackedArgs& a, int idx, int step, bool from_end,
         return e - s;
     };
     int s0;
-    const int nt0 = (span(lane, s0) + step - 1) / step;  // the first 64 sequences stay in registers
+    const int len0 = span(lane, s0), nt0 = (len0 + step - 1) / step;  // the first 64 sequences stay in registers
     auto total = [&](int L) {
         int v = max(0, nt0 - L);
         for (int i = lane + 64; i < n; i += 64) {
@@ -117,17 +135,12 @@ __device__ bool find_tile(const PackedArgs& a, int idx, int step, bool from_end,
         return wave_isum(v);
     };
     if (total(0) <= idx) return false;
-    int lo = 0, hi = (a.rows + step - 1) / step;  // f(lo) > idx >= f(hi) = 0
-    {
-        int m = nt0;
-        for (int i = lane + 64; i < n; i += 64) {
-            int s;
-            m = max(m, (span(i, s) + step - 1) / step);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
-        hi = __builtin_amdgcn_readfirstlane(m);
+    int m = nt0;
+    for (int i = lane + 64; i < n; i += 64) {
+        int s;
+        m = max(m, (span(i, s) + step - 1) / step);
     }
+    int lo = 0, hi = wave_imax(m);  // f(lo) > idx >= f(hi) = 0
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (total(mid) > idx) lo = mid;
@@ -135,8 +148,8 @@ __device__ bool find_tile(const PackedArgs& a, int idx, int step, bool from_end,
     }
     int rank = idx - total(lo + 1);
     for (int i0 = 0; i0 < n; i0 += 64) {
-        int s = s0, len = 0;
-        len = span(i0 + lane, s);
+        int s = s0, len = len0;
+        if (i0 > 0) len = span(i0 + lane, s);
         const int nt = (len + step - 1) / step;
         const unsigned long long has = __ballot(nt > lo);
         const int c = __popcll(has);
@@ -303,7 +316,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
-    if (!find_tile(a, blockIdx.x / a.H, BM, false, tl)) return;
+    if (!find_tile<BM>(a, blockIdx.x / a.H, false, tl)) return;
     const int h = head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), kvh = h / (a.H / a.Hkv);
     const int q0 = tl.tile * BM + wave * 32 * QB;  // in the sequence
 
@@ -443,9 +456,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
         // keys that the workgroup sees: up to its last query; the wave's diagonal lies in key block jd
         const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
         const int jd = q0 / 32, walk = q0 < tl.len ? jd / 2 : 0;  // tiles that the wave takes whole
+        issue(0, 0);
 #pragma unroll
         for (int X = 0; X < QB; ++X) settle(qf[X]);
-        issue(0, 0);
         if (ntiles > 1) {
             issue(1, 1);
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
@@ -518,7 +531,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
-    if (!find_tile(a, blockIdx.x / a.H, BM, false, tl)) return;
+    if (!find_tile<BM>(a, blockIdx.x / a.H, false, tl)) return;
     const int h = head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), kvh = h / (a.H / a.Hkv);
     const int q0 = tl.tile * BM + wave * 32, q = q0 + l31;
     const bool qok = q < tl.len;
@@ -532,6 +545,19 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         bf16x8 qf[NK], dof[NK];
         load_frags<D>(qf, a.Q + row * a.ldq + h * D, hh, qok);
         load_frags<D>(dof, a.dO + row * a.lddo + h * D, hh, qok);
+        const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
+        const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
+        const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
+        TileDma<D> kd, vd;
+        kd.init(wave, lane, ldkb);
+        vd.init(wave, lane, ldvb);
+        const unsigned lds0 = lds_addr(smem);
+        auto issue = [&](int t, int kslot) {
+            const int left = min(tl.len - t * PA_TILE, PA_TILE);
+            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, left, ldkb, ROWB), lds0 + (2 + kslot) * TILEB);
+            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, left, ldvb, ROWB), lds0 + (t & 1) * TILEB);
+        };
+        issue(0, 0);
         float dlt = 0.f;
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) {
@@ -546,21 +572,8 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
             for (int j = 0; j < 8; ++j) dlt = fmaf(x[j] + l[j], y[j], dlt);
         }
         dlt = half_sum(dlt);
-        if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = dlt;
+        if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = -dlt;  // (negative: where dP starts from)
         float lse = qok ? a.lse[(long long)h * a.rows + row] : 0.f;
-
-        const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
-        const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
-        const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
-        TileDma<D> kd, vd;
-        kd.init(wave, lane, ldkb);
-        vd.init(wave, lane, ldvb);
-        const unsigned lds0 = lds_addr(smem);
-        auto issue = [&](int t, int kslot) {
-            const int left = min(tl.len - t * PA_TILE, PA_TILE);
-            kd.issue(row_rsrc(kbase + (long long)t * PA_TILE * ldkb, left, ldkb, ROWB), lds0 + (2 + kslot) * TILEB);
-            vd.issue(row_rsrc(vbase + (long long)t * PA_TILE * ldvb, left, ldvb, ROWB), lds0 + (t & 1) * TILEB);
-        };
         int rread[NK], klo[ND], khi[ND];
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
@@ -605,7 +618,6 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         settle(qf);
         settle(dof);
         asm volatile("" : "+v"(lse), "+v"(dlt));
-        issue(0, 0);
         if (ntiles > 1) {
             issue(1, 1);
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
@@ -659,7 +671,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
     const int l31 = lane & 31, hh = lane >> 5;
     Tile tl;
     const int units = a.Hkv * a.parts;
-    if (!find_tile(a, blockIdx.x / units, BM, true, tl)) return;
+    if (!find_tile<BM>(a, blockIdx.x / units, true, tl)) return;
     const int kvh = blockIdx.x % a.Hkv, part = blockIdx.x % units / a.Hkv, G = a.H / a.Hkv / a.parts, h0 = (kvh * a.parts + part) * G;
     if (a.parts > 1 && tl.tail) return;  // (packed_join_kernel's)
     const int k0 = tl.tile * BM + wave * 32, key = k0 + l31;
@@ -702,9 +714,13 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, tlo[d], thi[d]);
         f32x16 s, dp;
-        auto scores = [&](f32x16& sr, f32x16& dr, const char* qb) {
+        auto scores = [&](f32x16& sr, f32x16& dr, const char* qb, const float* stat) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = 0.f; }
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 d4 = *(const f32x4*)(stat + 64 + 8 * g + 4 * hh);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { sr[4 * g + j] = 0.f; dr[4 * g + j] = d4[j]; }
+            }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
                 sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], sr, 0, 0, 0);
@@ -713,14 +729,14 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
         };
         // qb: Q of this query block (dO a tile behind it), stat: its lse and delta, rel: its index counted from the wave's diagonal,
         // qn: Q of the next block
-        auto step = [&](const char* qb, const float* stat, int rel, const char* qn) {
+        auto step = [&](const char* qb, const float* stat, int rel, const char* qn, const float* statn) {
             if (rel <= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (rel * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
             }
             f32x16 sn, dpn;
-            scores(sn, dpn, qn);
+            scores(sn, dpn, qn, statn);
             bf16x8 pfr[2], dsf[2];
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI) {
@@ -728,12 +744,12 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const int qo = 16 * sI + 8 * g + 4 * hh;  // registers 8 sI + 4 g .. + 3: four consecutive queries
-                    const f32x4 l4 = *(const f32x4*)(stat + qo), d4 = *(const f32x4*)(stat + 64 + qo);
+                    const f32x4 l4 = *(const f32x4*)(stat + qo);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int e = 8 * sI + 4 * g + j;
                         p[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -l4[j]));
-                        ds[4 * g + j] = p[4 * g + j] * (dp[e] - d4[j]);
+                        ds[4 * g + j] = p[4 * g + j] * dp[e];
                     }
                 }
                 pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
@@ -750,22 +766,22 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
             s = sn;
             dp = dpn;
         };
+        issue();
         settle(kf);
         settle(vf);
-        issue();
         stage_fence();
         issue();  // (the first fence of the walk waits for it)
-        scores(s, dp, smem);
+        scores(s, dp, smem, (const float*)(smem + 2 * TILEB));
         int slot = 0, rel = -wave;
         for (int i = 0, it2 = 0; i < steps; ++i) {
             const char* qb = smem + slot * STAGEB;
             const float* stat = (const float*)(qb + 2 * TILEB);
             slot = slot == 2 ? 0 : slot + 1;
-            step(qb, stat, rel, qb + BLOCKB);
+            step(qb, stat, rel, qb + BLOCKB, stat + 32);
             stage_fence();  // tile i + 1 has landed; tile i + 2 may overwrite tile i - 1
             issue();
             // (behind the last tile: the slot that was read two tiles ago, or nothing yet; its scores are not used)
-            step(qb + BLOCKB, stat + 32, rel + 1, smem + slot * STAGEB);
+            step(qb + BLOCKB, stat + 32, rel + 1, smem + slot * STAGEB, (const float*)(smem + slot * STAGEB + 2 * TILEB));
             rel += 2;
             if (++it2 == per_head) { it2 = 0; rel = -wave; }
         }
@@ -819,12 +835,12 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
 // Into how many parts the walk of a key tile over its group's query heads is cut.  One workgroup walks G heads x the queries
 // behind its keys; with few key heads and long sequences the longest of those walks outlasts the rest of the grid.  Parts cost
 // fp32 sums through memory (16 bytes a channel), so only walks of at least 8 tiles a head on average are cut, and only while the
-// grid has fewer than 2048 workgroups (four rounds of 512).
+// grid has fewer than 768 workgroups (three a CU).
 int parts_of(int n_seq, int rows, int H, int Hkv) {
     const int G = H / Hkv;
     if (rows < 512ll * (n_seq > 0 ? n_seq : 1)) return 1;
     int p = 1;
-    while (p < G && most_tiles(rows, n_seq, 128, 0) * Hkv * p < 2048) {
+    while (p < G && most_tiles(rows, n_seq, 128, 0) * Hkv * p < 768) {
         do ++p;
         while (G % p);
     }

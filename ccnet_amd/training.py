@@ -412,6 +412,56 @@ class Tape:
         self.steps.append(bw)
         return out
 
+    # ---- token lookup
+    def embedding(self, ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, param: Optional[nn.Parameter] = None,
+                  padding_idx: Optional[int] = None) -> Var:
+        """scale * table[ids] as bf16 rows [ids.numel(), C]; `param`: the parameter behind `table`, whose gradient (fp32, summed in
+        the order of the positions) is added up where several lookups share it."""
+        y = ops.embedding(ids, table, scale=scale)
+        want = param is not None and param.requires_grad
+        out = _v2d(y, want)
+        if not want:
+            return out
+
+        def bw():
+            if out.g is None:
+                return
+            have = self.grads.get(param)
+            g = ops.embedding_grad(ids, out.g, table.shape[0], scale=scale, padding_idx=padding_idx,
+                                   out=have, accumulate=have is not None)
+            self.grads[param] = g
+
+        self.steps.append(bw)
+        return out
+
+    # ---- causal attention over packed sequences, grouped heads (head dim 64 or 128)
+    def attention_packed(self, q: Var, q_off: int, kv: Var, k_off: int, v_off: int, cu_seqlens: torch.Tensor, H: int, Hkv: int, d: int,
+                         scale: float) -> Var:
+        """Causal self-attention of every sequence cu_seqlens[i] .. cu_seqlens[i+1] of the rows; q = q.a.t[:, q_off : q_off + H d],
+        k / v columns of kv.a.t (Hkv d each).  The gradients go straight into the column slices of gradient buffers that nothing
+        else has written yet, and are added where something has."""
+        views = (q.a.t[:, q_off:q_off + H * d], kv.a.t[:, k_off:k_off + Hkv * d], kv.a.t[:, v_off:v_off + Hkv * d])
+        rg = q.rg or kv.rg
+        o = ops.attention_packed(*views, cu_seqlens, H, Hkv, d, scale, with_lse=rg)
+        if not rg:
+            return _v2d(o, False)
+        o, stats = o
+        out = Var(Act(o, q.a.N, q.a.H, q.a.W, H * d), True)
+
+        def bw():
+            if out.g is None:
+                return
+            places = ((q, q_off, H * d), (kv, k_off, Hkv * d), (kv, v_off, Hkv * d))
+            if q.g is None and kv.g is None and q.rg and kv.rg:
+                into = [v.grad_buf()[:, c:c + n] for v, c, n in places]
+                ops.attention_packed_bwd(*views, o, out.g, stats, cu_seqlens, H, Hkv, d, scale, *into)
+            else:
+                for (v, c, _), g in zip(places, ops.attention_packed_bwd(*views, o, out.g, stats, cu_seqlens, H, Hkv, d, scale)):
+                    v.accumulate(g, c)
+
+        self.steps.append(bw)
+        return out
+
 
 # ================================================================================================ network lowering
 class _Net:
@@ -507,12 +557,14 @@ def _embedding(T: Tape, nt: _Net, timesteps, class_labels, B: int):
     if net.num_class_embeds is not None:
         if class_labels is None:
             raise ValueError("class_labels should be provided when num_class_embeds > 0")
-        if "class_table" in pk:
-            raise CcnetError("training lowering: nn.Embedding class conditioning has no backward here")
-        cl = class_labels.to(device=dev, dtype=torch.float32).reshape(B, 1).contiguous()
-        c1_pre = ops.linear_f32(cl, pk["ce0"][0], pk["ce0"][1])
-        c1 = torch.nn.functional.silu(c1_pre)
-        e = e + ops.linear_f32(c1, pk["ce2"][0], pk["ce2"][1])
+        if "class_table" in pk:  # nn.Embedding: one row per class, the labels are its indices
+            cl = class_labels.to(dev).long().reshape(-1)
+            e = e + ops.embedding(cl, pk["class_table"], dtype=torch.float32)
+        else:
+            cl = class_labels.to(device=dev, dtype=torch.float32).reshape(B, 1).contiguous()
+            c1_pre = ops.linear_f32(cl, pk["ce0"][0], pk["ce0"][1])
+            c1 = torch.nn.functional.silu(c1_pre)
+            e = e + ops.linear_f32(c1, pk["ce2"][0], pk["ce2"][1])
     semb = torch.nn.functional.silu(e)
     tall = ops.linear_f32(semb, pk["tproj_w"], pk["tproj_b"])
     if not nt.trainable:
@@ -549,6 +601,9 @@ def _embedding(T: Tape, nt: _Net, timesteps, class_labels, B: int):
         _, dw, db = lin_bw(dh * dsilu(h_pre), t_emb, pk["te0"][0])
         T.add_grad(net.time_embed[0].weight, dw)
         T.add_grad(net.time_embed[0].bias, db)
+        if "class_table" in pk:
+            table = net.class_embedding
+            T.add_grad(table.weight, ops.embedding_grad(cl, de.contiguous(), table.weight.shape[0], padding_idx=table.padding_idx))
         if c1 is not None:
             dc1, dw, db = lin_bw(de, c1, pk["ce2"][0])
             T.add_grad(net.class_embedding[2].weight, dw)
@@ -559,6 +614,19 @@ def _embedding(T: Tape, nt: _Net, timesteps, class_labels, B: int):
 
     T.steps.append(bw)
     return tall, dtall
+
+
+def _check_class_labels(nets: Sequence[_Net], class_labels: Optional[torch.Tensor], B: int) -> None:
+    """Labels that index a class table are read here, on the host, before any network runs on them: the sampler's own forward
+    (the frozen UNet's encoder) gathers its table's rows without a check of its own."""
+    tables = [nt.pk["class_table"].shape[0] for nt in nets if "class_table" in nt.pk]
+    if not tables or class_labels is None:
+        return
+    if class_labels.numel() != B:
+        raise ValueError(f"class_labels must have {B} elements, got {class_labels.numel()}")
+    lo, hi = (int(v) for v in torch.stack(torch.aminmax(class_labels.long())).tolist())
+    if lo < 0 or hi >= min(tables):
+        raise IndexError(f"class_labels from {lo} to {hi} in a class table of {min(tables)} rows")
 
 
 def _conv_in(T: Tape, nt: _Net, x: torch.Tensor, B: int, w, b, conv: nn.Conv2d, cout: int, ldo: int, res: Optional[Var]) -> Var:
@@ -640,6 +708,7 @@ def controlnet_unet_forward(T: Tape, controlnet, unet, noisy_e: torch.Tensor, ti
     x = noisy_e.contiguous().float()
     B = x.shape[0]
     dev = x.device
+    _check_class_labels((cn, un), class_labels, B)
     # frozen UNet: encoder + middle block without a tape (they depend on neither the ControlNet nor a trainable parameter)
     ust = unet.encode_phase(x, timesteps, context, class_labels)
     # ControlNet under the tape
@@ -765,21 +834,26 @@ def train_step(controlnet, unet, scheduler, optimizer, e, noise, timesteps, cond
             p.grad = grads.get(p)  # None where the tape recorded no gradient
             if p.grad is not None:
                 with_grad.append(p)
-    # one fused finite-ness test over the loss and every gradient (what GradScaler.unscale_ records as found_inf)
-    norms = torch._foreach_norm([p.grad for p in with_grad]) if with_grad else []
-    total = torch.linalg.vector_norm(torch.stack([n.float() for n in norms])) if norms else loss.new_zeros(())
-    finite = bool(torch.isfinite(loss).item()) and bool(torch.isfinite(total).item())
+    # one pass over the gradients for their norm (it is not finite where one of them is not: what GradScaler.unscale_ records as
+    # found_inf) and, clipping by norm, one that scales them (a norm that is not finite scales nothing); one read of the result
+    grads = [p.grad for p in with_grad]
+    by_norm = clip_grad_norm_by is not None and clip_grad_norm_or_value == "norm"
+    if not grads:
+        total = loss.new_zeros(())
+    elif by_norm:
+        total = ops.clip_grad_norm(grads, clip_grad_norm_by)
+    else:
+        total = ops.grad_norm(grads)
+    finite = bool(torch.isfinite(torch.stack([loss.float().reshape(()), total.float()])).all())
     norm = None
     if not finite:
         logging.getLogger(__name__).warning("train_step: non-finite loss or gradient (loss %s, gradient norm %s): optimizer step "
                                             "skipped", float(loss), float(total))
         return loss, norm
     if clip_grad_norm_by is not None:
-        if clip_grad_norm_or_value == "norm":
-            norm = torch.nn.utils.clip_grad_norm_(with_grad, clip_grad_norm_by)
-        else:
-            norm = total
-            torch.nn.utils.clip_grad_value_(with_grad, clip_grad_norm_by)
+        norm = total
+        if not by_norm and grads:
+            ops.clip_grad_value(grads, clip_grad_norm_by)
     optimizer.step()
     controlnet._invalidate()
     return loss, norm

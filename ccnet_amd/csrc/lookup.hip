@@ -3,17 +3,17 @@
 //   y[t] = scale * W[id[t]]                      (ids outside [0, vocab): a row of zeros)
 //   dW[v] = scale * sum over t with id[t] = v of dy[t], in rising t
 //
-// The gradient sorts (id, t) and then writes every row of dW once, in fp32, from a fixed tree over the row's run of sorted
-// positions: no float atomics, so equal inputs give equal bits.  A run may hold one position or nearly all of them (the
-// padding token of a batch of prompts), so runs are summed in three grains: single rows, whole aligned chunks of 64
-// sorted positions and whole aligned chunks of 512 that lie inside one run (run_kernel), joined by
-// table_grad_kernel.  Rows without a token are written as zeros by the same kernel.
+// The gradient sorts (id, t) and then writes the row of every id that occurs once, in fp32, from a fixed tree over the id's run
+// of sorted positions: no float atomics, so equal inputs give equal bits.  A run may hold one position or nearly all of them
+// (the padding token of a batch of prompts), so runs are summed in three grains: single rows, whole aligned chunks of 64
+// sorted positions and whole aligned chunks of 512 that lie inside one run (chunk_sum_kernel), joined by run_sum_kernel.
+// Sorting keeps only a few of the 256 CUs busy: the others write the table's zeros meanwhile (Fill), rows that occur being
+// overwritten afterwards.
 #include "common.h"
 
 namespace {
 
 typedef unsigned short bf16_t;
-typedef __attribute__((ext_vector_type(2))) int i32x2;
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf16_t v) { return bf16_bits_to_f32(v); }
@@ -102,38 +102,57 @@ __device__ __forceinline__ int key_of(const void* ids, int wide, long long t, in
     return id < 0 || id >= vocab || id == padding ? vocab : (int)id;
 }
 
-// every id's run of sorted positions [first, end): none yet
-__device__ __forceinline__ void clear_runs(i32x2* runs, int vocab) {
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < vocab; i += (long long)gridDim.x * blockDim.x) runs[i] = i32x2{0, 0};
+// Rows [row0, row1) of the table as zeros, by the workgroups of a launch behind its first `workers`.  flat: the rows are one
+// range of memory, 16-byte aligned at row0.
+struct Fill { float* grad; long long ldg; int C, row0, row1, workers, flat; };
+__device__ __forceinline__ bool fill_part(const Fill& f) {
+    if ((int)blockIdx.x < f.workers) return false;
+    const long long me = (long long)(blockIdx.x - f.workers) * blockDim.x + threadIdx.x, all = (long long)(gridDim.x - f.workers) * blockDim.x;
+    const long long n = (long long)(f.row1 - f.row0) * f.C;
+    float* p = f.grad + f.row0 * f.ldg;
+    if (f.flat) {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (long long i = me; i < n / 4; i += all) *(f32x4*)(p + 4 * i) = zero;
+        if (me < (n & 3)) p[(n & ~3ll) + me] = 0.f;
+    } else {  // a wave per row
+        const int lane = threadIdx.x & 63;
+        for (long long r = me >> 6; r < f.row1 - f.row0; r += all >> 6)
+            for (int c = lane; c < f.C; c += 64) p[r * f.ldg + c] = 0.f;
+    }
+    return true;
 }
 
 // Up to RANK_MOST positions: every position counts the ones in front of it.  key << 13 | t orders them all, in 32 bits
-// (vocab < 2^18); 64 positions a workgroup, its 16 waves each compare them with a sixteenth of all.
+// (vocab < 2^18).  A workgroup ranks 2^shift = 16 or 32 positions: 64 / 2^shift lanes of each of its 16 waves hold the same
+// position and compare it with a part of all.
 constexpr int RANK_MOST = 8192, RANK_VOCAB = 1 << 18;
-__global__ __launch_bounds__(1024) void rank_sort_kernel(const void* ids, int wide, int T, int vocab, long long padding, int* keys, int* perm, i32x2* runs) {
+__global__ __launch_bounds__(1024) void rank_sort_kernel(const void* ids, int wide, int T, int vocab, long long padding, int shift, int* keys, int* perm,
+                                                         const Fill fill) {
     __shared__ unsigned all[RANK_MOST];
-    __shared__ int part[16][64];
+    __shared__ int part[16][32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    clear_runs(runs, vocab);
-    if ((int)blockIdx.x * 64 >= T) return;
+    if (fill_part(fill)) return;
     const int T4 = (T + 3) & ~3;
+#pragma unroll 4
     for (int t = threadIdx.x; t < T4; t += 1024) all[t] = t < T ? (unsigned)key_of(ids, wide, t, vocab, padding) << 13 | t : 0xffffffffu;
     __syncthreads();
-    const int t = blockIdx.x * 64 + lane;
+    const int own = 1 << shift, slices = 64 >> shift, i = lane & (own - 1), t = blockIdx.x * own + i;
     const unsigned me = all[min(t, T - 1)];
-    const int quads = T4 / 4, per = (quads + 15) / 16;
+    const int quads = T4 / 4, per = (quads + 16 * slices - 1) / (16 * slices), from = (wave * slices + (lane >> shift)) * per;
     int before = 0;
 #pragma unroll 8
-    for (int i = wave * per; i < min(quads, (wave + 1) * per); ++i) {
-        const u32x4 v = *(const u32x4*)(all + 4 * i);
+    for (int q = from; q < min(quads, from + per); ++q) {
+        const u32x4 v = *(const u32x4*)(all + 4 * q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) before += v[e] < me;
     }
-    part[wave][lane] = before;
+    for (int o = own; o < 64; o <<= 1) before += __shfl_xor(before, o);
+    if (lane < own) part[wave][i] = before;
     __syncthreads();
-    if (wave == 0 && t < T) {
+    if (wave == 0 && lane < own && t < T) {
         int r = 0;
-        for (int w = 0; w < 16; ++w) r += part[w][lane];
+#pragma unroll
+        for (int w = 0; w < 16; ++w) r += part[w][i];
         keys[r] = (int)(me >> 13);
         perm[r] = t;
     }
@@ -146,15 +165,15 @@ struct SortArgs {
     const int* keys_in; const int* perm_in;  // NULL on the first pass: the ids themselves, in order
     int* keys_out; int* perm_out;
     int* hist; int shift;
-    i32x2* runs;  // cleared on the first pass
+    Fill fill;
 };
 __device__ __forceinline__ int sort_key(const SortArgs& a, long long t) {
     return a.keys_in ? a.keys_in[t] : key_of(a.ids, a.wide, t, a.vocab, a.padding);
 }
 __global__ __launch_bounds__(RS_THREADS) void sort_hist_kernel(const SortArgs a) {
     __shared__ int h[256];
+    if (fill_part(a.fill)) return;
     if (threadIdx.x < 256) h[threadIdx.x] = 0;
-    if (a.shift == 0) clear_runs(a.runs, a.vocab);
     __syncthreads();
     const long long t0 = (long long)blockIdx.x * RS_BLOCK;
     for (int i = threadIdx.x; i < RS_BLOCK && t0 + i < a.T; i += RS_THREADS) atomicAdd(&h[(sort_key(a, t0 + i) >> a.shift) & 255], 1);
@@ -166,11 +185,12 @@ __global__ __launch_bounds__(RS_THREADS) void sort_scatter_kernel(const SortArgs
     __shared__ int count[WAVES][256];
     __shared__ int base[2][256], total[2][256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (fill_part(a.fill)) return;
     for (int i = tid; i < WAVES * 256; i += RS_THREADS) (&count[0][0])[i] = 0;
     // digit totals of all blocks, and of the blocks in front of this one
     {  // (half of the blocks each half of the threads)
         int before = 0, all = 0;
-        const int nb = gridDim.x, mine = blockIdx.x, half = tid >> 8, digit = tid & 255;
+        const int nb = a.fill.workers, mine = blockIdx.x, half = tid >> 8, digit = tid & 255;
 #pragma unroll 8
         for (int b = half; b < nb; b += 2) {
             const int v = a.hist[b * 256 + digit];
@@ -241,9 +261,9 @@ __global__ __launch_bounds__(RS_THREADS) void sort_scatter_kernel(const SortArgs
 struct GradArgs {
     const int* keys; const int* perm; int T, vocab;
     const void* dy; long long lddy; int C; float scale;
-    i32x2* runs;              // [vocab]
     float* p64; float* p512;  // [T / 64][C], [T / 512][C]
-    float* grad; long long ldg; int accumulate, rows_per_wave;
+    float* grad; long long ldg; int accumulate, per_wave;
+    Fill fill;
 };
 
 // Eight columns as they lie in memory, so that many rows in flight cost no more registers than their bytes.
@@ -316,23 +336,16 @@ __device__ __forceinline__ void add_chunks(const float* p, int C, int first, int
     }
 }
 
-// grid (T / 512 rounded up, C / 512 rounded up), 8 waves: wave w marks where runs begin and end in chunk 8 b + w, and sums the
-// chunk if it lies inside one run
+// 8 waves, workgroup (b, column span): wave w sums chunk 8 b + w if it lies inside one run, together they sum chunk b of 512
 template <typename T, bool VEC>
-__global__ __launch_bounds__(512) void run_kernel(const GradArgs a) {
+__global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     __shared__ float red[8][512];
     __shared__ int key0[8];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.y * 512;
-    const int s = blockIdx.x * 512 + wave * 64, i = s + lane;
-    const int key = i < a.T ? a.keys[i] : -1, prev = i > 0 && i < a.T ? a.keys[i - 1] : -1;
-    const int pos = i < a.T ? a.perm[i] : 0;
-    if (blockIdx.y == 0 && i < a.T) {
-        if (key != prev) {
-            if (key < a.vocab) ((int*)a.runs)[2ll * key] = i;
-            if (prev >= 0) ((int*)a.runs)[2ll * prev + 1] = i;  // (the positions that take no part sort last: prev < vocab)
-        }
-        if (i == a.T - 1 && key < a.vocab) ((int*)a.runs)[2ll * key + 1] = a.T;
-    }
+    if (fill_part(a.fill)) return;
+    const int spans = (a.C + 511) / 512, b = blockIdx.x / spans, c0 = (blockIdx.x - b * spans) * 512;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int s = b * 512 + wave * 64, i = s + lane;
+    const int key = i < a.T ? a.keys[i] : -1, pos = i < a.T ? a.perm[i] : 0;
     const int first = __builtin_amdgcn_readfirstlane(key);
     const bool whole = first >= 0 && first < a.vocab && __all(key == first);
     float acc[8] = {};
@@ -355,25 +368,19 @@ __global__ __launch_bounds__(512) void run_kernel(const GradArgs a) {
             for (int w = 0; w < 8; ++w) v += red[w][j * 64 + lane];
             acc[j] = v;
         }
-        store8<VEC>(a.p512 + (long long)blockIdx.x * a.C + c0, lane, a.C - c0, acc);
+        store8<VEC>(a.p512 + (long long)b * a.C + c0, lane, a.C - c0, acc);
     }
 }
 
-// grid (G, C / 512 rounded up), 4 waves of R = rows_per_wave <= TG_ROWS rows.  A wave writes R neighbouring rows whose runs are
-// short: their sorted positions are neighbours too, so it streams them eight at a time across the rows' borders.  Long runs are
-// summed by the four waves together; those of the workgroup are rows blockIdx.x + i G, as frequent ids are neighbours in a
-// vocabulary.
-constexpr int TG_ROWS = 4, TG_SHORT = 32;
+// grid (T / 4 per_wave rounded up, C / 512 rounded up), 4 waves: a wave takes the runs that begin in its per_wave <= 32 sorted
+// positions.  Runs of up to 32 positions it streams one after the other, eight positions at a time, across their borders.  A longer one (at most
+// one begins there, the last) is summed by the four waves together, from the chunk sums where they cover it.
+constexpr int RUN_SHORT = 32;
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void table_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
     __shared__ float red[4][512];
+    __shared__ int long_at[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 512, cols = a.C - c0;
-    const int R = a.rows_per_wave;
-    const long long v0 = (long long)blockIdx.x * 4 * R + wave * R;
-    i32x2 mine = {0, 0}, strided = {0, 0};
-    if (a.T > 0 && lane < R && v0 + lane < a.vocab) mine = a.runs[v0 + lane];
-    const long long vs = blockIdx.x + (long long)lane * gridDim.x;
-    if (a.T > 0 && lane < 4 * R && vs < a.vocab) strided = a.runs[vs];
     auto put = [&](long long v, float* acc) {
         float* row = a.grad + v * a.ldg + c0;
         if (a.accumulate) {
@@ -387,70 +394,69 @@ __global__ __launch_bounds__(256) void table_grad_kernel(const GradArgs a) {
         }
         store8<VEC>(row, lane, cols, acc);
     };
-    const int n = mine[1] - mine[0];
-    if (!a.accumulate) {
-        for (int r = 0; r < R; ++r)
-            if (v0 + r < a.vocab && __builtin_amdgcn_readlane(n, r) == 0) {
-                const float zero[8] = {};
-                store8<VEC>(a.grad + (v0 + r) * a.ldg + c0, lane, cols, zero);
-            }
+    // this wave's positions and the 32 behind them: where runs begin (a position behind the last counts as a beginning)
+    const int p0 = (blockIdx.x * 4 + wave) * a.per_wave, p = p0 + lane;
+    const int key = p < a.T ? a.keys[p] : a.vocab, pos = p < a.T ? a.perm[p] : 0;
+    const int front = p0 > 0 && p0 < a.T ? a.keys[p0 - 1] : -1, up = __shfl_up(key, 1);
+    const bool begins = p >= a.T || key != (lane == 0 ? front : up);
+    const unsigned long long marks = __ballot(begins), live = __ballot(key < a.vocab);  // (live positions come first)
+    const unsigned mine = (unsigned)marks & (unsigned)live & (0xffffffffu >> (32 - a.per_wave));
+    int begin = 0, end = 0, long_s = -1;
+    if (mine) {
+        begin = __ffs(mine) - 1;
+        const int last = 31 - __clz(mine);  // the last run that begins here
+        const unsigned long long behind = marks >> last >> 1;
+        const int len = behind ? __ffsll(behind) : 64;
+        if (len > RUN_SHORT) long_s = p0 + last;
+        end = len > RUN_SHORT ? last : last + len;
     }
-    // short runs: from row to row while their positions follow each other
     const T* dy = (const T*)a.dy + c0;
-    for (int r = 0; r < R;) {
-        const int begin = __builtin_amdgcn_readlane(mine[0], r);
-        int end = begin, r1 = r;
-        for (; r1 < R; ++r1) {
-            const int k = __builtin_amdgcn_readlane(n, r1);
-            if (k > TG_SHORT) break;
-            if (k == 0) {
-                if (end == begin) break;  // (nothing yet: the next row starts anew)
-                continue;
-            }
-            end = __builtin_amdgcn_readlane(mine[1], r1);
-        }
+    {
         float acc[8] = {};
-        long long row = -1;
-        for (int p0 = begin; p0 < end; p0 += 64) {
-            const int left = min(end - p0, 64);
-            const int key = lane < left ? a.keys[p0 + lane] : 0, pos = lane < left ? a.perm[p0 + lane] : 0;
-            for (int j = 0; j < left; j += 8) {
-                Raw<T, VEC> x[8];
+        int row = -1;
+        for (int j = begin; j < end; j += 8) {
+            Raw<T, VEC> x[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    x[u].load(dy + (long long)__builtin_amdgcn_readlane(pos, min(j + u, left - 1)) * a.lddy, lane, j + u < left ? cols : 0);
+            for (int u = 0; u < 8; ++u)
+                x[u].load(dy + (long long)__builtin_amdgcn_readlane(pos, min(j + u, end - 1)) * a.lddy, lane, j + u < end ? cols : 0);
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (j + u < left) {
-                        const int k = __builtin_amdgcn_readlane(key, j + u);
-                        if (k != row) {
-                            if (row >= 0) put(row, acc);
-                            row = k;
+            for (int u = 0; u < 8; ++u)
+                if (j + u < end) {
+                    const int k = __builtin_amdgcn_readlane(key, j + u);
+                    if (k != row) {
+                        if (row >= 0) put(row, acc);
+                        row = k;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-                        }
-                        x[u].add(acc);
+                        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
                     }
-            }
+                    x[u].add(acc);
+                }
         }
         if (row >= 0) put(row, acc);
-        r = r1 > r ? r1 : r + 1;
     }
-    // long runs
-    unsigned long long todo = __ballot(strided[1] - strided[0] > TG_SHORT);
-    while (todo) {
-        const int i = __ffsll((unsigned long long)todo) - 1;
-        todo &= todo - 1;
-        const int s = __builtin_amdgcn_readlane(strided[0], i), e = __builtin_amdgcn_readlane(strided[1], i);
-        const long long v = blockIdx.x + (long long)i * gridDim.x;
+    if (lane == 0) long_at[wave] = long_s;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+        const int s = __builtin_amdgcn_readfirstlane(long_at[w]);
+        if (s < 0) continue;
+        const int v = a.keys[s];
+        int lo = s + RUN_SHORT, e = a.T;  // keys[lo] is the run's, position e is not: 64 probes a round
+        while (e - lo > 1) {
+            const int n = e - lo, at = lo + (int)((long long)n * (lane + 1) / 65);
+            const int in = __popcll(__ballot(a.keys[at] == v));
+            const int l2 = in == 0 ? lo : lo + (int)((long long)n * in / 65), e2 = in == 64 ? e : lo + (int)((long long)n * (in + 1) / 65);
+            if (l2 == lo && e2 == e) break;  // (not reached: a round cuts n to at most n / 65 + 1)
+            lo = l2;
+            e = e2;
+        }
         // rows [s, 64 ca), chunks [ca, 8 da) of 64, chunks [da, db) of 512, chunks [8 db, cb) of 64, rows [64 cb, e)
         float acc[8] = {};
         const int ca = (s + 63) / 64, cb = e / 64, da = (ca + 7) / 8, db = cb / 8;
-        auto rows = [&](int from, int to) {  // at most 192: every fourth of them a wave's
+        auto rows = [&](int from, int to) {  // at most 126: every fourth of them a wave's
             const int cnt = (to - from - wave + 3) / 4;
             if (cnt <= 0) return;
-            const int pos = lane < cnt ? a.perm[from + wave + 4 * lane] : 0;
-            add_rows<T, VEC>(a, pos, cnt, c0, lane, acc);
+            const int at = lane < cnt ? a.perm[from + wave + 4 * lane] : 0;
+            add_rows<T, VEC>(a, at, cnt, c0, lane, acc);
         };
         if (ca >= cb) {
             rows(s, e);
@@ -486,16 +492,13 @@ void launch_lookup(bool vec, const void* ids, int wide, int T, int vocab, const 
 }
 
 template <typename T, bool VEC>
-int launch_grad(GradArgs a, hipStream_t st) {
-    const unsigned ct = (unsigned)((a.C + 511) / 512);
-    if (a.T > 0) {
-        hipLaunchKernelGGL((run_kernel<T, VEC>), dim3((unsigned)(((long long)a.T + 511) / 512), ct), dim3(512), 0, st, a);
-        CCNET_LAUNCH_CHECK();
-    }
-    // four rows a wave where that still fills the chip (256 CUs x 8 workgroups of four waves), one in smaller tables
-    a.rows_per_wave = a.vocab >= 16 * 1024 ? TG_ROWS : 1;
-    const long long per = 4ll * a.rows_per_wave;
-    hipLaunchKernelGGL((table_grad_kernel<T, VEC>), dim3((unsigned)((a.vocab + per - 1) / per), ct), dim3(256), 0, st, a);
+int launch_grad(GradArgs a, unsigned fillers, hipStream_t st) {
+    // few positions a wave while the grid is small (2464 positions: 41 us against 46 with 16), more where waves abound (131071: 145 / 147)
+    a.per_wave = a.T <= 65536 ? 8 : 16;
+    const unsigned spans = (unsigned)((a.C + 511) / 512);
+    hipLaunchKernelGGL((chunk_sum_kernel<T, VEC>), dim3((unsigned)a.fill.workers + fillers), dim3(512), 0, st, a);
+    CCNET_LAUNCH_CHECK();
+    hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)((a.T + 4 * a.per_wave - 1) / (4 * a.per_wave)), spans), dim3(256), 0, st, a);
     CCNET_LAUNCH_CHECK();
     return CCNET_OK;
 }
@@ -503,14 +506,13 @@ int launch_grad(GradArgs a, hipStream_t st) {
 bool aligned16(const void* p, long long ld, int esz) { return !((uintptr_t)p & 15) && (ld * esz) % 16 == 0; }
 
 // workspace: sorted keys and positions (twice: a pass reads one copy and writes the other), digit counts, chunk sums
-struct Layout { size_t keys[2], perm[2], hist, runs, p64, p512, bytes; };
-Layout layout_of(int T, int vocab, int C) {
+struct Layout { size_t keys[2], perm[2], hist, p64, p512, bytes; };
+Layout layout_of(int T, int C) {
     Layout l{};
     size_t at = 0;
     auto take = [&](size_t n) { const size_t r = at; at += (n + 255) & ~(size_t)255; return r; };
     for (int i = 0; i < 2; ++i) { l.keys[i] = take((size_t)T * 4); l.perm[i] = take((size_t)T * 4); }
     l.hist = take(((size_t)T + RS_BLOCK - 1) / RS_BLOCK * 1024);
-    l.runs = take((size_t)vocab * 8);
     l.p64 = take((size_t)(T / 64) * C * 4);
     l.p512 = take((size_t)(T / 512) * C * 4);
     l.bytes = at;
@@ -538,9 +540,9 @@ extern "C" int ccnet_embedding(const void* ids, int id_bytes, int T, int vocab, 
     return CCNET_OK;
 }
 
-extern "C" size_t ccnet_embedding_grad_workspace_bytes(int T, int vocab, int C) {
-    if (T <= 0 || vocab <= 0 || C <= 0) return 0;
-    return layout_of(T, vocab, C).bytes;
+extern "C" size_t ccnet_embedding_grad_workspace_bytes(int T, int C) {
+    if (T <= 0 || C <= 0) return 0;
+    return layout_of(T, C).bytes;
 }
 
 extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const void* dy, int dy_dtype, int lddy, int C,
@@ -552,46 +554,68 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     const int ds = dy_dtype == 0 ? 4 : 2;
     if (!grad || ((uintptr_t)grad & 3) || (C + 511) / 512 > 65535) return CCNET_EINVAL;
     if (T > 0 && (!ids || !dy || (uintptr_t)ids % id_bytes || (uintptr_t)dy % ds)) return CCNET_EINVAL;
-    const Layout l = layout_of(T, vocab, C);
+    const Layout l = layout_of(T, C);
     if (T > 0 && (!workspace || ((uintptr_t)workspace & 15))) return CCNET_EINVAL;
     if (T > 0 && workspace_bytes < l.bytes) return CCNET_EWS;
     if (T == 0 && accumulate) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
+    // the table's zeros in parts [0, vocab): part k of n with a launch that has `workers` workgroups of its own
+    const bool flat = ldg == C && !((uintptr_t)grad & 15);
+    int filled = 0;
+    unsigned fillers = 0;
+    auto fill_next = [&](int workers, int k, int n) {
+        Fill f{grad, ldg, C, filled, accumulate ? filled : k == n ? vocab : (int)((long long)vocab * k / n / 4 * 4), workers, flat};
+        filled = f.row1;
+        const long long bytes = (long long)(f.row1 - f.row0) * C * 4;  // 64 KiB a workgroup, at most 4 a CU
+        fillers = bytes <= 0 ? 0u : (unsigned)(bytes < 64ll * 1024 * 1024 ? (bytes + 65535) / 65536 : 1024);
+        return f;
+    };
+    if (T == 0) {
+        SortArgs s{};
+        s.fill = fill_next(0, 1, 1);
+        hipLaunchKernelGGL(sort_hist_kernel, dim3(fillers), dim3(RS_THREADS), 0, st, s);
+        CCNET_LAUNCH_CHECK();
+        return CCNET_OK;
+    }
     char* ws = (char*)workspace;
     GradArgs g{};
     g.T = T; g.vocab = vocab; g.dy = dy; g.lddy = lddy; g.C = C; g.scale = scale; g.grad = grad; g.ldg = ldg; g.accumulate = accumulate != 0;
-    if (T > 0) {
-        int* keys[2] = {(int*)(ws + l.keys[0]), (int*)(ws + l.keys[1])};
-        int* perm[2] = {(int*)(ws + l.perm[0]), (int*)(ws + l.perm[1])};
-        g.runs = (i32x2*)(ws + l.runs);
-        g.p64 = (float*)(ws + l.p64);
-        g.p512 = (float*)(ws + l.p512);
-        int cur = 0;
-        if (T <= RANK_MOST && vocab < RANK_VOCAB) {
-            const int sorting = (T + 63) / 64, clearing = (vocab + 8191) / 8192;
-            hipLaunchKernelGGL(rank_sort_kernel, dim3(sorting > clearing ? sorting : clearing), dim3(1024), 0, st, ids, (int)(id_bytes == 8), T, vocab,
-                               (long long)padding_idx, keys[0], perm[0], g.runs);
+    g.p64 = (float*)(ws + l.p64);
+    g.p512 = (float*)(ws + l.p512);
+    int* keys[2] = {(int*)(ws + l.keys[0]), (int*)(ws + l.keys[1])};
+    int* perm[2] = {(int*)(ws + l.perm[0]), (int*)(ws + l.perm[1])};
+    int cur = 0, passes = 0;
+    const int chunk_workers = (int)((T + 511) / 512) * ((C + 511) / 512);
+    if (T <= RANK_MOST && vocab < RANK_VOCAB) {
+        const int shift = T <= 4096 ? 4 : 5;  // (at most 256 workgroups: one a CU)
+        const Fill f = fill_next((T + (1 << shift) - 1) >> shift, 1, 2);
+        hipLaunchKernelGGL(rank_sort_kernel, dim3(f.workers + fillers), dim3(1024), 0, st, ids, (int)(id_bytes == 8), T, vocab, (long long)padding_idx, shift,
+                           keys[0], perm[0], f);
+        CCNET_LAUNCH_CHECK();
+        passes = 1;
+    } else {
+        SortArgs s{};
+        s.ids = ids; s.wide = id_bytes == 8; s.T = T; s.vocab = vocab; s.padding = padding_idx; s.hist = (int*)(ws + l.hist);
+        const int blocks = (T + RS_BLOCK - 1) / RS_BLOCK;
+        for (int shift = 0; shift < 32 && (vocab >> shift) > 0; shift += 8) passes += 2;
+        cur = 1;
+        for (int k = 0; k < passes; k += 2) {
+            s.shift = 4 * k;
+            s.keys_out = keys[1 - cur]; s.perm_out = perm[1 - cur];
+            s.fill = fill_next(blocks, k + 1, passes + 1);
+            hipLaunchKernelGGL(sort_hist_kernel, dim3(blocks + fillers), dim3(RS_THREADS), 0, st, s);
             CCNET_LAUNCH_CHECK();
-        } else {
-            SortArgs s{};
-            s.ids = ids; s.wide = id_bytes == 8; s.T = T; s.vocab = vocab; s.padding = padding_idx; s.hist = (int*)(ws + l.hist); s.runs = g.runs;
-            const unsigned blocks = (unsigned)(((long long)T + RS_BLOCK - 1) / RS_BLOCK);
-            cur = 1;
-            for (int shift = 0; shift < 32 && (vocab >> shift) > 0; shift += 8) {
-                s.shift = shift;
-                s.keys_out = keys[1 - cur]; s.perm_out = perm[1 - cur];
-                hipLaunchKernelGGL(sort_hist_kernel, dim3(blocks), dim3(RS_THREADS), 0, st, s);
-                CCNET_LAUNCH_CHECK();
-                hipLaunchKernelGGL(sort_scatter_kernel, dim3(blocks), dim3(RS_THREADS), 0, st, s);
-                CCNET_LAUNCH_CHECK();
-                cur = 1 - cur;
-                s.keys_in = keys[cur]; s.perm_in = perm[cur];
-            }
+            s.fill = fill_next(blocks, k + 2, passes + 1);
+            hipLaunchKernelGGL(sort_scatter_kernel, dim3(blocks + fillers), dim3(RS_THREADS), 0, st, s);
+            CCNET_LAUNCH_CHECK();
+            cur = 1 - cur;
+            s.keys_in = keys[cur]; s.perm_in = perm[cur];
         }
-        g.keys = keys[cur];
-        g.perm = perm[cur];
     }
+    g.keys = keys[cur];
+    g.perm = perm[cur];
+    g.fill = fill_next(chunk_workers, passes + 1, passes + 1);
     const bool vec = C % 8 == 0 && aligned16(dy, lddy, ds) && aligned16(grad, ldg, 4);
-    if (dy_dtype == 0) return vec ? launch_grad<float, true>(g, st) : launch_grad<float, false>(g, st);
-    return vec ? launch_grad<bf16_t, true>(g, st) : launch_grad<bf16_t, false>(g, st);
+    if (dy_dtype == 0) return vec ? launch_grad<float, true>(g, fillers, st) : launch_grad<float, false>(g, fillers, st);
+    return vec ? launch_grad<bf16_t, true>(g, fillers, st) : launch_grad<bf16_t, false>(g, fillers, st);
 }

@@ -134,7 +134,7 @@ def load() -> C.CDLL:
     lib.ccnet_xattn_kv_image_bytes.argtypes = [i, i]
     lib.ccnet_xattn_kv_image_bytes.restype = C.c_int64
     lib.ccnet_embedding.argtypes = [vp, i, i, i, vp, i, i, i, f, vp, i, i, vp]
-    lib.ccnet_embedding_grad_workspace_bytes.argtypes = [i, i, i]
+    lib.ccnet_embedding_grad_workspace_bytes.argtypes = [i, i]
     lib.ccnet_embedding_grad_workspace_bytes.restype = sz
     lib.ccnet_embedding_grad.argtypes = [vp, i, i, i, vp, i, i, i, f, i64, vp, i, i, vp, sz, vp]
     lib.ccnet_attention_packed_bf16.argtypes = [vp, i, vp, i, vp, i, vp, i, vp, i, i, i, i, i, f, i, vp, vp, vp]

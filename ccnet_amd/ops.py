@@ -674,7 +674,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float
     if out is None:
         out = torch.empty((vocab, Cc), dtype=torch.float32, device=dy.device)
     ldg = _rows_ld(out, "out", vocab, Cc, (torch.float32,))
-    wsb = lib.ccnet_embedding_grad_workspace_bytes(T, vocab, Cc)
+    wsb = lib.ccnet_embedding_grad_workspace_bytes(T, Cc)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device)
     _l.check(lib.ccnet_embedding_grad(flat.data_ptr(), flat.element_size(), T, vocab, dy.data_ptr(), _F32_BF16[dy.dtype], lddy, Cc,
                                       scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ldg, int(accumulate),

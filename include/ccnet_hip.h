@@ -394,8 +394,8 @@ int ccnet_embedding(const void* ids, int id_bytes, int T, int vocab, const void*
 /* grad[v] (fp32) = scale * sum of dy[t] over the positions with ids[t] = v; every row is written, rows without a position as
  * zeros.  accumulate != 0: added to what is there, rows without a position are not touched.  Positions whose id is outside
  * [0, vocab) or equal to padding_idx (-1: none) take no part.  T <= 2^30; workspace (16-byte aligned):
- * ccnet_embedding_grad_workspace_bytes(T, vocab, C) bytes. */
-size_t ccnet_embedding_grad_workspace_bytes(int T, int vocab, int C);
+ * ccnet_embedding_grad_workspace_bytes(T, C) bytes. */
+size_t ccnet_embedding_grad_workspace_bytes(int T, int C);
 int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const void* dy, int dy_dtype, int lddy, int C, float scale,
                          int64_t padding_idx, float* grad, int ldg, int accumulate, void* workspace, size_t workspace_bytes,
                          void* stream);

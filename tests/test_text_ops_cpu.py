@@ -88,8 +88,8 @@ def test_c_abi_refusals():
     a[2] = 0
     assert E(*a) == 0  # no rows: nothing to do
     G = l.ccnet_embedding_grad
-    need = l.ccnet_embedding_grad_workspace_bytes(1000, 10, 64)
-    assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 10, 64) == 0
+    need = l.ccnet_embedding_grad_workspace_bytes(1000, 64)
+    assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 64) == 0
     ok = [p, 8, 1000, 10, p, 1, 64, 64, 1.0, -1, p, 64, 0, p, need, None]
     for i, v, rc in ((1, 3, EINVAL), (2, -1, EINVAL), (3, 0, EINVAL), (3, 0x7fffffff, EINVAL), (4, None, EINVAL), (5, 2, EINVAL), (6, 8, EINVAL),
                      (7, 0, EINVAL), (10, None, EINVAL), (10, C.c_void_p(1026), EINVAL), (11, 63, EINVAL), (13, None, EINVAL),

@@ -129,7 +129,7 @@ def test_c_abi_refusals():
         assert B(*a) == rc, (i, v)
     ptrs, n = (C.c_void_p * 2)(1 << 20, 1 << 24), (C.c_int64 * 2)(1000, 70000)
     need = l.ccnet_grad_norm_workspace_bytes(ptrs, n, 2, 0)
-    assert need == 8 * (1 + 1 + 3)
+    assert need == 8 * (1 + 1 + 5)
     for args, rc in (((ptrs, n, 2, 2, p, need, p, None), EINVAL), ((ptrs, n, -1, 0, p, need, p, None), EINVAL), ((None, n, 2, 0, p, need, p, None), EINVAL),
                      ((ptrs, n, 2, 0, None, need, p, None), EINVAL), ((ptrs, n, 2, 0, p, need - 1, p, None), EWS), ((ptrs, n, 2, 0, p, need, None, None), EINVAL)):
         assert l.ccnet_grad_norm(*args) == rc

@@ -714,7 +714,17 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, tlo[d], thi[d]);
         f32x16 s, dp;
-        auto scores = [&](f32x16& sr, f32x16& dr, const char* qb, const float* stat) {
+        // fragments of the next block's rows (fq, fd) and of this block's transposed reads (tq, td) are read a phase ahead of the
+        // products that take them
+        bf16x8 fq[NK], fd[NK], tq[2][ND], td[2][ND];
+        auto rows = [&](const char* qb) {
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                fq[ks] = *(const bf16x8*)(qb + rread[ks]);
+                fd[ks] = *(const bf16x8*)(qb + TILEB + rread[ks]);
+            }
+        };
+        auto scores = [&](f32x16& sr, f32x16& dr, const float* stat) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 d4 = *(const f32x4*)(stat + 64 + 8 * g + 4 * hh);
@@ -723,20 +733,20 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
             }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], sr, 0, 0, 0);
-                dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + TILEB + rread[ks]), vf[ks], dr, 0, 0, 0);
+                sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[ks], kf[ks], sr, 0, 0, 0);
+                dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fd[ks], vf[ks], dr, 0, 0, 0);
             }
         };
-        // qb: Q of this query block (dO a tile behind it), stat: its lse and delta, rel: its index counted from the wave's diagonal,
-        // qn: Q of the next block
-        auto step = [&](const char* qb, const float* stat, int rel, const char* qn, const float* statn) {
+        // qb: Q of this query block (dO a tile behind it), stat: its lse, rel: its index counted from the wave's diagonal, statn: of
+        // the next block, qnn: Q of the block after that
+        auto step = [&](const char* qb, const float* stat, int rel, const float* statn, const char* qnn, auto fence_c) {
             if (rel <= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (rel * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
             }
             f32x16 sn, dpn;
-            scores(sn, dpn, qn, statn);
+            scores(sn, dpn, statn);
             bf16x8 pfr[2], dsf[2];
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI) {
@@ -760,8 +770,23 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
                     const char* x = qb + sI * 16 * ROWB;
-                    dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + TILEB + tlo[d], x + TILEB + thi[d]), pfr[sI], dv[d], 0, 0, 0);
-                    dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + tlo[d], x + thi[d]), dsf[sI], dk[d], 0, 0, 0);
+                    td[sI][d] = tr_pair(x + TILEB + tlo[d], x + TILEB + thi[d]);
+                    tq[sI][d] = tr_pair(x + tlo[d], x + thi[d]);
+                }
+            if constexpr (decltype(fence_c)::value) {
+                stage_fence();  // the next tile has landed; the tile after it may overwrite the one before this
+                issue();
+            } else {
+                asm volatile("" ::: "memory");
+            }
+            rows(qnn);
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int sI = 0; sI < 2; ++sI)
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(td[sI][d], pfr[sI], dv[d], 0, 0, 0);
+                    dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[sI][d], dsf[sI], dk[d], 0, 0, 0);
                 }
             s = sn;
             dp = dpn;
@@ -771,17 +796,18 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
         settle(vf);
         stage_fence();
         issue();  // (the first fence of the walk waits for it)
-        scores(s, dp, smem, (const float*)(smem + 2 * TILEB));
+        rows(smem);
+        scores(s, dp, (const float*)(smem + 2 * TILEB));
+        rows(smem + BLOCKB);
         int slot = 0, rel = -wave;
         for (int i = 0, it2 = 0; i < steps; ++i) {
             const char* qb = smem + slot * STAGEB;
             const float* stat = (const float*)(qb + 2 * TILEB);
             slot = slot == 2 ? 0 : slot + 1;
-            step(qb, stat, rel, qb + BLOCKB, stat + 32);
-            stage_fence();  // tile i + 1 has landed; tile i + 2 may overwrite tile i - 1
-            issue();
             // (behind the last tile: the slot that was read two tiles ago, or nothing yet; its scores are not used)
-            step(qb + BLOCKB, stat + 32, rel + 1, smem + slot * STAGEB, (const float*)(smem + slot * STAGEB + 2 * TILEB));
+            const char* qn = smem + slot * STAGEB;
+            step(qb, stat, rel, stat + 32, qn, std::true_type{});
+            step(qb + BLOCKB, stat + 32, rel + 1, (const float*)(qn + 2 * TILEB), qn + BLOCKB, std::false_type{});
             rel += 2;
             if (++it2 == per_head) { it2 = 0; rel = -wave; }
         }

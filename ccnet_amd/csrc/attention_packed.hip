@@ -23,7 +23,6 @@
 
 namespace {
 
-constexpr int PA_THREADS = 256;
 constexpr int PA_TILE = 64;  // rows of a staged tile
 
 struct PackedArgs {
@@ -221,9 +220,9 @@ __device__ __forceinline__ void tr_lane(int lane, int d, int& lo, int& hi) {
 }
 
 // the DMA pieces of a 64-row tile that a wave brings: piece p holds 1024 / (2 D) rows, lane l of it chunk position l mod (D / 8)
-template <int D>
+template <int D, int W>
 struct TileDma {
-    static constexpr int ROWB = 2 * D, CH = D / 8, BYTES = PA_TILE * ROWB, PIECES = BYTES / 1024 / 4;
+    static constexpr int ROWB = 2 * D, CH = D / 8, BYTES = PA_TILE * ROWB, PIECES = BYTES / 1024 / W;
     unsigned voff[PIECES];
     int wave;
     __device__ __forceinline__ void init(int wave_, int lane, long long ldb) {
@@ -309,9 +308,9 @@ __device__ __forceinline__ float half_sum(float v) {
 // pipe, which need about 512 cycles a step each at d = 128, run at once.  Half way through a tile's two steps lies the fence at
 // which the next tile has landed (its keys are needed by the second step) and the tile after it is sent for: K in a ring of
 // two, V, which is needed a step longer, in a ring of three.
-template <int D, int QB>
-__global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedArgs a) {
-    constexpr int BM = 128 * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+template <int D, int QB, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs a) {
+    constexpr int BM = 32 * W * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
     __shared__ __attribute__((aligned(1024))) char smem[5 * TILEB];  // K 0, K 1, V 0, V 1, V 2
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
@@ -341,7 +340,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
         const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
         const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
         const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
-        TileDma<D> kd, vd;
+        TileDma<D, W> kd, vd;
         kd.init(wave, lane, ldkb);
         vd.init(wave, lane, ldvb);
         const unsigned lds0 = lds_addr(smem);
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
         for (int X = 0; X < QB; ++X) settle(qf[X]);
         if (ntiles > 1) {
             issue(1, 1);
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D, W>::PIECES) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         }
@@ -524,9 +523,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_fwd_kernel(const PackedA
 // The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
 // and left for the dK / dV kernel.
-template <int D>
-__global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
-    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
+    constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
     __shared__ __attribute__((aligned(1024))) char smem[5 * TILEB];  // V 0, V 1, K 0, K 1, K 2
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
@@ -548,7 +547,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         const long long ldkb = a.ldk * 2, ldvb = a.ldv * 2;
         const char* kbase = (const char*)(a.K + (long long)tl.start * a.ldk + kvh * D);
         const char* vbase = (const char*)(a.V + (long long)tl.start * a.ldv + kvh * D);
-        TileDma<D> kd, vd;
+        TileDma<D, W> kd, vd;
         kd.init(wave, lane, ldkb);
         vd.init(wave, lane, ldvb);
         const unsigned lds0 = lds_addr(smem);
@@ -620,7 +619,7 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
         asm volatile("" : "+v"(lse), "+v"(dlt));
         if (ntiles > 1) {
             issue(1, 1);
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D>::PIECES) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * TileDma<D, W>::PIECES) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         }
@@ -663,9 +662,9 @@ __global__ __launch_bounds__(PA_THREADS, 2) void packed_bwd_dq_kernel(const Pack
 // group (or of its part of it) in turn, so the group's sum is taken in the accumulators, in a fixed order.  As above the scores
 // of the next query block are computed beside the exponentials of this one; Q and dO are both needed a step longer (rings of
 // three).  Query blocks in front of a wave's own keys (in the first two tiles of a head) are masked whole.
-template <int D>
-__global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
-    constexpr int BM = 128, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, STAGEB = 2 * TILEB + 512;
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
+    constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, STAGEB = 2 * TILEB + 512;
     __shared__ __attribute__((aligned(1024))) char smem[3 * STAGEB];  // per stage: Q, dO, lse and delta of the 64 queries
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
@@ -687,7 +686,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 64 ? 2 : 1) void packed_bwd_dkv_ke
         load_frags<D>(kf, a.K + row * a.ldk + kvh * D, hh, kok);
         load_frags<D>(vf, a.V + row * a.ldv + kvh * D, hh, kok);
         const long long ldqb = a.ldq * 2, lddob = a.lddo * 2;
-        TileDma<D> qd, dd;
+        TileDma<D, W> qd, dd;
         qd.init(wave, lane, ldqb);
         dd.init(wave, lane, lddob);
         const unsigned lds0 = lds_addr(smem);
@@ -858,6 +857,10 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
     return ((long long)rows + (long long)(n_seq + tail) * (step - 1)) / step;
 }
 
+// Two waves instead of four to a workgroup of the forward and dQ kernels where most sequences fit 64 rows (d 64): twice as many
+// workgroups are resident and fewer waves idle (64 x 40 rows, 16 heads: forward 11.0 -> 8.4 us; from 77 rows on there is nothing in it)
+int waves_of(int rows, int n_seq, int d) { return d == 64 && rows <= 64ll * n_seq ? 2 : 4; }
+
 // Into how many parts the walk of a key tile over its group's query heads is cut.  One workgroup walks G heads x the queries
 // behind its keys; with few key heads and long sequences the longest of those walks outlasts the rest of the grid.  Parts cost
 // fp32 sums through memory (16 bytes a channel), so only walks of at least 8 tiles a head on average are cut, and only while the
@@ -893,14 +896,20 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     a.cu = cu_seqlens; a.n_seq = n_seq; a.rows = rows; a.H = H; a.Hkv = Hkv;
     a.scale = scale; a.scale_log2e = scale * 1.4426950408889634f; a.zero_tail = zero_tail != 0; a.lse = lse;
     a.o_low = (__bf16*)o_low;
-    const bool wide = d == 64 && rows >= 256ll * n_seq;  // (mean length of at least 256: whole 256-query tiles are the rule)
-    const long long grid = most_tiles(rows, n_seq, wide ? 256 : 128, a.zero_tail) * H;
+    // 64 queries a wave (a K or V fragment feeds two products) where whole 256-query tiles are the rule and there are at least four of
+    // them a CU: 64 x 1024 rows, 16 heads 231 us against 255, 4 x 8192 rows, 32 heads 1160 / 1236; with fewer the longest walks
+    // outlast the rest (2048 rows, 16 heads 47 / 31), with shorter sequences the last tiles are mostly empty (300 x 300 rows 381 / 371)
+    const bool wide = d == 64 && rows >= 512ll * n_seq && (long long)rows * H >= 256ll * 1024;
+    const int waves = waves_of(rows, n_seq, d);
+    const long long grid = most_tiles(rows, n_seq, wide ? 256 : 32 * waves, a.zero_tail) * H;
     if (grid > 0x7fffffffLL) return CCNET_EUNSUP;
     if (grid == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
-    if (d == 128) hipLaunchKernelGGL((packed_fwd_kernel<128, 1>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
-    else if (wide) hipLaunchKernelGGL((packed_fwd_kernel<64, 2>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
-    else hipLaunchKernelGGL((packed_fwd_kernel<64, 1>), dim3((unsigned)grid), dim3(PA_THREADS), 0, st, a);
+    const dim3 g((unsigned)grid), b(64 * waves);
+    if (wide) hipLaunchKernelGGL((packed_fwd_kernel<64, 2, 4>), g, dim3(256), 0, st, a);
+    else if (d == 128) hipLaunchKernelGGL((packed_fwd_kernel<128, 1, 4>), g, b, 0, st, a);
+    else if (waves == 4) hipLaunchKernelGGL((packed_fwd_kernel<64, 1, 4>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((packed_fwd_kernel<64, 1, 2>), g, b, 0, st, a);
     CCNET_LAUNCH_CHECK();
     return CCNET_OK;
 }
@@ -936,16 +945,19 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     a.delta = (float*)workspace;
     a.part = (float*)((char*)workspace + delta_bytes(rows, H));
     a.parts = parts_of(n_seq, rows, H, Hkv);
-    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail);
-    if (tiles * H > 0x7fffffffLL) return CCNET_EUNSUP;
-    if (tiles == 0) return CCNET_OK;
+    const int waves = waves_of(rows, n_seq, d);
+    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, 32 * waves, a.zero_tail);
+    if (qtiles * H > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
-    if (d == 128) hipLaunchKernelGGL(packed_bwd_dq_kernel<128>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
-    else hipLaunchKernelGGL(packed_bwd_dq_kernel<64>, dim3((unsigned)(tiles * H)), dim3(PA_THREADS), 0, st, a);
+    const dim3 gq((unsigned)(qtiles * H)), gk((unsigned)(tiles * Hkv * a.parts)), b(64 * waves);
+    if (d == 128) hipLaunchKernelGGL((packed_bwd_dq_kernel<128, 4>), gq, b, 0, st, a);
+    else if (waves == 4) hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 4>), gq, b, 0, st, a);
+    else hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 2>), gq, b, 0, st, a);
     CCNET_LAUNCH_CHECK();
-    const dim3 grid((unsigned)(tiles * Hkv * a.parts));
-    if (d == 128) hipLaunchKernelGGL(packed_bwd_dkv_kernel<128>, grid, dim3(PA_THREADS), 0, st, a);
-    else hipLaunchKernelGGL(packed_bwd_dkv_kernel<64>, grid, dim3(PA_THREADS), 0, st, a);
+    if (tiles == 0) return CCNET_OK;
+    if (d == 128) hipLaunchKernelGGL((packed_bwd_dkv_kernel<128, 4>), gk, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((packed_bwd_dkv_kernel<64, 4>), gk, dim3(256), 0, st, a);
     CCNET_LAUNCH_CHECK();
     if (a.parts > 1) {
         const long long threads = 2ll * rows * (Hkv * d / 8);

@@ -714,8 +714,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     o = q.new_empty((rows, H * d)) if out is None else out
     stats = None
     if with_lse:
-        stats = PackedStats(torch.empty((H, rows), dtype=torch.float32, device=q.device),
-                            torch.empty((rows, H * d), dtype=BF16, device=q.device))
+        stats = PackedStats(q.new_empty((H, rows), dtype=torch.float32), q.new_empty((rows, H * d)))
     _l.check(lib.ccnet_attention_packed_bf16(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(),
                                              _rows_ld(o, "out", rows, H * d, (BF16,)), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1,
                                              rows, H, Hkv, d, scale, int(out is None), stats.lse.data_ptr() if with_lse else None,
@@ -742,11 +741,10 @@ def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
             or o_low.shape != (rows, H * d) or not o_low.is_contiguous():
         raise _l.CcnetError(f"attention_packed_bwd: stats must be the forward's, fp32 [{H}, {rows}] and bf16 [{rows}, {H * d}]")
     if not given:
-        dq = torch.empty((rows, H * d), dtype=BF16, device=q.device)
-        dk, dv = (torch.empty((rows, Hkv * d), dtype=BF16, device=q.device) for _ in range(2))
+        dq, dk, dv = q.new_empty((rows, H * d)), q.new_empty((rows, Hkv * d)), q.new_empty((rows, Hkv * d))
     n_seq = cu_seqlens.numel() - 1
     wsb = lib.ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(wsb // 2)
     _l.check(lib.ccnet_attention_packed_bwd_bf16(
         q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, o.data_ptr(), _rows_ld(o, "o", rows, H * d, (BF16,)), o_low.data_ptr(),
         do.data_ptr(), _rows_ld(do, "do", rows, H * d, (BF16,)), lse.data_ptr(), dq.data_ptr(), _rows_ld(dq, "dq", rows, H * d, (BF16,)),

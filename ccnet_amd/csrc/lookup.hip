@@ -11,6 +11,8 @@
 // overwritten afterwards.
 #include "common.h"
 
+#include <algorithm>
+
 namespace {
 
 typedef unsigned short bf16_t;
@@ -112,7 +114,7 @@ __device__ __forceinline__ bool fill_part(const Fill& f) {
     float* p = f.grad + f.row0 * f.ldg;
     if (f.flat) {
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        for (long long i = me; i < n / 4; i += all) *(f32x4*)(p + 4 * i) = zero;
+        for (long long i = me; i < n / 4; i += all) __builtin_nontemporal_store(zero, (f32x4*)(p + 4 * i));  // (a table is larger than the caches: 160 -> 147 us at 131k tokens)
         if (me < (n & 3)) p[(n & ~3ll) + me] = 0.f;
     } else {  // a wave per row
         const int lane = threadIdx.x & 63;
@@ -266,26 +268,32 @@ struct GradArgs {
     Fill fill;
 };
 
-// Eight columns as they lie in memory, so that many rows in flight cost no more registers than their bytes.
-template <typename T, bool VEC> struct Raw;
-template <> struct Raw<float, true> {
+// Eight columns as they lie in memory, so that many rows in flight cost no more registers than their bytes.  PAST: past the
+// caches, for gradients that are larger than them (131k x 1024 bf16: 147 -> 132 us; 2464 x 1024, which stay in them: 50 -> 57).
+template <typename V, bool PAST>
+__device__ __forceinline__ V load16(const void* p) {
+    if constexpr (PAST) return __builtin_nontemporal_load((const V*)p);
+    else return *(const V*)p;
+}
+template <typename T, bool VEC, bool PAST> struct Raw;
+template <bool PAST> struct Raw<float, true, PAST> {
     static constexpr int DEEP = 8;
     f32x4 a, b;
     __device__ __forceinline__ void load(const float* row, int lane, int cols) {
         a = b = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (lane * 8 < cols) { a = *(const f32x4*)(row + lane * 8); b = *(const f32x4*)(row + lane * 8 + 4); }
+        if (lane * 8 < cols) { a = load16<f32x4, PAST>(row + lane * 8); b = load16<f32x4, PAST>(row + lane * 8 + 4); }
     }
     __device__ __forceinline__ void add(float* acc) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e) { acc[e] += a[e]; acc[4 + e] += b[e]; }
     }
 };
-template <> struct Raw<bf16_t, true> {
+template <bool PAST> struct Raw<bf16_t, true, PAST> {
     static constexpr int DEEP = 16;
     u32x4 a;
     __device__ __forceinline__ void load(const bf16_t* row, int lane, int cols) {
         a = u32x4{0u, 0u, 0u, 0u};
-        if (lane * 8 < cols) a = *(const u32x4*)(row + lane * 8);
+        if (lane * 8 < cols) a = load16<u32x4, PAST>(row + lane * 8);
     }
     __device__ __forceinline__ void add(float* acc) const {
         float f[8];
@@ -294,7 +302,7 @@ template <> struct Raw<bf16_t, true> {
         for (int e = 0; e < 8; ++e) acc[e] += f[e];
     }
 };
-template <typename T> struct Raw<T, false> {
+template <typename T, bool PAST> struct Raw<T, false, PAST> {
     static constexpr int DEEP = 8;
     T v[8];
     __device__ __forceinline__ void load(const T* row, int lane, int cols) {
@@ -308,9 +316,9 @@ template <typename T> struct Raw<T, false> {
 };
 
 // acc += rows pos[0 .. n) of dy, pos[j] in lane j (n <= 64): DEEP rows in flight, their addresses from registers
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool PAST>
 __device__ __forceinline__ void add_rows(const GradArgs& a, int pos, int n, int c0, int lane, float* acc) {
-    typedef Raw<T, VEC> X;
+    typedef Raw<T, VEC, PAST> X;
     const T* dy = (const T*)a.dy + c0;
     for (int j = 0; j < n; j += X::DEEP) {
         X x[X::DEEP];
@@ -337,7 +345,7 @@ __device__ __forceinline__ void add_chunks(const float* p, int C, int first, int
 }
 
 // 8 waves, workgroup (b, column span): wave w sums chunk 8 b + w if it lies inside one run, together they sum chunk b of 512
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool PAST>
 __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     __shared__ float red[8][512];
     __shared__ int key0[8];
@@ -350,7 +358,7 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     const bool whole = first >= 0 && first < a.vocab && __all(key == first);
     float acc[8] = {};
     if (whole) {
-        add_rows<T, VEC>(a, pos, 64, c0, lane, acc);
+        add_rows<T, VEC, PAST>(a, pos, 64, c0, lane, acc);
         store8<VEC>(a.p64 + (long long)(s / 64) * a.C + c0, lane, a.C - c0, acc);
     }
     if (lane == 0) key0[wave] = whole ? first : -1;
@@ -376,7 +384,7 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
 // positions.  Runs of up to 32 positions it streams one after the other, eight positions at a time, across their borders.  A longer one (at most
 // one begins there, the last) is summed by the four waves together, from the chunk sums where they cover it.
 constexpr int RUN_SHORT = 32;
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool PAST>
 __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
     __shared__ float red[4][512];
     __shared__ int long_at[4];
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
         float acc[8] = {};
         int row = -1;
         for (int j = begin; j < end; j += 8) {
-            Raw<T, VEC> x[8];
+            Raw<T, VEC, PAST> x[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 x[u].load(dy + (long long)__builtin_amdgcn_readlane(pos, min(j + u, end - 1)) * a.lddy, lane, j + u < end ? cols : 0);
@@ -456,7 +464,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
             const int cnt = (to - from - wave + 3) / 4;
             if (cnt <= 0) return;
             const int at = lane < cnt ? a.perm[from + wave + 4 * lane] : 0;
-            add_rows<T, VEC>(a, at, cnt, c0, lane, acc);
+            add_rows<T, VEC, PAST>(a, at, cnt, c0, lane, acc);
         };
         if (ca >= cb) {
             rows(s, e);
@@ -491,14 +499,14 @@ void launch_lookup(bool vec, const void* ids, int wide, int T, int vocab, const 
     else hipLaunchKernelGGL((lookup_kernel<TW, TO, false>), grid, dim3(256), 0, st, ids, wide, T, vocab, (const TW*)table, (long long)ldt, C, scale, (TO*)out, (long long)ldo);
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool PAST>
 int launch_grad(GradArgs a, unsigned fillers, hipStream_t st) {
     // few positions a wave while the grid is small (2464 positions: 41 us against 46 with 16), more where waves abound (131071: 145 / 147)
     a.per_wave = a.T <= 65536 ? 8 : 16;
     const unsigned spans = (unsigned)((a.C + 511) / 512);
-    hipLaunchKernelGGL((chunk_sum_kernel<T, VEC>), dim3((unsigned)a.fill.workers + fillers), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((chunk_sum_kernel<T, VEC, PAST>), dim3((unsigned)a.fill.workers + fillers), dim3(512), 0, st, a);
     CCNET_LAUNCH_CHECK();
-    hipLaunchKernelGGL((run_sum_kernel<T, VEC>), dim3((unsigned)((a.T + 4 * a.per_wave - 1) / (4 * a.per_wave)), spans), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((run_sum_kernel<T, VEC, PAST>), dim3((unsigned)((a.T + 4 * a.per_wave - 1) / (4 * a.per_wave)), spans), dim3(256), 0, st, a);
     CCNET_LAUNCH_CHECK();
     return CCNET_OK;
 }
@@ -566,8 +574,8 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     auto fill_next = [&](int workers, int k, int n) {
         Fill f{grad, ldg, C, filled, accumulate ? filled : k == n ? vocab : (int)((long long)vocab * k / n / 4 * 4), workers, flat};
         filled = f.row1;
-        const long long bytes = (long long)(f.row1 - f.row0) * C * 4;  // 64 KiB a workgroup, at most 4 a CU
-        fillers = bytes <= 0 ? 0u : (unsigned)(bytes < 64ll * 1024 * 1024 ? (bytes + 65535) / 65536 : 1024);
+        const long long bytes = (long long)(f.row1 - f.row0) * C * 4;  // 32 KiB a workgroup, at most 8 a CU
+        fillers = bytes <= 0 ? 0u : (unsigned)std::min<long long>((bytes + 32767) / 32768, 2048);
         return f;
     };
     if (T == 0) {
@@ -616,6 +624,7 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     g.perm = perm[cur];
     g.fill = fill_next(chunk_workers, passes + 1, passes + 1);
     const bool vec = C % 8 == 0 && aligned16(dy, lddy, ds) && aligned16(grad, ldg, 4);
-    if (dy_dtype == 0) return vec ? launch_grad<float, true>(g, fillers, st) : launch_grad<float, false>(g, fillers, st);
-    return vec ? launch_grad<bf16_t, true>(g, fillers, st) : launch_grad<bf16_t, false>(g, fillers, st);
+    const bool past = vec && (long long)T * C * ds > 192ll << 20;  // (the memory-side cache holds 256 MiB)
+    if (dy_dtype == 0) return past ? launch_grad<float, true, true>(g, fillers, st) : vec ? launch_grad<float, true, false>(g, fillers, st) : launch_grad<float, false, false>(g, fillers, st);
+    return past ? launch_grad<bf16_t, true, true>(g, fillers, st) : vec ? launch_grad<bf16_t, true, false>(g, fillers, st) : launch_grad<bf16_t, false, false>(g, fillers, st);
 }

@@ -885,7 +885,7 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
                                            const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale,
                                            int zero_tail, float* lse, void* o_low, void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
-    if (d != 64 && d != 128) return CCNET_EUNSUP;
+    if ((d != 64 && d != 128) || rows > (1 << 30)) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d)) return CCNET_EINVAL;
     if ((uintptr_t)o_low & 15) return CCNET_EINVAL;
@@ -926,7 +926,7 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
                                                int H, int Hkv, int d, float scale, int zero_tail, void* workspace, size_t workspace_bytes,
                                                void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
-    if (d != 64 && d != 128) return CCNET_EUNSUP;
+    if ((d != 64 && d != 128) || rows > (1 << 30)) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !lse || !workspace || ((uintptr_t)workspace & 15) || ((uintptr_t)o_low & 15) || !row_ok(Q, ldq, H * d) ||
         !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) ||

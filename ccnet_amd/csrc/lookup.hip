@@ -558,7 +558,7 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
                                     size_t workspace_bytes, void* stream) {
     if (T < 0 || vocab <= 0 || vocab == 0x7fffffff || C <= 0 || (id_bytes != 4 && id_bytes != 8) || dy_dtype < 0 || dy_dtype > 1 || lddy < C || ldg < C)
         return CCNET_EINVAL;
-    if (T > (1 << 30)) return CCNET_EUNSUP;
+    if (T > (1 << 30) || ((long long)T / 512 + 1) * ((C + 511) / 512) > 0x3fffffffLL) return CCNET_EUNSUP;
     const int ds = dy_dtype == 0 ? 4 : 2;
     if (!grad || ((uintptr_t)grad & 3) || (C + 511) / 512 > 65535) return CCNET_EINVAL;
     if (T > 0 && (!ids || !dy || (uintptr_t)ids % id_bytes || (uintptr_t)dy % ds)) return CCNET_EINVAL;

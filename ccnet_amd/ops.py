@@ -782,8 +782,8 @@ def _grad_list(grads, what: str):
 
 
 def _clip_outputs(grads, ptrs, sizes, out, what: str):
-    """(pointers to write to, the tensors written): in place, or `out` with the same shapes, strides and type.  That they do not
-    overlap is the library's check."""
+    """(pointers to write to, the tensors written): in place, or `out` of the same type, shapes and strides (contiguous tensors: of
+    the same numbers of elements).  That they do not overlap is the library's check."""
     if out is None:
         return ptrs, grads
     outs = list(out)
@@ -795,6 +795,12 @@ def _clip_outputs(grads, ptrs, sizes, out, what: str):
     if not same:
         raise _l.CcnetError(f"{what}: out must match the gradients' shapes, strides and type")
     return (C.c_void_p * len(outs))(*map(torch.Tensor.data_ptr, outs)), outs
+
+
+def _check_clip(rc: int, what: str) -> None:
+    if rc == -1:
+        raise _l.CcnetError(f"{what}: the tensors written overlap each other (one given twice?) or a gradient other than their own")
+    _l.check(rc, what)
 
 
 def grad_norm(grads) -> torch.Tensor:
@@ -827,8 +833,8 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
     ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
     norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _l.check(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()),
-             "clip_grad_norm")
+    _check_clip(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()),
+                "clip_grad_norm")
     return norm
 
 
@@ -842,7 +848,7 @@ def clip_grad_value(grads, limit: float, out=None) -> None:
     if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
         with torch.cuda.device(grads[0].device):
             return clip_grad_value(grads, limit, None if out is None else outs)
-    _l.check(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _raw_stream()), "clip_grad_value")
+    _check_clip(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _raw_stream()), "clip_grad_value")
 
 
 _prof_on = False

@@ -427,9 +427,14 @@ class Tape:
             if out.g is None:
                 return
             have = self.grads.get(param)
-            g = ops.embedding_grad(ids, out.g, table.shape[0], scale=scale, padding_idx=padding_idx,
-                                   out=have, accumulate=have is not None)
-            self.grads[param] = g
+            if have is not None and have.is_contiguous():
+                ops.embedding_grad(ids, out.g, table.shape[0], scale=scale, padding_idx=padding_idx, out=have, accumulate=True)
+                return
+            g = ops.embedding_grad(ids, out.g, table.shape[0], scale=scale, padding_idx=padding_idx)
+            if have is None:
+                self.grads[param] = g
+            else:
+                have += g
 
         self.steps.append(bw)
         return out

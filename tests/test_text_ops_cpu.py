@@ -67,6 +67,14 @@ def test_clip_outputs_must_not_overlap_other_gradients():
         assert go(grads, outs) == EINVAL, (grads, outs)
 
 
+def test_overlapping_clip_is_named():
+    from ccnet_amd import ops
+    with pytest.raises(_err(), match="overlap"):
+        ops._check_clip(EINVAL, "clip_grad_norm")
+    with pytest.raises(_err(), match="workspace"):
+        ops._check_clip(EWS, "clip_grad_norm")
+
+
 def test_dense_layouts():
     from ccnet_amd import ops
     x = torch.zeros(4, 6, 5)
@@ -103,7 +111,7 @@ def test_c_abi_refusals():
     for i, v, rc in ((0, None, EINVAL), (0, odd, EINVAL), (1, 255, EINVAL), (1, 248, EINVAL), (2, None, EINVAL), (3, 64, EINVAL), (4, odd, EINVAL),
                      (5, 132, EINVAL), (6, None, EINVAL), (7, 192, EINVAL), (8, None, EINVAL), (9, -1, EINVAL), (10, -1, EINVAL), (11, 0, EINVAL),
                      (11, 3, EINVAL), (12, 0, EINVAL), (13, 96, EUNSUP), (13, 32, EUNSUP), (14, 0.0, EINVAL), (14, -1.0, EINVAL),
-                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP), (17, odd, EINVAL)):
+                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP), (17, odd, EINVAL), (10, (1 << 30) + 1, EUNSUP)):
         a = list(ok)
         a[i] = v
         assert F(*a) == rc, (i, v)
@@ -123,7 +131,7 @@ def test_c_abi_refusals():
         a = list(ok)
         a[i] = 100
         assert B(*a) == EINVAL, i
-    for i, v, rc in ((8, odd, EINVAL), (26, odd, EINVAL), (21, 3, EINVAL), (23, 80, EUNSUP), (24, 0.0, EINVAL), (20, 0, 0), (27, need - 1, EWS)):
+    for i, v, rc in ((8, odd, EINVAL), (26, odd, EINVAL), (21, 3, EINVAL), (23, 80, EUNSUP), (24, 0.0, EINVAL), (20, 0, 0), (20, (1 << 30) + 1, EUNSUP), (27, need - 1, EWS)):
         a = list(ok)
         a[i] = v
         assert B(*a) == rc, (i, v)

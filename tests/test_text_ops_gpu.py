@@ -92,7 +92,7 @@ def _ids_of(kind, T, vocab, seed):
 @pytest.mark.parametrize("T,vocab,C", [(0, 5, 8), (1, 1, 1), (1, 300000, 8), (63, 2, 64), (64, 17, 333), (65, 1000, 1024), (97, 3, 520),
                                        (511, 17, 40), (512, 1, 512), (513, 2, 1032), (2464, 49408, 64), (8192, 1000, 24),
                                        (8193, 1000, 24), (8192, 262143, 8), (5000, 262144, 8), (20000, 70000, 16), (50001, 255, 72),
-                                       (12289, 256, 9)])
+                                       (12289, 256, 9), (300, 20_000_000, 1), (9000, 20_000_000, 1)])
 @pytest.mark.parametrize("kind", ["uniform", "one", "mostly", "two"])
 def test_table_gradient(cuda, T, vocab, C, kind):
     ops = _ops()
@@ -154,6 +154,26 @@ def test_table_gradient_in_strided_memory(cuda):
         ops.embedding_grad(ids, dy, 33, out=buf[:, off:off + C])
         _within(buf[:, off:off + C], ref, tol, "strided")
         assert (buf[:, :off] == 2).all() and (buf[:, off + C:] == 2).all()
+
+
+def test_table_gradient_in_a_graph_serves_other_ids(cuda):
+    ops = _ops()
+    for T, vocab in ((700, 90), (20000, 3000)):
+        ids, dy = _ids_of("mostly", T, vocab, 1), _randn(T, 40, seed=1)
+        out = torch.full((vocab, 40), 5.0, device="cuda")
+        ops.embedding_grad(ids, dy, vocab, out=out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.embedding_grad(ids, dy, vocab, out=out)
+            rows = ops.embedding(ids, out, dtype=F32)
+        for k, kind in enumerate(("uniform", "one", "two", "mostly")):
+            ids.copy_(_ids_of(kind, T, vocab, k))
+            dy.copy_(_randn(T, 40, seed=k + 5))
+            graph.replay()
+            torch.cuda.synchronize()
+            got, looked = out.clone(), rows.clone()
+            assert torch.equal(got, ops.embedding_grad(ids, dy, vocab)) and torch.equal(looked, got[ids]), kind
 
 
 def test_table_gradient_against_differences(cuda):

@@ -877,7 +877,10 @@ int parts_of(int n_seq, int rows, int H, int Hkv) {
 }
 size_t delta_bytes(int rows, int H) { return ((size_t)rows * H * 4 + 255) & ~(size_t)255; }
 
-bool row_ok(const void* p, int ld, int width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
+constexpr long long MOST_GROUPS = (1 << 24) - 1;  // (a launch has less than 2^32 threads)
+
+RowSpan span(const void* p, int ld, int width, int rows) { return {p, 2ll * ld, 2ll * width, rows}; }
+bool row_ok(const void* p, int ld, long long width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
 
 }  // namespace
 
@@ -885,11 +888,15 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
                                            const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale,
                                            int zero_tail, float* lse, void* o_low, void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
-    if ((d != 64 && d != 128) || rows > (1 << 30)) return CCNET_EUNSUP;
+    if ((d != 64 && d != 128) || rows > (1 << 29) || H > (1 << 20)) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d)) return CCNET_EINVAL;
     if ((uintptr_t)o_low & 15) return CCNET_EINVAL;
     if (ldk > (1 << 24) || ldv > (1 << 24)) return CCNET_EUNSUP;
+    const RowSpan q = span(Q, ldq, H * d, rows), k = span(K, ldk, Hkv * d, rows), v = span(V, ldv, Hkv * d, rows), o = span(O, ldo, H * d, rows),
+                  low = span(o_low, H * d, H * d, rows);
+    if (!spans_apart(o, k) || !spans_apart(o, v) || !(spans_apart(o, q) || (O == Q && ldo == ldq))) return CCNET_EINVAL;
+    if (!spans_apart(low, q) || !spans_apart(low, k) || !spans_apart(low, v) || !spans_apart(low, o)) return CCNET_EINVAL;
     PackedArgs a{};
     a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.out = (__bf16*)O;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;
@@ -902,7 +909,7 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     const bool wide = d == 64 && rows >= 512ll * n_seq && (long long)rows * H >= 256ll * 1024;
     const int waves = waves_of(rows, n_seq, d);
     const long long grid = most_tiles(rows, n_seq, wide ? 256 : 32 * waves, a.zero_tail) * H;
-    if (grid > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (grid > MOST_GROUPS) return CCNET_EUNSUP;
     if (grid == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     const dim3 g((unsigned)grid), b(64 * waves);
@@ -926,7 +933,7 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
                                                int H, int Hkv, int d, float scale, int zero_tail, void* workspace, size_t workspace_bytes,
                                                void* stream) {
     if (rows < 0 || n_seq < 0 || H <= 0 || Hkv <= 0 || H % Hkv || !(scale > 0.f) || scale > 3.0e38f) return CCNET_EINVAL;
-    if ((d != 64 && d != 128) || rows > (1 << 30)) return CCNET_EUNSUP;
+    if ((d != 64 && d != 128) || rows > (1 << 29) || H > (1 << 20)) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !lse || !workspace || ((uintptr_t)workspace & 15) || ((uintptr_t)o_low & 15) || !row_ok(Q, ldq, H * d) ||
         !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) ||
@@ -934,6 +941,16 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
         return CCNET_EINVAL;
     if (ldq > (1 << 24) || ldk > (1 << 24) || ldv > (1 << 24) || lddo > (1 << 24)) return CCNET_EUNSUP;
     if (workspace_bytes < ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d)) return CCNET_EWS;
+    const RowSpan in[] = {span(Q, ldq, H * d, rows),         span(K, ldk, Hkv * d, rows),  span(V, ldv, Hkv * d, rows),
+                          span(O, ldo, H * d, rows),         span(dO, lddo, H * d, rows),  span(o_low, H * d, H * d, rows),
+                          span(lse, 2 * rows, 2 * rows, H)};
+    const RowSpan out[] = {span(dQ, lddq, H * d, rows), span(dK, lddk, Hkv * d, rows), span(dV, lddv, Hkv * d, rows)};
+    for (int i = 0; i < 3; ++i) {
+        for (const RowSpan& s : in)
+            if (!spans_apart(out[i], s)) return CCNET_EINVAL;
+        for (int j = 0; j < i; ++j)
+            if (!spans_apart(out[i], out[j])) return CCNET_EINVAL;
+    }
     PackedArgs a{};
     a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.O = (const __bf16*)O; a.dO = (const __bf16*)dO;
     a.o_low = (__bf16*)o_low;
@@ -947,7 +964,7 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     a.parts = parts_of(n_seq, rows, H, Hkv);
     const int waves = waves_of(rows, n_seq, d);
     const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, 32 * waves, a.zero_tail);
-    if (qtiles * H > 0x7fffffffLL) return CCNET_EUNSUP;
+    if (qtiles * H > MOST_GROUPS) return CCNET_EUNSUP;
     if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     const dim3 gq((unsigned)(qtiles * H)), gk((unsigned)(tiles * Hkv * a.parts)), b(64 * waves);

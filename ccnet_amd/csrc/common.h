@@ -17,6 +17,19 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
         if (hipGetLastError() != hipSuccess) return CCNET_ELAUNCH; \
     } while (0)
 
+// Whether two matrices of rows (`ld` bytes apart, `width` bytes used) share no byte: their ranges are apart, or they are column
+// slices of rows of one stride.  (Ranges that mingle under different strides count as shared.)
+struct RowSpan { const void* p; long long ld, width, rows; };
+inline bool spans_apart(const RowSpan& a, const RowSpan& b) {
+    if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return true;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    if (x + (a.rows - 1) * a.ld + a.width <= y || y + (b.rows - 1) * b.ld + b.width <= x) return true;
+    const long long ld = a.rows == 1 ? b.ld : a.ld;
+    if (b.rows > 1 && b.ld != ld) return false;
+    const long long at = x <= y ? (long long)((y - x) % ld) : (ld - (long long)((x - y) % ld)) % ld;
+    return at >= a.width && ld - at >= b.width;
+}
+
 __device__ __forceinline__ float bf16_bits_to_f32(unsigned short b) {
     return __uint_as_float(((unsigned int)b) << 16);
 }

@@ -160,13 +160,16 @@ __global__ __launch_bounds__(1024) void rank_sort_kernel(const void* ids, int wi
     }
 }
 
-// More positions: least significant digits first, 8 bits a pass, RS_BLOCK positions a workgroup.  hist[block][digit].
-constexpr int RS_BLOCK = 2048, RS_THREADS = 512, RS_ROUNDS = RS_BLOCK / RS_THREADS;
+// More positions: least significant digits first, 8 bits a pass; a workgroup takes `per` positions, in blocks of RS_BLOCK.  Every
+// workgroup adds the counts hist[workgroup][digit] of the ones in front of it itself, a launch less than a scan of its own; as that
+// work grows with the square of their number, there are at most RS_MOST (16.8M positions x 320: 8550 us without a limit, 3140 with
+// 256, 3090 with 1024, 3075 with 512).
+constexpr int RS_BLOCK = 2048, RS_MOST = 512, RS_THREADS = 512, RS_ROUNDS = RS_BLOCK / RS_THREADS;
 struct SortArgs {
     const void* ids; int wide; int T, vocab; long long padding;
     const int* keys_in; const int* perm_in;  // NULL on the first pass: the ids themselves, in order
     int* keys_out; int* perm_out;
-    int* hist; int shift;
+    int* hist; int shift, per;
     Fill fill;
 };
 __device__ __forceinline__ int sort_key(const SortArgs& a, long long t) {
@@ -177,8 +180,9 @@ __global__ __launch_bounds__(RS_THREADS) void sort_hist_kernel(const SortArgs a)
     if (fill_part(a.fill)) return;
     if (threadIdx.x < 256) h[threadIdx.x] = 0;
     __syncthreads();
-    const long long t0 = (long long)blockIdx.x * RS_BLOCK;
-    for (int i = threadIdx.x; i < RS_BLOCK && t0 + i < a.T; i += RS_THREADS) atomicAdd(&h[(sort_key(a, t0 + i) >> a.shift) & 255], 1);
+    const long long t0 = (long long)blockIdx.x * a.per;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < a.per && t0 + i < a.T; i += RS_THREADS) atomicAdd(&h[(sort_key(a, t0 + i) >> a.shift) & 255], 1);
     __syncthreads();
     if (threadIdx.x < 256) a.hist[blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
 }
@@ -216,46 +220,55 @@ __global__ __launch_bounds__(RS_THREADS) void sort_scatter_kernel(const SortArgs
 #pragma unroll
         for (int e = 0; e < 4; ++e) base[0][lane * 4 + e] += base[1][lane * 4 + e] + up - s + v[e];
     }
-    // a wave takes RS_ROUNDS * 64 neighbouring positions in order; equal digits of a round find each other by ballots
-    const long long t0 = (long long)blockIdx.x * RS_BLOCK + wave * (RS_ROUNDS * 64);
-    int key[RS_ROUNDS], perm[RS_ROUNDS], rank[RS_ROUNDS];
-    volatile int* mine = count[wave];
+    // a wave takes RS_ROUNDS * 64 neighbouring positions of a block in order; equal digits of a round find each other by ballots
+    const long long end = min((long long)a.T, (long long)(blockIdx.x + 1) * a.per);
+    for (long long block = (long long)blockIdx.x * a.per;;) {
+        const long long t0 = block + wave * (RS_ROUNDS * 64);
+        int key[RS_ROUNDS], perm[RS_ROUNDS], rank[RS_ROUNDS];
+        volatile int* mine = count[wave];
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
-        const long long t = t0 + r * 64 + lane;
-        const bool ok = t < a.T;
-        key[r] = ok ? sort_key(a, t) : 0;
-        perm[r] = ok ? (a.perm_in ? a.perm_in[t] : (int)t) : 0;
-        const int digit = (key[r] >> a.shift) & 255;
-        unsigned long long same = __ballot(ok);
+        for (int r = 0; r < RS_ROUNDS; ++r) {
+            const long long t = t0 + r * 64 + lane;
+            const bool ok = t < a.T;
+            key[r] = ok ? sort_key(a, t) : 0;
+            perm[r] = ok ? (a.perm_in ? a.perm_in[t] : (int)t) : 0;
+            const int digit = (key[r] >> a.shift) & 255;
+            unsigned long long same = __ballot(ok);
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
-            const unsigned long long has = __ballot((digit >> b) & 1);
-            same &= (digit >> b) & 1 ? has : ~has;
+            for (int b = 0; b < 8; ++b) {
+                const unsigned long long has = __ballot((digit >> b) & 1);
+                same &= (digit >> b) & 1 ? has : ~has;
+            }
+            const int lower = __popcll(same & ((1ull << lane) - 1));
+            if (ok) rank[r] = mine[digit] + lower;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (ok && lower == 0) mine[digit] += __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        const int lower = __popcll(same & ((1ull << lane) - 1));
-        if (ok) rank[r] = mine[digit] + lower;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (ok && lower == 0) mine[digit] += __popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    __syncthreads();
-    if (tid < 256) {  // where each wave's run of a digit begins
-        int s = base[0][tid];
-        for (int w = 0; w < WAVES; ++w) {
-            const int c = count[w][tid];
-            count[w][tid] = s;
-            s += c;
+        __syncthreads();
+        if (tid < 256) {  // where each wave's run of a digit begins
+            int s = base[0][tid];
+            for (int w = 0; w < WAVES; ++w) {
+                const int c = count[w][tid];
+                count[w][tid] = s;
+                s += c;
+            }
+            base[0][tid] = s;
         }
-    }
-    __syncthreads();
+        __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RS_ROUNDS; ++r) {
-        if (t0 + r * 64 + lane < a.T) {
-            const int at = count[wave][(key[r] >> a.shift) & 255] + rank[r];
-            a.keys_out[at] = key[r];
-            a.perm_out[at] = perm[r];
+        for (int r = 0; r < RS_ROUNDS; ++r) {
+            if (t0 + r * 64 + lane < a.T) {
+                const int at = count[wave][(key[r] >> a.shift) & 255] + rank[r];
+                a.keys_out[at] = key[r];
+                a.perm_out[at] = perm[r];
+            }
         }
+        block += RS_BLOCK;
+        if (block >= end) return;
+        __syncthreads();
+        for (int i = tid; i < WAVES * 256; i += RS_THREADS) (&count[0][0])[i] = 0;
+        __syncthreads();
     }
 }
 
@@ -494,9 +507,15 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
 template <typename TW, typename TO>
 void launch_lookup(bool vec, const void* ids, int wide, int T, int vocab, const void* table, int ldt, int C, float scale, void* out, int ldo,
                    hipStream_t st) {
-    const dim3 grid((unsigned)(((long long)T + 3) / 4));
-    if (vec) hipLaunchKernelGGL((lookup_kernel<TW, TO, true>), grid, dim3(256), 0, st, ids, wide, T, vocab, (const TW*)table, (long long)ldt, C, scale, (TO*)out, (long long)ldo);
-    else hipLaunchKernelGGL((lookup_kernel<TW, TO, false>), grid, dim3(256), 0, st, ids, wide, T, vocab, (const TW*)table, (long long)ldt, C, scale, (TO*)out, (long long)ldo);
+    constexpr int MOST = 1 << 25;  // (a launch has less than 2^32 threads)
+    for (long long t = 0; t < T; t += MOST) {
+        const int n = (int)std::min<long long>(T - t, MOST);
+        const dim3 grid((unsigned)((n + 3) / 4));
+        const void* id = (const char*)ids + t * (wide ? 8 : 4);
+        TO* to = (TO*)out + t * ldo;
+        if (vec) hipLaunchKernelGGL((lookup_kernel<TW, TO, true>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
+        else hipLaunchKernelGGL((lookup_kernel<TW, TO, false>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
+    }
 }
 
 template <typename T, bool VEC, bool PAST>
@@ -513,6 +532,8 @@ int launch_grad(GradArgs a, unsigned fillers, hipStream_t st) {
 
 bool aligned16(const void* p, long long ld, int esz) { return !((uintptr_t)p & 15) && (ld * esz) % 16 == 0; }
 
+int sort_per(int T) { return T > 0 ? ((T - 1) / (RS_MOST * RS_BLOCK) + 1) * RS_BLOCK : RS_BLOCK; }
+
 // workspace: sorted keys and positions (twice: a pass reads one copy and writes the other), digit counts, chunk sums
 struct Layout { size_t keys[2], perm[2], hist, p64, p512, bytes; };
 Layout layout_of(int T, int C) {
@@ -520,7 +541,7 @@ Layout layout_of(int T, int C) {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t r = at; at += (n + 255) & ~(size_t)255; return r; };
     for (int i = 0; i < 2; ++i) { l.keys[i] = take((size_t)T * 4); l.perm[i] = take((size_t)T * 4); }
-    l.hist = take(((size_t)T + RS_BLOCK - 1) / RS_BLOCK * 1024);
+    l.hist = take(((size_t)T + sort_per(T) - 1) / sort_per(T) * 1024);
     l.p64 = take((size_t)(T / 64) * C * 4);
     l.p512 = take((size_t)(T / 512) * C * 4);
     l.bytes = at;
@@ -537,6 +558,8 @@ extern "C" int ccnet_embedding(const void* ids, int id_bytes, int T, int vocab, 
     if (T == 0) return CCNET_OK;
     const int ws = table_dtype == 0 ? 4 : 2, os = out_dtype == 0 ? 4 : 2;
     if (!ids || !table || !out || (uintptr_t)ids % id_bytes || (uintptr_t)table % ws || (uintptr_t)out % os) return CCNET_EINVAL;
+    const RowSpan to{out, (long long)ldo * os, (long long)C * os, T};
+    if (!spans_apart(to, {table, (long long)ldt * ws, (long long)C * ws, vocab}) || !spans_apart(to, {ids, id_bytes, id_bytes, T})) return CCNET_EINVAL;
     const bool vec = C % 8 == 0 && aligned16(table, ldt, ws) && aligned16(out, ldo, os);
     hipStream_t st = (hipStream_t)stream;
     const int wide = id_bytes == 8;
@@ -558,13 +581,15 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
                                     size_t workspace_bytes, void* stream) {
     if (T < 0 || vocab <= 0 || vocab == 0x7fffffff || C <= 0 || (id_bytes != 4 && id_bytes != 8) || dy_dtype < 0 || dy_dtype > 1 || lddy < C || ldg < C)
         return CCNET_EINVAL;
-    if (T > (1 << 30) || ((long long)T / 512 + 1) * ((C + 511) / 512) > 0x3fffffffLL) return CCNET_EUNSUP;
+    if (T > (1 << 29) || ((long long)T / 512 + 1) * ((C + 511) / 512) > 0x3fffffffLL) return CCNET_EUNSUP;
     const int ds = dy_dtype == 0 ? 4 : 2;
     if (!grad || ((uintptr_t)grad & 3) || (C + 511) / 512 > 65535) return CCNET_EINVAL;
     if (T > 0 && (!ids || !dy || (uintptr_t)ids % id_bytes || (uintptr_t)dy % ds)) return CCNET_EINVAL;
     const Layout l = layout_of(T, C);
     if (T > 0 && (!workspace || ((uintptr_t)workspace & 15))) return CCNET_EINVAL;
     if (T > 0 && workspace_bytes < l.bytes) return CCNET_EWS;
+    const RowSpan to{grad, (long long)ldg * 4, (long long)C * 4, vocab};
+    if (!spans_apart(to, {dy, (long long)lddy * ds, (long long)C * ds, T}) || !spans_apart(to, {ids, id_bytes, id_bytes, T})) return CCNET_EINVAL;
     if (T == 0 && accumulate) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     // the table's zeros in parts [0, vocab): part k of n with a launch that has `workers` workgroups of its own
@@ -604,7 +629,8 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     } else {
         SortArgs s{};
         s.ids = ids; s.wide = id_bytes == 8; s.T = T; s.vocab = vocab; s.padding = padding_idx; s.hist = (int*)(ws + l.hist);
-        const int blocks = (T + RS_BLOCK - 1) / RS_BLOCK;
+        s.per = sort_per(T);
+        const int blocks = (T - 1) / s.per + 1;
         for (int shift = 0; shift < 32 && (vocab >> shift) > 0; shift += 8) passes += 2;
         cur = 1;
         for (int k = 0; k < passes; k += 2) {

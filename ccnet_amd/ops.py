@@ -632,7 +632,8 @@ def _ids(ids: torch.Tensor) -> torch.Tensor:
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype: torch.dtype = BF16,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scale * table[ids] as [ids.numel(), C] rows: ids int64 / int32, table fp32 / bf16 [vocab, C] (row stride free), result in
-    `dtype` (fp32 / bf16, rounded once) or in `out`.  An id outside the table gives a row of zeros."""
+    `dtype` (fp32 / bf16, rounded once) or in `out`, which shares no memory with the others (the library refuses it).  An id
+    outside the table gives a row of zeros."""
     lib = _l.load()
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise _l.CcnetError(f"table must be [vocab, C], got {list(table.shape)}")
@@ -654,7 +655,7 @@ def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float
                    out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """Gradient of `embedding` with respect to its table, fp32 [vocab, C]: row v = scale * sum of dy[t] over ids[t] == v (zeros
     for rows no position names).  dy fp32 / bf16 [T, C].  Positions with padding_idx or an id outside the table take no part.
-    accumulate: added to `out`, whose other rows are not touched."""
+    accumulate: added to `out`, whose other rows are not touched.  out shares no memory with dy or ids."""
     lib = _l.load()
     if accumulate and out is None:
         raise _l.CcnetError("embedding_grad: accumulate needs out")
@@ -704,8 +705,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Causal self-attention over sequences that lie end to end in the rows: q [rows, H*d], k / v [rows, Hkv*d] bf16 (column
     slices of one matrix allowed), query head h on key head h // (H // Hkv), d 64 or 128, sequence i = rows
     cu_seqlens[i] .. cu_seqlens[i+1] (int32 on the GPU, never copied to the host).  Returns o [rows, H*d], with_lse: (o, stats) for
-    `attention_packed_bwd`.  Rows behind the last sequence are zeros, or with `out` (which must not overlap k or v) left as
-    they are."""
+    `attention_packed_bwd`.  Rows behind the last sequence are zeros, or with `out` (q itself, or a tensor that shares
+    no memory with q, k or v) left as they are."""
     lib = _l.load()
     if _elsewhere(q, k, v, cu_seqlens, out):
         with torch.cuda.device(q.device):
@@ -727,7 +728,8 @@ def attention_packed_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
                          dk: Optional[torch.Tensor] = None, dv: Optional[torch.Tensor] = None):
     """(dq, dk, dv) of `attention_packed` from its (o, stats) and the gradient `do` of o; dk / dv hold the sum over the query heads
     of a key head.  The results overwrite dq / dk / dv where given (all three, e.g. column slices of one matrix; rows behind the
-    last sequence are then left as they are) or are new tensors (those rows zeros)."""
+    last sequence are then left as they are; they share no memory with one another or the operands) or are new tensors (those
+    rows zeros)."""
     lib = _l.load()
     given = dq is not None
     if given != (dk is not None) or given != (dv is not None):

@@ -385,7 +385,9 @@ int ccnet_resample_bwd_bf16(const void* in, int ldi, void* out, int ldo, int N, 
 /* ---------------------------------------------------------------------------------------------------------------------
  * Token lookup, causal attention over packed prompts and gradient clipping: the text side of training.  dtype codes of these
  * entry points: 0 = fp32, 1 = bf16.  Sums and statistics are fp32 or fp64, in an order that the inputs alone fix (no float
- * atomics), so equal inputs give equal bits.  Wrong ids or offsets in device memory give wrong rows, never an access outside. */
+ * atomics), so equal inputs give equal bits.  Wrong ids or offsets in device memory give wrong rows, never an access outside.
+ * Results that share memory with an operand or with one another are refused (CCNET_EINVAL) except where said; column slices of
+ * rows of one stride share none. */
 
 /* out[t][0..C) = scale * table[ids[t]][0..C), rounded once; an id outside [0, vocab) gives a row of zeros.  ids: id_bytes (4 or
  * 8) wide.  Any C and strides >= C (16-byte accesses where C % 8 == 0 and both matrices' rows are 16-byte aligned). */
@@ -393,7 +395,7 @@ int ccnet_embedding(const void* ids, int id_bytes, int T, int vocab, const void*
                     void* out, int out_dtype, int ldo, void* stream);
 /* grad[v] (fp32) = scale * sum of dy[t] over the positions with ids[t] = v; every row is written, rows without a position as
  * zeros.  accumulate != 0: added to what is there, rows without a position are not touched.  Positions whose id is outside
- * [0, vocab) or equal to padding_idx (-1: none) take no part.  T <= 2^30; workspace (16-byte aligned):
+ * [0, vocab) or equal to padding_idx (-1: none) take no part.  T <= 2^29; workspace (16-byte aligned):
  * ccnet_embedding_grad_workspace_bytes(T, C) bytes. */
 size_t ccnet_embedding_grad_workspace_bytes(int T, int C);
 int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const void* dy, int dy_dtype, int lddy, int C, float scale,
@@ -406,8 +408,8 @@ int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const 
  *   out = softmax(scale q k^T) v;   lse[h][row] (may be NULL) = log2 of the sum of 2^(scale log2(e) q k^T);
  *   o_low [rows][H d] (may be NULL) = what the rounding of out to bf16 took away, itself rounded to bf16
  * Rows behind the last sequence: left as they are, or with zero_tail != 0 written as zeros (lse: -inf).  A key or value that is
- * not finite reaches only the queries of its sequence that see it.  16-byte aligned rows (ld % 8 == 0); out must not overlap
- * k or v.  Grids follow from rows and n_seq alone: a captured graph serves other lengths with the same totals. */
+ * not finite reaches only the queries of its sequence that see it.  16-byte aligned rows (ld % 8 == 0); out may be q
+ * itself.  Grids follow from rows and n_seq alone: a captured graph serves other lengths with the same totals. */
 int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo,
                                 const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale, int zero_tail,
                                 float* lse, void* o_low, void* stream);

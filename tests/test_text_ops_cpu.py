@@ -84,9 +84,9 @@ def test_dense_layouts():
 
 def test_c_abi_refusals():
     l = _lib()
-    p = C.c_void_p(1 << 20)  # never dereferenced: every call here returns before a launch
+    p, *P = [C.c_void_p((1 + k) << 20) for k in range(12)]  # never dereferenced: every call here returns before a launch
     E = l.ccnet_embedding
-    ok = [p, 8, 4, 10, p, 0, 64, 64, 1.0, p, 1, 64, None]
+    ok = [p, 8, 4, 10, P[0], 0, 64, 64, 1.0, P[1], 1, 64, None]
     for i, v in ((1, 2), (2, -1), (3, 0), (4, None), (5, 2), (6, 63), (7, 0), (9, None), (10, 3), (11, 10), (0, None), (0, C.c_void_p(1028)),
                  (4, C.c_void_p(1026)), (9, C.c_void_p(1025))):
         a = list(ok)
@@ -98,20 +98,21 @@ def test_c_abi_refusals():
     G = l.ccnet_embedding_grad
     need = l.ccnet_embedding_grad_workspace_bytes(1000, 64)
     assert need > 1000 * 16 and l.ccnet_embedding_grad_workspace_bytes(0, 64) == 0
-    ok = [p, 8, 1000, 10, p, 1, 64, 64, 1.0, -1, p, 64, 0, p, need, None]
+    ok = [p, 8, 1000, 10, P[0], 1, 64, 64, 1.0, -1, P[1], 64, 0, P[2], need, None]
     for i, v, rc in ((1, 3, EINVAL), (2, -1, EINVAL), (3, 0, EINVAL), (3, 0x7fffffff, EINVAL), (4, None, EINVAL), (5, 2, EINVAL), (6, 8, EINVAL),
                      (7, 0, EINVAL), (10, None, EINVAL), (10, C.c_void_p(1026), EINVAL), (11, 63, EINVAL), (13, None, EINVAL),
                      (13, C.c_void_p(1028), EINVAL), (14, need - 1, EWS), (2, (1 << 30) + 1, EUNSUP)):
         a = list(ok)
         a[i] = v
         assert G(*a) == rc, (i, v)
+    assert G(None, 8, 0, 10, None, 1, 64, 64, 1.0, -1, P[1], 64, 1, None, 0, None) == 0  # no positions: nothing to add
     F = l.ccnet_attention_packed_bf16
-    ok = [p, 256, p, 128, p, 128, p, 256, p, 3, 100, 4, 2, 64, 0.125, 1, None, None, None]
+    ok = [p, 256, P[0], 128, P[1], 128, P[2], 256, P[3], 3, 100, 4, 2, 64, 0.125, 1, None, None, None]
     odd = C.c_void_p(1 << 20 | 8)
     for i, v, rc in ((0, None, EINVAL), (0, odd, EINVAL), (1, 255, EINVAL), (1, 248, EINVAL), (2, None, EINVAL), (3, 64, EINVAL), (4, odd, EINVAL),
                      (5, 132, EINVAL), (6, None, EINVAL), (7, 192, EINVAL), (8, None, EINVAL), (9, -1, EINVAL), (10, -1, EINVAL), (11, 0, EINVAL),
                      (11, 3, EINVAL), (12, 0, EINVAL), (13, 96, EUNSUP), (13, 32, EUNSUP), (14, 0.0, EINVAL), (14, -1.0, EINVAL),
-                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP), (17, odd, EINVAL), (10, (1 << 30) + 1, EUNSUP)):
+                     (14, float("nan"), EINVAL), (14, float("inf"), EINVAL), (3, 1 << 25, EUNSUP), (17, odd, EINVAL), (10, (1 << 30) + 1, EUNSUP), (11, 1 << 21, EUNSUP), (9, 1 << 28, EUNSUP)):
         a = list(ok)
         a[i] = v
         assert F(*a) == rc, (i, v)
@@ -122,7 +123,7 @@ def test_c_abi_refusals():
     size = l.ccnet_attention_packed_bwd_workspace_bytes
     need = size(3, 100, 4, 2, 64)
     assert need >= 100 * 4 * 4 and size(1, 4096, 16, 4, 64) >= 4096 * 16 * 4 + 2 * 2 * 4096 * 4 * 64 * 4  # (long walks of few key heads are cut)
-    ok = [p, 256, p, 128, p, 128, p, 256, p, p, 256, p, p, 256, p, 128, p, 128, p, 3, 100, 4, 2, 64, 0.125, 1, p, need, None]
+    ok = [p, 256, P[0], 128, P[1], 128, P[2], 256, P[3], P[4], 256, P[5], P[6], 256, P[7], 128, P[8], 128, P[9], 3, 100, 4, 2, 64, 0.125, 1, P[10], need, None]
     for i in (0, 2, 4, 6, 9, 11, 12, 14, 16, 18, 26):
         a = list(ok)
         a[i] = None
@@ -153,6 +154,47 @@ def test_c_abi_refusals():
         assert l.ccnet_clip_grad_norm(ptrs, ptrs, n, 2, 0, m, p, need, p, None) == EINVAL
         assert l.ccnet_clip_grad_value(ptrs, ptrs, n, 2, 0, m, None) == EINVAL
     assert l.ccnet_clip_grad_norm(ptrs, ptrs, n, 2, 0, 1.0, p, need - 1, p, None) == EWS
+
+
+def test_results_must_not_share_memory_with_operands():
+    """Addresses that are never dereferenced: a call that breaks the rule returns CCNET_EINVAL, one that keeps it gets as far as the
+    next check or, in the last lines, to the size that no launch can have."""
+    l = _lib()
+    p = lambda b: C.c_void_p((1 << 30) + b)  # noqa: E731
+
+    def look(table, ldt, out, ldo, ids=0, T=4):  # table fp32 [10][64], out bf16 [T][64]
+        return l.ccnet_embedding(p(ids), 8, T, 10, p(table), 0, ldt, 64, 1.0, p(out), 1, ldo, None)
+
+    for a in ((4096, 64, 4096, 64), (4096, 64, 4096 + 2556, 64), (4096, 64, 4096 - 510, 64), (4096, 64, 16, 64), (4096, 256, 4096 + 2, 512), (4096, 256, 4096 + 256, 260)):
+        assert look(*a) == EINVAL, a
+    G, need = l.ccnet_embedding_grad, l.ccnet_embedding_grad_workspace_bytes(100, 64)
+    for dy, lddy, out, ldg, ids in ((1 << 20, 64, 1 << 20, 64, 0), (1 << 20, 64, (1 << 20) + 64 * 100 * 4 - 4, 64, 0), (1 << 20, 64, 400, 64, 0),
+                                    (1 << 20, 128, (1 << 20) + 252, 128, 0), (1 << 20, 128, (1 << 20) + 260, 128, 0), (1 << 20, 128, (1 << 20) + 256, 132, 0)):
+        assert G(p(ids), 8, 100, 10, p(dy), 0, lddy, 64, 1.0, -1, p(out), ldg, 0, p(1 << 25), need, None) == EINVAL, (dy, lddy, out, ldg)
+
+    most = 1 << 28  # sequences: more workgroups than a launch has, the check behind this one
+
+    def fwd(q, k, v, o, ldq=768, ldk=768, ldv=768, ldo=768, low=None):
+        return l.ccnet_attention_packed_bf16(p(q), ldq, p(k), ldk, p(v), ldv, p(o), ldo, p(0), most, 100, 4, 4, 64, 1.0, 1, None, low and p(low), None)
+
+    m = 1 << 20
+    for a in ((m, m + 512, m + 1024, 4 * m), (m, m + 512, m + 1024, m), (m, 2 * m, 3 * m, m + 512), (m, m + 512, 2 * m, m + 1024), (m, m + 512, m + 1024, m + 1536 * 100)):
+        assert fwd(*a) == EUNSUP, a
+    for a in ((m, m + 512, m + 1024, m + 512), (m, m + 512, m + 1024, m + 1024), (m, m + 512, m + 1024, m + 16), (m, 2 * m, 3 * m, m + 1536), (m, m + 512, m + 1024, m + 1536 * 99)):
+        assert fwd(*a) == EINVAL, a
+    assert fwd(m, 2 * m, 3 * m, m, ldo=776) == EINVAL and fwd(m, 2 * m, 3 * m, m + 512, ldo=776) == EINVAL
+    assert fwd(m, 2 * m, 3 * m, 4 * m, low=5 * m) == EUNSUP and fwd(m, 2 * m, 3 * m, 4 * m, low=4 * m) == EINVAL
+    size = l.ccnet_attention_packed_bwd_workspace_bytes(most, 100, 4, 4, 64)
+
+    def bwd(dq, dk, dv, ld=768):  # q, k, v slices of one matrix at 1 m, o at 2 m, o_low 3 m, do 4 m, lse 5 m
+        return l.ccnet_attention_packed_bwd_bf16(p(m), 768, p(m + 512), 768, p(m + 1024), 768, p(2 * m), 256, p(3 * m), p(4 * m), 256, p(5 * m), p(dq), ld,
+                                                 p(dk), ld, p(dv), ld, p(0), most, 100, 4, 4, 64, 1.0, 1, p(9 * m), size, None)
+
+    for a in ((6 * m, 6 * m + 512, 6 * m + 1024), (6 * m, 7 * m, 8 * m)):
+        assert bwd(*a) == EUNSUP, a
+    for a in ((m, 6 * m, 7 * m), (6 * m, 6 * m, 7 * m), (6 * m, 7 * m, 7 * m + 256), (6 * m, m + 512, 7 * m), (6 * m, 7 * m, m + 1024), (2 * m, 6 * m, 7 * m),
+              (3 * m + 51184, 6 * m, 7 * m), (6 * m, 4 * m, 7 * m), (6 * m, 7 * m, 5 * m + 1584), (6 * m + 16, 7 * m, 6 * m + 512)):
+        assert bwd(*a) == EINVAL, a
 
 
 def test_packed_attention_wrapper_refusals():

@@ -106,6 +106,30 @@ def test_table_gradient(cuda, T, vocab, C, kind):
         assert torch.equal(got, ops.embedding_grad(ids.int(), dy, vocab, scale=22.0)), "the sum's order depends on something else"
 
 
+@pytest.mark.parametrize("kind", ["uniform", "mostly"])
+def test_table_gradient_of_millions_of_positions(cuda, kind):
+    """More than a million positions: a workgroup of the sort takes several blocks one after the other."""
+    ops = _ops()
+    T, vocab, C = 2_100_003, 70000, 8
+    ids = _ids_of(kind, T, vocab, 5)
+    dy = _randn(T, C, seed=6, dtype=BF16)
+    at, x = ids.cpu(), dy.cpu().double()  # (on the CPU: one row's sum of 1.7 million terms takes atomics on the GPU minutes)
+    ref, mag, count = torch.zeros(vocab, C, dtype=F64), torch.zeros(vocab, C, dtype=F64), torch.bincount(at, minlength=vocab).double()
+    ref.index_add_(0, at, x)
+    mag.index_add_(0, at, x.abs())
+    # the sums of 512 rows (depth below 512), of which a long run's four waves each add every fourth in turn
+    tol = (count.clamp(max=512) + count / 2048)[:, None] * H32 * mag + 2 * H32 * ref.abs()
+    _within(ops.embedding_grad(ids, dy, vocab), ref.cuda(), tol.cuda(), kind)
+
+
+def test_lookup_of_more_rows_than_a_launch_takes(cuda):
+    ops = _ops()
+    table = _randn(100, 3, seed=1, dtype=BF16)
+    ids = torch.randint(0, 100, ((1 << 25) + 5,), device="cuda")
+    got = ops.embedding(ids, table)
+    assert torch.equal(got, table[ids])
+
+
 def test_table_gradient_padding_and_ids_outside(cuda):
     ops = _ops()
     for T in (300, 9000):

@@ -288,10 +288,11 @@ def _run_attention(q, k, v, do, cu, H, Hkv, d, scale):
 
 LENS = [(1,), (2,), (31,), (32,), (33,), (77,), (63, 64, 65), (127, 128, 129), (0, 5, 0, 0, 77, 0), (256,), (257, 300), (511, 3, 640),
         tuple(range(1, 78)), (1,) * 130]
+MANY = tuple((i * 37 + i // 5) % 71 for i in range(290)) + (0, 0, 301, 0, 130) + (3,) * 10  # (more sequences than are searched in order)
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("lens", LENS, ids=lambda x: f"{len(x)}x{max(x)}")
+@pytest.mark.parametrize("lens", LENS + [MANY], ids=lambda x: f"{len(x)}x{max(x)}")
 def test_packed_attention(cuda, lens, d):
     for H, Hkv in ((1, 1), (6, 2)):
         q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=sum(lens) + d + H)
@@ -338,9 +339,10 @@ def test_packed_attention_without_sequences_or_rows(cuda, d):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_rows_behind_the_last_sequence(cuda, d):
+@pytest.mark.parametrize("lens", [(70, 33), MANY], ids=lambda x: f"{len(x)}x{max(x)}")
+def test_rows_behind_the_last_sequence(cuda, lens, d):
     ops = _ops()
-    lens, H, Hkv = (70, 33), 4, 2
+    H, Hkv = 4, 2
     q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, pad=141, seed=3)
     n = sum(lens)
     clean = _run_attention(q[:n], k[:n], v[:n], do[:n], cu, H, Hkv, d, 0.1)
@@ -465,6 +467,10 @@ def test_packed_attention_offsets_that_are_wrong_stay_inside(cuda):
     assert all(torch.equal(got[x], ref[x]) for x in NAMES)
     got = _run_attention(q, k, v, do, torch.tensor([0, 100, 40], dtype=torch.int32, device="cuda"), 2, 2, 64, 0.1)
     assert torch.isfinite(got["o"]).all()
+    cu = torch.randint(-10, 120, (400,), generator=torch.Generator().manual_seed(2), dtype=torch.int32).cuda()
+    got = _run_attention(q, k, v, do, cu, 2, 2, 64, 0.1)
+    assert got["o"].shape == ref["o"].shape and torch.equal(_run_attention(q, k, v, do, torch.tensor([0] + [100] * 300, dtype=torch.int32, device="cuda"),
+                                                                         2, 2, 64, 0.1)["o"], ref["o"])
 
 
 def test_packed_attention_in_a_graph_serves_other_lengths(cuda):

@@ -36,6 +36,8 @@ struct PackedArgs {
     float* lse;     // [H][rows]
     float* delta;   // [H][rows]
     __bf16* o_low;  // [rows][H d]: what the rounding of O took away
+    int skip;       // sequences of at most so many rows have no tiles (packed_bwd_short_kernel takes them)
+    int rest, per;  // its workgroups for longer sequences, and how many heads or key heads each takes one after the other
     int parts;      // dK / dV: workgroups that share a key tile's walk, each with H / Hkv / parts query heads
     float* part;    // parts > 1: [parts][2][rows][Hkv d] sums of dK (not scaled yet) and dV
 };
@@ -136,7 +138,7 @@ __device__ __forceinline__ bool find_place(const PackedArgs& a, int idx, bool fr
     t.ntiles = (t.len + step - 1) / step;
     t.tail = lo == a.n_seq;
     const int k = idx - (t.start / step + lo);
-    if (k < 0 || k >= t.ntiles) return false;
+    if (k < 0 || k >= t.ntiles || (t.len <= a.skip && !t.tail)) return false;
     t.tile = from_end ? k : t.ntiles - 1 - k;
     return true;
 }
@@ -148,7 +150,7 @@ __device__ __forceinline__ bool find_tile(const PackedArgs& a, int idx, bool fro
         if (i >= n) { s = 0; return 0; }
         s = min(max(a.cu[i], 0), a.rows);
         const int e = i < a.n_seq ? min(max(a.cu[i + 1], s), a.rows) : (a.zero_tail ? a.rows : s);
-        return e - s;
+        return i < a.n_seq && e - s <= a.skip ? 0 : e - s;
     };
     int s0;
     const int len0 = span(lane, s0), nt0 = (len0 + step - 1) / step;  // the first 64 sequences stay in registers
@@ -551,14 +553,11 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
 // and left for the dK / dV kernel.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
+__device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int h, char* smem) {
     constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
-    __shared__ __attribute__((aligned(1024))) char smem[5 * TILEB];  // V 0, V 1, K 0, K 1, K 2
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
-    Tile tl;
-    if (!find_tile<BM>(a, blockIdx.x / a.H, false, tl)) return;
-    const int h = head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), kvh = h / (a.H / a.Hkv);
+    const int kvh = h / (a.H / a.Hkv);
     const int q0 = tl.tile * BM + wave * 32, q = q0 + l31;
     const bool qok = q < tl.len;
     const long long row = tl.start + (qok ? q : 0);
@@ -597,18 +596,19 @@ __global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedAr
 #pragma unroll
             for (int j = 0; j < 8; ++j) dlt = fmaf(x[j] + l[j], y[j], dlt);
         }
-        dlt = half_sum(dlt);
-        if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = -dlt;  // (negative: where dP starts from)
+        dlt = -half_sum(dlt);  // (negative: where dP starts from)
+        if (hh == 0 && qok) a.delta[(long long)h * a.rows + row] = dlt;
         float lse = qok ? a.lse[(long long)h * a.rows + row] : 0.f;
         int rread[NK], klo[ND], khi[ND];
 #pragma unroll
         for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, klo[d], khi[d]);
+        constexpr bool FROM_DELTA = D == 64;  // (dP begins at -delta, to the bit as in the other kernels; at d 128 that spills)
         f32x16 s, dp;
         auto scores = [&](f32x16& sr, f32x16& dr, const char* kb, const char* vb) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = 0.f; }
+            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = FROM_DELTA ? dlt : 0.f; }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
                 sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kb + rread[ks]), qf[ks], sr, 0, 0, 0);
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedAr
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int e = 8 * sI + j;
-                    ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (dp[e] - dlt);
+                    ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (FROM_DELTA ? dp[e] : dp[e] + dlt);
                     if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > l31) ds[j] = 0.f;
                 }
                 dsf[sI] = __builtin_bit_cast(bf16x8, pack8(ds));
@@ -684,22 +684,26 @@ __global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedAr
     store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, qok);
 }
 
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[5 * PA_TILE * 2 * D];  // V 0, V 1, K 0, K 1, K 2
+    Tile tl;
+    if (find_tile<32 * W>(a, blockIdx.x / a.H, false, tl)) dq_walk<D, W>(a, tl, head_of_slot(blockIdx.x % a.H, a.H, a.Hkv), smem);
+}
+
 // ------------------------------------------------------------------ backward: dK, dV
 // A wave owns 32 keys of a key head; the workgroup walks the query tiles from its own diagonal on, for the query heads of the
 // group (or of its part of it) in turn, so the group's sum is taken in the accumulators, in a fixed order.  As above the scores
 // of the next query block are computed beside the exponentials of this one; Q and dO are both needed a step longer (rings of
 // three).  Query blocks in front of a wave's own keys (in the first two tiles of a head) are masked whole.
+template <int D>
+constexpr int dkv_stage() { return 2 * PA_TILE * 2 * D + 512; }  // Q, dO, lse and delta of 64 queries
 template <int D, int W>
-__global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
-    constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, STAGEB = 2 * TILEB + 512;
-    __shared__ __attribute__((aligned(1024))) char smem[3 * STAGEB];  // per stage: Q, dO, lse and delta of the 64 queries
+__device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, int kvh, int part, char* smem) {
+    constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, STAGEB = dkv_stage<D>();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5;
-    Tile tl;
-    const int units = a.Hkv * a.parts;
-    if (!find_tile<BM>(a, blockIdx.x / units, true, tl)) return;
-    const int kvh = blockIdx.x % a.Hkv, part = blockIdx.x % units / a.Hkv, G = a.H / a.Hkv / a.parts, h0 = (kvh * a.parts + part) * G;
-    if (a.parts > 1 && tl.tail) return;  // (packed_join_kernel's)
+    const int G = a.H / a.Hkv / a.parts, h0 = (kvh * a.parts + part) * G;
     const int k0 = tl.tile * BM + wave * 32, key = k0 + l31;
     const bool kok = key < tl.len;
     const long long row = tl.start + (kok ? key : 0);
@@ -855,6 +859,192 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
     store_row<D>(a.dV + row * a.lddv + kvh * D, nullptr, dv, 1.0f, hh, kok);
 }
 
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel(const PackedArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[3 * dkv_stage<D>()];
+    Tile tl;
+    const int units = a.Hkv * a.parts;
+    if (!find_tile<32 * W>(a, blockIdx.x / units, true, tl)) return;
+    if (a.parts > 1 && tl.tail) return;  // (packed_join_kernel's)
+    dkv_walk<D, W>(a, tl, blockIdx.x % a.Hkv, blockIdx.x % units / a.Hkv, smem);
+}
+
+// ------------------------------------------------------------------ backward of short sequences
+// A sequence of at most 64 rows fits two waves and its operands one stage: one workgroup takes it, for a key head and the query heads
+// of its group in turn, from loads to dQ, dK and dV.  Every operand is read once, S and dP are computed once.  Waves own 32 keys as
+// in the dK / dV kernel (block pairs (0, 0), (0, 1); (1, 1)); dS, rounded for dK's product, is also left in LDS as rows of keys, from
+// where transposed reads give the B operand of dQ^T = K^T dS^T, the waves owning 32 queries now.
+// Sequences that are longer, a few among many, have the launch's first workgroups, which end at once where there are none: a tile of
+// 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.
+constexpr int SHORT_ROWS = 64, SHORT_SMEM = 4 * PA_TILE * 128 + 512;  // Q, dO, K, dS; lse, delta
+// dK and dV of 64 keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
+template <bool WHOLE>
+__device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len, int k0, bool tail, int kvh, char* smem) {
+    constexpr int D = 64, NK = 4, ND = 2, ROWB = 128, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+    char *qs = smem, *dos = smem + TILEB, *ks_ = smem + 2 * TILEB, *dss = smem + 3 * TILEB;
+    float* stat = (float*)(smem + 4 * TILEB);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l31 = lane & 31, hh = lane >> 5, G = a.H / a.Hkv, own = wave * 32 + l31;
+    const bool ok = k0 + own < len, busy = k0 + wave * 32 < len;
+    const long long row = start + (ok ? k0 + own : 0);
+    const long long ldqb = a.ldq * 2, lddob = a.lddo * 2, ldkb = a.ldk * 2;
+    TileDma<D, 2> qd, dd, kd;
+    qd.init(wave, lane, ldqb);
+    dd.init(wave, lane, lddob);
+    kd.init(wave, lane, ldkb);
+    const unsigned lds0 = lds_addr(smem);
+    if constexpr (WHOLE) kd.issue(row_rsrc((const char*)(a.K + (long long)start * a.ldk + kvh * D), len, ldkb, ROWB), lds0 + 2 * TILEB);
+    bf16x8 kf[NK], vf[NK];
+    load_frags<D>(kf, a.K + row * a.ldk + kvh * D, hh, ok);
+    load_frags<D>(vf, a.V + row * a.ldv + kvh * D, hh, ok);
+    int rread[NK], tlo[ND], thi[ND];
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, tlo[d], thi[d]);
+    f32x16 dk[ND], dv[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
+    int g = 0, q0 = k0;  // head of the group, first row of the tile of queries
+    for (bool first = true; g < (tail ? 0 : G); first = false) {
+        const int h = kvh * G + g, left = min(len - q0, PA_TILE);
+        const bool qok = WHOLE ? ok : own < left;
+        const long long qrow = WHOLE ? row : start + q0 + (qok ? own : 0);
+        if (!first) __syncthreads();
+        qd.issue(row_rsrc((const char*)(a.Q + (long long)(start + q0) * a.ldq + h * D), left, ldqb, ROWB), lds0);
+        dd.issue(row_rsrc((const char*)(a.dO + (long long)(start + q0) * a.lddo + h * D), left, lddob, ROWB), lds0 + TILEB);
+        // delta of the wave's 32 queries: O and what its rounding took away from memory, dO from LDS
+        u32x4 ov[NK], lv[NK];
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            ov[ks] = lv[ks] = u32x4{0u, 0u, 0u, 0u};
+            if (qok) ov[ks] = *(const u32x4*)(a.O + qrow * a.ldo + h * D + ks * 16 + hh * 8);
+            if (qok && a.o_low) lv[ks] = *(const u32x4*)(a.o_low + (qrow * a.H + h) * D + ks * 16 + hh * 8);
+        }
+        const float lse = qok ? a.lse[(long long)h * a.rows + qrow] : 0.f;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the wave's own pieces; the other's behind the barrier)
+        __syncthreads();
+        float dlt = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            float x[8], l[8], y[8];
+            unpack8(ov[ks], x);
+            unpack8(lv[ks], l);
+            unpack8(*(const u32x4*)(dos + wave * BLOCKB + rread[ks]), y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dlt = fmaf(x[j] + l[j], y[j], dlt);
+        }
+        dlt = half_sum(dlt);
+        if (hh == 0) {  // (queries behind the end: zero, P = 1 meets only zeros)
+            stat[own] = lse;
+            stat[64 + own] = -dlt;
+        }
+        __syncthreads();
+        if (busy) {
+            for (int b = WHOLE || q0 == k0 ? wave : 0; b < 2 && b * 32 < left; ++b) {
+                const float* st = stat + 32 * b;
+                const char *qb = qs + b * BLOCKB, *db = dos + b * BLOCKB;
+                f32x16 s, dp;
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {
+                    const f32x4 d4 = *(const f32x4*)(st + 64 + 8 * gq + 4 * hh);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { s[4 * gq + j] = 0.f; dp[4 * gq + j] = d4[j]; }
+                }
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], s, 0, 0, 0);
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(db + rread[ks]), vf[ks], dp, 0, 0, 0);
+                }
+                if (b == wave && (WHOLE || q0 == k0)) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if ((e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
+                }
+                bf16x8 pfr[2], dsf[2];
+#pragma unroll
+                for (int sI = 0; sI < 2; ++sI) {
+                    float p[8], ds[8];
+#pragma unroll
+                    for (int gq = 0; gq < 2; ++gq) {
+                        const f32x4 l4 = *(const f32x4*)(st + 16 * sI + 8 * gq + 4 * hh);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int e = 8 * sI + 4 * gq + j;
+                            p[4 * gq + j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -l4[j]));
+                            ds[4 * gq + j] = p[4 * gq + j] * dp[e];
+                        }
+                    }
+                    pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
+                    const u32x4 packed = pack8(ds);
+                    dsf[sI] = __builtin_bit_cast(bf16x8, packed);
+                    if constexpr (WHOLE)
+#pragma unroll
+                        for (int gq = 0; gq < 2; ++gq)  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
+                            *(u32x2*)(dss + own * ROWB + (((4 * b + 2 * sI + gq) ^ swz<D>(own)) << 4) + 8 * hh) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
+                }
+#pragma unroll
+                for (int sI = 0; sI < 2; ++sI)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const char *x = qb + sI * 16 * ROWB, *y = db + sI * 16 * ROWB;
+                        dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(y + tlo[d], y + thi[d]), pfr[sI], dv[d], 0, 0, 0);
+                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + tlo[d], x + thi[d]), dsf[sI], dk[d], 0, 0, 0);
+                    }
+            }
+        }
+        if (!WHOLE && q0 + PA_TILE < len) {
+            q0 += PA_TILE;
+            continue;
+        }
+        q0 = k0;
+        ++g;
+        if constexpr (!WHOLE) continue;
+        __syncthreads();
+        if (busy) {
+            f32x16 dq[ND];
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
+            const int qlo = wave ? tlo[1] : tlo[0], qhi = wave ? thi[1] : thi[0];
+            for (int b = 0; b <= wave; ++b)
+#pragma unroll
+                for (int sI = 0; sI < 2; ++sI) {
+                    const char *x = dss + b * BLOCKB + sI * 16 * ROWB, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
+                    const bf16x8 f = tr_pair(x + qlo, x + qhi);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(y + tlo[d], y + thi[d]), f, dq[d], 0, 0, 0);
+                }
+            store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, ok);
+        }
+    }
+    if (busy) {
+        store_row<D>(a.dK + row * a.lddk + kvh * D, nullptr, dk, a.scale, hh, ok);
+        store_row<D>(a.dV + row * a.lddv + kvh * D, nullptr, dv, 1.0f, hh, ok);
+    }
+}
+__global__ __launch_bounds__(128, 2) void packed_bwd_short_kernel(const PackedArgs a) {
+    constexpr int BYTES = 5 * PA_TILE * 128 > SHORT_SMEM ? 5 * PA_TILE * 128 : SHORT_SMEM;
+    __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+    const int at = (int)blockIdx.x - a.rest;
+    if (at >= 0) {
+        const int i = at / a.Hkv, start = min(max(a.cu[i], 0), a.rows), len = min(max(a.cu[i + 1], start), a.rows) - start;
+        if (len > 0 && len <= a.skip) key_tile<true>(a, start, len, 0, false, at % a.Hkv, smem);
+        return;
+    }
+    const int u = blockIdx.x, groups = (a.H + a.Hkv + a.per - 1) / a.per, u0 = u % groups * a.per;
+    Tile tl;
+    if (!find_tile<PA_TILE>(a, u / groups, false, tl)) return;
+    for (int j = u0; j < min(u0 + a.per, a.H + a.Hkv); ++j) {
+        if (j > u0) __syncthreads();
+        if (j < a.Hkv) key_tile<false>(a, tl.start, tl.len, tl.tile * PA_TILE, tl.tail, j, smem);
+        else dq_walk<64, 2>(a, tl, j - a.Hkv, smem);
+    }
+}
+
 // dK and dV of the parts, in their order: a thread per 8 channels of a row and gradient
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a, int width) {
     const int end = min(max(a.cu[a.n_seq], 0), a.rows), chunks = width / 8;
@@ -905,6 +1095,9 @@ int parts_of(int n_seq, int rows, int H, int Hkv) {
 }
 size_t delta_bytes(int rows, int H) { return ((size_t)rows * H * 4 + 255) & ~(size_t)255; }
 
+// Workgroups for sequences that are longer than most, of which there may be none: so many at most, each with several heads if need
+// be (prompts of up to 77 rows, 16 heads, backward: 256 of them 54.7 us with 8192, 63.8 with 2048; 4096 of them 1103 / 1020)
+constexpr long long MOST_EMPTY = 4096;
 constexpr long long MOST_GROUPS = (1 << 24) - 1;  // (a launch has less than 2^32 threads)
 
 RowSpan span(const void* p, int ld, int width, int rows) { return {p, 2ll * ld, 2ll * width, rows}; }
@@ -995,10 +1188,19 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     if (qtiles * H > MOST_GROUPS) return CCNET_EUNSUP;
     if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
+    if (waves == 2) {  // most sequences fit 64 rows
+        a.skip = SHORT_ROWS;
+        a.per = (int)((qtiles * (H + Hkv) + MOST_EMPTY - 1) / MOST_EMPTY);
+        const long long rest = qtiles * ((H + Hkv + a.per - 1) / a.per), groups = (long long)n_seq * Hkv + rest;
+        a.rest = (int)rest;
+        if (groups > MOST_GROUPS) return CCNET_EUNSUP;
+        hipLaunchKernelGGL(packed_bwd_short_kernel, dim3((unsigned)groups), dim3(128), 0, st, a);
+        CCNET_LAUNCH_CHECK();
+        return CCNET_OK;
+    }
     const dim3 gq((unsigned)(qtiles * H)), gk((unsigned)(tiles * Hkv * a.parts)), b(64 * waves);
     if (d == 128) hipLaunchKernelGGL((packed_bwd_dq_kernel<128, 4>), gq, b, 0, st, a);
-    else if (waves == 4) hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 4>), gq, b, 0, st, a);
-    else hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 2>), gq, b, 0, st, a);
+    else hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 4>), gq, b, 0, st, a);
     CCNET_LAUNCH_CHECK();
     if (tiles == 0) return CCNET_OK;
     if (d == 128) hipLaunchKernelGGL((packed_bwd_dkv_kernel<128, 4>), gk, dim3(256), 0, st, a);

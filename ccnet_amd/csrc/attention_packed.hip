@@ -875,7 +875,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // in the dK / dV kernel (block pairs (0, 0), (0, 1); (1, 1)); dS, rounded for dK's product, is also left in LDS as rows of keys, from
 // where transposed reads give the B operand of dQ^T = K^T dS^T, the waves owning 32 queries now.
 // Sequences that are longer, a few among many, have the launch's first workgroups, which end at once where there are none: a tile of
-// 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.
+// 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.  That is slower
+// than the kernels above where one sequence holds most of the rows (3000 and 63 of 9, 16 heads: 151 us against 127, with 4 key heads
+// 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741).
+// Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.1 TB/s.
 constexpr int SHORT_ROWS = 64, SHORT_SMEM = 4 * PA_TILE * 128 + 512;  // Q, dO, K, dS; lse, delta
 // dK and dV of 64 keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
 template <bool WHOLE>
@@ -1035,12 +1038,14 @@ __global__ __launch_bounds__(128, 2) void packed_bwd_short_kernel(const PackedAr
         if (len > 0 && len <= a.skip) key_tile<true>(a, start, len, 0, false, at % a.Hkv, smem);
         return;
     }
-    const int u = blockIdx.x, groups = (a.H + a.Hkv + a.per - 1) / a.per, u0 = u % groups * a.per;
+    const int u = blockIdx.x, groups = (a.H + a.Hkv + a.per - 1) / a.per, u0 = u % groups;
     Tile tl;
     if (!find_tile<PA_TILE>(a, u / groups, false, tl)) return;
-    for (int j = u0; j < min(u0 + a.per, a.H + a.Hkv); ++j) {
+    for (int j = u0; j < a.H + a.Hkv; j += groups) {
         if (j > u0) __syncthreads();
-        if (j < a.Hkv) key_tile<false>(a, tl.start, tl.len, tl.tile * PA_TILE, tl.tail, j, smem);
+        // (one unit a workgroup: the longest walks come first, dQ's of the last tile and dK's of the first; more: their lengths add up
+        // to the same for every tile)
+        if (j < a.Hkv) key_tile<false>(a, tl.start, tl.len, (a.per == 1 ? tl.ntiles - 1 - tl.tile : tl.tile) * PA_TILE, tl.tail, j, smem);
         else dq_walk<64, 2>(a, tl, j - a.Hkv, smem);
     }
 }

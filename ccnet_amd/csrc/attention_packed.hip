@@ -321,6 +321,17 @@ __device__ __forceinline__ void store_row(__bf16* row, __bf16* low_row, const f3
         }
 }
 
+// what the rounding of f to the bf16 of `hi` took away, rounded itself
+__device__ __forceinline__ u32x4 rounded_off(const float (&f)[8], const u32x4& hi) {
+    float r[8];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        r[2 * w] = f[2 * w] - __uint_as_float(hi[w] << 16);
+        r[2 * w + 1] = f[2 * w + 1] - __uint_as_float(hi[w] & 0xffff0000u);
+    }
+    return pack8(r);
+}
+
 __device__ __forceinline__ float half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -615,14 +626,16 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
                 dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(vb + rread[ks]), dof[ks], dr, 0, 0, 0);
             }
         };
-        // kb: K of this key block; kn, vn: K and V of the next
-        auto step = [&](const char* kb, const char* kn, const char* vn, auto diag_c, auto next_c) {
-            constexpr bool DIAG = decltype(diag_c)::value, NEXT = decltype(next_c)::value;
+        // kb: K of this key block; kn, vn: K and V of the next.  MORE (every other block): what the rounding of dS to bf16 takes away from
+        // the block's first 16 keys goes into a second product.  Without it dQ is 1.5 times as far from the exact one as its own rounding to
+        // bf16 brings it; with it for these keys 1.4 times, as dK is (13.6k rows, 16 / 4 heads: 330 -> 344 us), for half of them 1.3 (353),
+        // for all 1.1 (369).
+        auto step = [&](const char* kb, const char* kn, const char* vn, auto diag_c, auto next_c, auto more_c) {
+            constexpr bool DIAG = decltype(diag_c)::value, NEXT = decltype(next_c)::value, MORE = decltype(more_c)::value;
             f32x16 sn, dpn;
             if constexpr (NEXT) scores(sn, dpn, kn, vn);
-            bf16x8 dsf[2];
-#pragma unroll
-            for (int sI = 0; sI < 2; ++sI) {
+            bf16x8 dsf[2], low;
+            auto terms = [&](int sI) {
                 float ds[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -630,13 +643,27 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
                     ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (FROM_DELTA ? dp[e] : dp[e] + dlt);
                     if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > l31) ds[j] = 0.f;
                 }
-                dsf[sI] = __builtin_bit_cast(bf16x8, pack8(ds));
+                const u32x4 hi = pack8(ds);
+                dsf[sI] = __builtin_bit_cast(bf16x8, hi);
+                if (MORE && sI == 0) low = __builtin_bit_cast(bf16x8, rounded_off(ds, hi));
+            };
+            auto products = [&](int sI) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const bf16x8 kt = tr_pair(kb + sI * 16 * ROWB + klo[d], kb + sI * 16 * ROWB + khi[d]);
+                    dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsf[sI], dq[d], 0, 0, 0);
+                    if (MORE && sI == 0) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, low, dq[d], 0, 0, 0);
+                }
+            };
+            terms(0);
+            if constexpr (D == 128) {  // (the other order spills)
+                products(0);
+                terms(1);
+            } else {
+                terms(1);
+                products(0);
             }
-#pragma unroll
-            for (int sI = 0; sI < 2; ++sI)
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-                    dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(kb + sI * 16 * ROWB + klo[d], kb + sI * 16 * ROWB + khi[d]), dsf[sI], dq[d], 0, 0, 0);
+            products(1);
             if constexpr (NEXT) { s = sn; dp = dpn; }
         };
         const int ntiles = (min((tl.tile + 1) * BM, tl.len) + PA_TILE - 1) / PA_TILE;
@@ -661,19 +688,19 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
         if (q0 < tl.len) scores(s, dp, smem + 2 * TILEB, smem);
         for (; t < walk; ++t) {
             const char* kb = smem + (2 + kslot) * TILEB;
-            step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{});
+            step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{}, std::true_type{});
             fence();
-            step(kb + BLOCKB, smem + (2 + next_slot()) * TILEB, smem + ((t + 1) & 1) * TILEB, std::false_type{}, std::true_type{});
+            step(kb + BLOCKB, smem + (2 + next_slot()) * TILEB, smem + ((t + 1) & 1) * TILEB, std::false_type{}, std::true_type{}, std::false_type{});
             kslot = next_slot();
         }
         if (q0 < tl.len) {
             const char* kb = smem + (2 + kslot) * TILEB;
             if (jd & 1) {
-                step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{});
+                step(kb, kb + BLOCKB, smem + (t & 1) * TILEB + BLOCKB, std::false_type{}, std::true_type{}, std::true_type{});
                 fence();
-                step(kb + BLOCKB, nullptr, nullptr, std::true_type{}, std::false_type{});
+                step(kb + BLOCKB, nullptr, nullptr, std::true_type{}, std::false_type{}, std::false_type{});
             } else {
-                step(kb, nullptr, nullptr, std::true_type{}, std::false_type{});
+                step(kb, nullptr, nullptr, std::true_type{}, std::false_type{}, std::true_type{});
                 fence();
             }
             kslot = next_slot();
@@ -879,13 +906,14 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // than the kernels above where one sequence holds most of the rows (3000 and 63 of 9, 16 heads: 151 us against 127, with 4 key heads
 // 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741).
 // Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.1 TB/s.
-constexpr int SHORT_ROWS = 64, SHORT_SMEM = 4 * PA_TILE * 128 + 512;  // Q, dO, K, dS; lse, delta
+constexpr int SHORT_ROWS = 64, SHORT_SMEM = 4 * PA_TILE * 128 + 16 * 128 + 512;  // Q, dO, K, dS; its low parts; lse, delta
 // dK and dV of 64 keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
 template <bool WHOLE>
 __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len, int k0, bool tail, int kvh, char* smem) {
     constexpr int D = 64, NK = 4, ND = 2, ROWB = 128, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
     char *qs = smem, *dos = smem + TILEB, *ks_ = smem + 2 * TILEB, *dss = smem + 3 * TILEB;
-    float* stat = (float*)(smem + 4 * TILEB);
+    char* lows = smem + 4 * TILEB;  // what the rounding of dS took away from keys 0 .. 15
+    float* stat = (float*)(smem + 4 * TILEB + 16 * ROWB);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5, G = a.H / a.Hkv, own = wave * 32 + l31;
     const bool ok = k0 + own < len, busy = k0 + wave * 32 < len;
@@ -983,10 +1011,15 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
                     const u32x4 packed = pack8(ds);
                     dsf[sI] = __builtin_bit_cast(bf16x8, packed);
-                    if constexpr (WHOLE)
+                    if constexpr (WHOLE) {  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
+                        const u32x4 low = rounded_off(ds, packed);
 #pragma unroll
-                        for (int gq = 0; gq < 2; ++gq)  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
-                            *(u32x2*)(dss + own * ROWB + (((4 * b + 2 * sI + gq) ^ swz<D>(own)) << 4) + 8 * hh) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
+                        for (int gq = 0; gq < 2; ++gq) {
+                            const int c = (((4 * b + 2 * sI + gq) ^ swz<D>(own)) << 4) + 8 * hh;
+                            *(u32x2*)(dss + own * ROWB + c) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
+                            if (own < 16) *(u32x2*)(lows + own * ROWB + c) = u32x2{low[2 * gq], low[2 * gq + 1]};
+                        }
+                    }
                 }
 #pragma unroll
                 for (int sI = 0; sI < 2; ++sI)
@@ -1019,7 +1052,11 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     const char *x = dss + b * BLOCKB + sI * 16 * ROWB, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
                     const bf16x8 f = tr_pair(x + qlo, x + qhi);
 #pragma unroll
-                    for (int d = 0; d < ND; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(y + tlo[d], y + thi[d]), f, dq[d], 0, 0, 0);
+                    for (int d = 0; d < ND; ++d) {
+                        const bf16x8 kt = tr_pair(y + tlo[d], y + thi[d]);
+                        dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, f, dq[d], 0, 0, 0);
+                        if (b == 0 && sI == 0) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, tr_pair(lows + qlo, lows + qhi), dq[d], 0, 0, 0);
+                    }
                 }
             store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, ok);
         }

@@ -596,17 +596,20 @@ _F32_BF16 = {torch.float32: 0, BF16: 1}
 
 def _raw_stream() -> int:
     """The current device's current stream, without the 2.5 us that building a torch.cuda.Stream object costs."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _elsewhere(*ts: Optional[torch.Tensor]) -> bool:
     """Whether the operands live on another device than the current one (the op then runs with that device made current); raises
     where they are on the CPU or on different devices."""
-    dev = {t.get_device() for t in ts if t is not None}
-    if len(dev) != 1 or -1 in dev:
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _need_cuda(*ts)
+            raise _l.CcnetError(f"operands are on different devices: {sorted({t.get_device() for t in ts if t is not None})}")
+    if dev < 0:
         _need_cuda(*ts)
-        raise _l.CcnetError(f"operands are on different devices: {sorted(dev)}")
-    return dev.pop() != torch.cuda.current_device()
+    return dev != torch.cuda.current_device()
 
 
 def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
@@ -626,7 +629,7 @@ def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
 def _ids(ids: torch.Tensor) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise _l.CcnetError(f"ids must be int64 or int32, got {ids.dtype}")
-    return ids.reshape(-1).contiguous()
+    return (ids if ids.dim() == 1 else ids.reshape(-1)).contiguous()
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype: torch.dtype = BF16,
@@ -644,7 +647,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, dtype:
     flat = _ids(ids)
     T, Cc = flat.numel(), table.shape[1]
     if out is None:
-        out = torch.empty((T, Cc), dtype=dtype, device=table.device)
+        out = table.new_empty((T, Cc), dtype=dtype)
     ldo = _rows_ld(out, "out", T, Cc, _F32_BF16)
     _l.check(lib.ccnet_embedding(flat.data_ptr(), flat.element_size(), T, table.shape[0], table.data_ptr(), _F32_BF16[table.dtype],
                                  ldt, Cc, scale, out.data_ptr(), _F32_BF16[out.dtype], ldo, _raw_stream()), "embedding")
@@ -814,8 +817,8 @@ def grad_norm(grads) -> torch.Tensor:
         with torch.cuda.device(grads[0].device):
             return grad_norm(grads)
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
-    ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = grads[0].new_empty(wsb // 8, dtype=torch.float64)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     _l.check(lib.ccnet_grad_norm(ptrs, numel, n, dt, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()), "grad_norm")
     return norm
 
@@ -833,8 +836,8 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
         with torch.cuda.device(grads[0].device):
             return clip_grad_norm(grads, max_norm, None if out is None else outs)
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
-    ws = torch.empty(wsb // 8, dtype=torch.float64, device=grads[0].device)
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    ws = grads[0].new_empty(wsb // 8, dtype=torch.float64)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     _check_clip(lib.ccnet_clip_grad_norm(ptrs, optrs, numel, n, dt, max_norm, ws.data_ptr(), wsb, norm.data_ptr(), _raw_stream()),
                 "clip_grad_norm")
     return norm

@@ -348,6 +348,9 @@ __device__ __forceinline__ float half_sum(float v) {
 // pipe, which need about 512 cycles a step each at d = 128, run at once.  Half way through a tile's two steps lies the fence at
 // which the next tile has landed (its keys are needed by the second step) and the tile after it is sent for: K in a ring of
 // two, V, which is needed a step longer, in a ring of three.
+// Bound by both pipes' issue at d = 128 (4 sequences of 2811 to 8192 rows, 32 / 8 heads: 856 us = 1022 TFLOP/s, a square product of
+// 16384 reaches 1364), by the exponentials at d = 64 (5 of 1528 to 4096 rows, 16 / 4 heads: 107 us = 800 TFLOP/s, where every product
+// has half the work an exponential), by latency for prompts (77 rows, 16 heads: 5.8 us; 32 prompts 6.6 us).
 template <int D, int QB, int W>
 __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs a) {
     constexpr int BM = 32 * W * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
@@ -562,7 +565,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
 // ------------------------------------------------------------------ backward: dQ (and delta)
 // The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
-// and left for the dK / dV kernel.
+// and left for the dK / dV kernel.  7 products' worth of MFMA for 6 at d = 64; 13.6k rows, 16 / 4 heads: 151 us = 850 TFLOP/s counted as
+// three products a pair of blocks.
 template <int D, int W>
 __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int h, char* smem) {
     constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
@@ -615,6 +619,7 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
         for (int ks = 0; ks < NK; ++ks) rread[ks] = l31 * ROWB + (((2 * ks + hh) ^ swz<D>(l31)) << 4);
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, klo[d], khi[d]);
+        const int last = q == 0 ? -1 : l31;  // the last key of the diagonal block whose dS counts: query 0 sees one key, P = 1, dS = 0
         constexpr bool FROM_DELTA = D == 64;  // (dP begins at -delta, to the bit as in the other kernels; at d 128 that spills)
         f32x16 s, dp;
         auto scores = [&](f32x16& sr, f32x16& dr, const char* kb, const char* vb) {
@@ -628,8 +633,8 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
         };
         // kb: K of this key block; kn, vn: K and V of the next.  MORE (every other block): what the rounding of dS to bf16 takes away from
         // the block's first 16 keys goes into a second product.  Without it dQ is 1.5 times as far from the exact one as its own rounding to
-        // bf16 brings it; with it for these keys 1.4 times, as dK is (13.6k rows, 16 / 4 heads: 330 -> 344 us), for half of them 1.3 (353),
-        // for all 1.1 (369).
+        // bf16 brings it; with it for these keys 1.4 times, or 1.1 for prompts (backward of 13.6k rows, 16 / 4 heads: 330 -> 344 us), for
+        // half of them 1.3 (353), for all 1.1 (369).
         auto step = [&](const char* kb, const char* kn, const char* vn, auto diag_c, auto next_c, auto more_c) {
             constexpr bool DIAG = decltype(diag_c)::value, NEXT = decltype(next_c)::value, MORE = decltype(more_c)::value;
             f32x16 sn, dpn;
@@ -641,7 +646,7 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
                 for (int j = 0; j < 8; ++j) {
                     const int e = 8 * sI + j;
                     ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (FROM_DELTA ? dp[e] : dp[e] + dlt);
-                    if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > l31) ds[j] = 0.f;
+                    if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > last) ds[j] = 0.f;
                 }
                 const u32x4 hi = pack8(ds);
                 dsf[sI] = __builtin_bit_cast(bf16x8, hi);
@@ -794,6 +799,8 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
                 dr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fd[ks], vf[ks], dr, 0, 0, 0);
             }
         };
+        // MORE (every other block): as in dQ, for the block's first 16 queries (dK 1.45 to 1.7 -> 1.1 to 1.4 times its own rounding;
+        // backward of 13.6k rows 350 -> 360 us).
         // qb: Q of this query block (dO a tile behind it), stat: its lse, rel: its index counted from the wave's diagonal, statn: of
         // the next block, qnn: Q of the block after that
         auto step = [&](const char* qb, const float* stat, int rel, const float* statn, const char* qnn, auto fence_c) {
@@ -801,10 +808,12 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (rel * 32 + (e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
+                if (rel == 0 && k0 + hh == 0) dp[0] = 0.f;                                // (query 0 sees one key: P = 1, dS = 0)
             }
             f32x16 sn, dpn;
             scores(sn, dpn, statn);
-            bf16x8 pfr[2], dsf[2];
+            constexpr bool MORE = decltype(fence_c)::value;
+            bf16x8 pfr[2], dsf[2], low;
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI) {
                 float p[8], ds[8];
@@ -820,7 +829,9 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
                     }
                 }
                 pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
-                dsf[sI] = __builtin_bit_cast(bf16x8, pack8(ds));
+                const u32x4 hi = pack8(ds);
+                dsf[sI] = __builtin_bit_cast(bf16x8, hi);
+                if (MORE && sI == 0) low = __builtin_bit_cast(bf16x8, rounded_off(ds, hi));
             }
 #pragma unroll
             for (int sI = 0; sI < 2; ++sI)
@@ -844,6 +855,7 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
                 for (int d = 0; d < ND; ++d) {
                     dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(td[sI][d], pfr[sI], dv[d], 0, 0, 0);
                     dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[sI][d], dsf[sI], dk[d], 0, 0, 0);
+                    if (MORE && sI == 0) dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[sI][d], low, dk[d], 0, 0, 0);
                 }
             s = sn;
             dp = dpn;
@@ -993,8 +1005,9 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if ((e & 3) + 8 * (e >> 2) + 4 * hh < l31) s[e] = -INFINITY;  // P = 0, dS = 0
+                    if (q0 + b + hh == 0) dp[0] = 0.f;                                // (query 0 sees one key: P = 1, dS = 0)
                 }
-                bf16x8 pfr[2], dsf[2];
+                bf16x8 pfr[2], dsf[2], low0;
 #pragma unroll
                 for (int sI = 0; sI < 2; ++sI) {
                     float p[8], ds[8];
@@ -1011,8 +1024,9 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     pfr[sI] = __builtin_bit_cast(bf16x8, pack8(p));
                     const u32x4 packed = pack8(ds);
                     dsf[sI] = __builtin_bit_cast(bf16x8, packed);
+                    const u32x4 low = rounded_off(ds, packed);
+                    if (sI == 0) low0 = __builtin_bit_cast(bf16x8, low);
                     if constexpr (WHOLE) {  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
-                        const u32x4 low = rounded_off(ds, packed);
 #pragma unroll
                         for (int gq = 0; gq < 2; ++gq) {
                             const int c = (((4 * b + 2 * sI + gq) ^ swz<D>(own)) << 4) + 8 * hh;
@@ -1027,7 +1041,9 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     for (int d = 0; d < ND; ++d) {
                         const char *x = qb + sI * 16 * ROWB, *y = db + sI * 16 * ROWB;
                         dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(y + tlo[d], y + thi[d]), pfr[sI], dv[d], 0, 0, 0);
-                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(x + tlo[d], x + thi[d]), dsf[sI], dk[d], 0, 0, 0);
+                        const bf16x8 qt = tr_pair(x + tlo[d], x + thi[d]);
+                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, dsf[sI], dk[d], 0, 0, 0);
+                        if (b == 0 && sI == 0) dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, low0, dk[d], 0, 0, 0);
                     }
             }
         }

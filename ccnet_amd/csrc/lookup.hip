@@ -79,7 +79,10 @@ __device__ __forceinline__ long long id_at(const void* ids, int wide, long long 
     return wide ? ((const long long*)ids)[t] : (long long)((const int*)ids)[t];
 }
 
-// ------------------------------------------------------------------ lookup: a wave per row and 512 columns
+// ------------------------------------------------------------------ lookup
+// A wave per row, 512 columns at a time, 16 bytes a lane.  Bound by memory: every row written once, the rows of a table read from the
+// caches where tokens repeat (50021 tokens of 49408, bf16 1024 -> bf16: 23.8 us, 4.3 TB/s written; 77 tokens: 2.6 us, of which the
+// launch and two dependent loads are all).
 template <typename TW, typename TO, bool VEC>
 __global__ __launch_bounds__(256) void lookup_kernel(const void* ids, int wide, int T, int vocab, const TW* table, long long ldt, int C,
                                                      float scale, TO* out, long long ldo) {
@@ -124,7 +127,9 @@ __device__ __forceinline__ bool fill_part(const Fill& f) {
     return true;
 }
 
-// Up to RANK_MOST positions: every position counts the ones in front of it.  key << 13 | t orders them all, in 32 bits
+// Up to RANK_MOST positions: one launch, every position counts the ones in front of it (T^2 comparisons of 4 bytes from LDS; with the
+// zeros of half a table of 49408 x 1024 beside it, 2464 positions take 19.1 us, which is the 101 MB at 5.3 TB/s; 5003 positions alone
+// 6.8 us, where the radix sort below takes four launches).  key << 13 | t orders them all, in 32 bits
 // (vocab < 2^18).  A workgroup ranks 2^shift = 16 or 32 positions: 64 / 2^shift lanes of each of its 16 waves hold the same
 // position and compare it with a part of all.
 constexpr int RANK_MOST = 8192, RANK_VOCAB = 1 << 18;
@@ -163,7 +168,8 @@ __global__ __launch_bounds__(1024) void rank_sort_kernel(const void* ids, int wi
 // More positions: least significant digits first, 8 bits a pass; a workgroup takes `per` positions, in blocks of RS_BLOCK.  Every
 // workgroup adds the counts hist[workgroup][digit] of the ones in front of it itself, a launch less than a scan of its own; as that
 // work grows with the square of their number, there are at most RS_MOST (16.8M positions x 320: 8550 us without a limit, 3140 with
-// 256, 3090 with 1024, 3075 with 512).
+// 256, 3090 with 1024, 3075 with 512).  131071 positions and two fifths of the table's zeros each: counting 7.5 us, moving 11.7 us a
+// pass, the zeros' write rate or nearly so.
 constexpr int RS_BLOCK = 2048, RS_MOST = 512, RS_THREADS = 512, RS_ROUNDS = RS_BLOCK / RS_THREADS;
 struct SortArgs {
     const void* ids; int wide; int T, vocab; long long padding;
@@ -357,6 +363,9 @@ __device__ __forceinline__ void add_chunks(const float* p, int C, int first, int
     }
 }
 
+// Sums of 64 and of 512 sorted rows, only where they lie inside one run (the padding token of a batch of prompts): without them a
+// run of thousands of rows would be one wave's chain.  Other workgroups of the launch write the last of the table's zeros (2464 rows
+// of 1024 and half a table's zeros 21.8 us; 131071 rows and a fifth of the zeros 30.7 us).
 // 8 waves, workgroup (b, column span): wave w sums chunk 8 b + w if it lies inside one run, together they sum chunk b of 512
 template <typename T, bool VEC, bool PAST>
 __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
@@ -393,9 +402,11 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     }
 }
 
+// The rows of the table that occur, each written once.  Bound by the gather of dy's rows outside whole chunks: 131071 rows of 1024 bf16
+// 62.9 us (with the chunks' sums 94 us for 268 MB read, the occurring rows and the last zeros written); 2464 rows 7.1 us.
 // grid (T / 4 per_wave rounded up, C / 512 rounded up), 4 waves: a wave takes the runs that begin in its per_wave <= 32 sorted
-// positions.  Runs of up to 32 positions it streams one after the other, eight positions at a time, across their borders.  A longer one (at most
-// one begins there, the last) is summed by the four waves together, from the chunk sums where they cover it.
+// positions.  Runs of up to 32 positions it streams one after the other, eight positions at a time, across their borders.  A longer
+// one (at most one begins there, the last) is summed by the four waves together, from the chunk sums where they cover it.
 constexpr int RUN_SHORT = 32;
 template <typename T, bool VEC, bool PAST>
 __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {

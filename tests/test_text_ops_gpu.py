@@ -427,6 +427,22 @@ def test_packed_attention_scores_of_any_size(cuda, d):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [(1, 1, 5, 1, 70), (1, 300, 1, 700)], ids=lambda x: f"{len(x)}x{max(x)}")
+def test_a_query_that_sees_one_key_has_no_gradient(cuda, lens, d):
+    """softmax of one score is 1 whatever the score is: dq of every sequence's first row and dk of a sequence of one row are zero, to
+    the bit, and its dv is the sum of its group's do."""
+    H, Hkv = 6, 3
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=12)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.7)
+    first = [0] + list(torch.tensor(lens).cumsum(0))
+    for n, at in zip(lens, map(int, first)):
+        assert (got["dq"][at] == 0).all()
+        if n == 1:
+            assert (got["dk"][at] == 0).all()
+            assert torch.equal(got["dv"][at], do[at].float().reshape(Hkv, 2, d).sum(1).reshape(-1).to(BF16))
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_packed_attention_gradients_against_differences(cuda, d):
     lens, H, Hkv, scale = (45, 70), 2, 1, 0.15
     q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=11)

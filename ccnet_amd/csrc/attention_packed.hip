@@ -565,8 +565,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
 // ------------------------------------------------------------------ backward: dQ (and delta)
 // The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
-// and left for the dK / dV kernel.  7 products' worth of MFMA for 6 at d = 64; 13.6k rows, 16 / 4 heads: 151 us = 850 TFLOP/s counted as
-// three products a pair of blocks.
+// and left for the dK / dV kernel.  Bound by matrix and vector issue side by side: 13.6k rows, 16 / 4 heads,
+// d 64: 151 us = 850 TFLOP/s of its three products (a twelfth more are for dS's low parts).
 template <int D, int W>
 __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int h, char* smem) {
     constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
@@ -728,6 +728,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedAr
 // group (or of its part of it) in turn, so the group's sum is taken in the accumulators, in a fixed order.  As above the scores
 // of the next query block are computed beside the exponentials of this one; Q and dO are both needed a step longer (rings of
 // three).  Query blocks in front of a wave's own keys (in the first two tiles of a head) are masked whole.
+// Bound like dQ, with one workgroup a CU less (256 registers, 50 KB): the same 13.6k rows 198 us = 860 TFLOP/s of its four products.
 template <int D>
 constexpr int dkv_stage() { return 2 * PA_TILE * 2 * D + 512; }  // Q, dO, lse and delta of 64 queries
 template <int D, int W>
@@ -1103,7 +1104,8 @@ __global__ __launch_bounds__(128, 2) void packed_bwd_short_kernel(const PackedAr
     }
 }
 
-// dK and dV of the parts, in their order: a thread per 8 channels of a row and gradient
+// dK and dV of the parts, in their order: a thread per 8 channels of a row and gradient.  Bound by memory: 2 parts of 13.6k rows x 256,
+// 56 MB read and 14 written, 12.5 us = 5.6 TB/s.
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs a, int width) {
     const int end = min(max(a.cu[a.n_seq], 0), a.rows), chunks = width / 8;
     const long long plane = (long long)a.rows * width, n = 2ll * a.rows * chunks;

@@ -612,6 +612,12 @@ def _elsewhere(*ts: Optional[torch.Tensor]) -> bool:
     return dev != torch.cuda.current_device()
 
 
+def _all_elsewhere(ts) -> bool:
+    """`_elsewhere` of a list of tensors, in half the time."""
+    dev = set(map(torch.Tensor.get_device, ts))
+    return _elsewhere(*ts) if len(dev) != 1 or -1 in dev else dev.pop() != torch.cuda.current_device()
+
+
 def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
     """Row stride of a 2-D operand [rows, width] whose rows are contiguous; raises on anything else."""
     if t.shape != (rows, width) or t.dtype not in dtypes:
@@ -813,7 +819,7 @@ def grad_norm(grads) -> torch.Tensor:
     an fp32 scalar on the GPU."""
     lib = _l.load()
     grads, ptrs, numel, n, dt, _ = _grad_list(grads, "grad_norm")
-    if _elsewhere(*grads):
+    if _all_elsewhere(grads):
         with torch.cuda.device(grads[0].device):
             return grad_norm(grads)
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
@@ -832,7 +838,7 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     if not max_norm >= 0:
         raise _l.CcnetError(f"clip_grad_norm: max_norm {max_norm}")
     optrs, outs = _clip_outputs(grads, ptrs, sizes, out, "clip_grad_norm")
-    if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
+    if _all_elsewhere(grads if outs is grads else grads + outs):
         with torch.cuda.device(grads[0].device):
             return clip_grad_norm(grads, max_norm, None if out is None else outs)
     wsb = lib.ccnet_grad_norm_workspace_bytes(ptrs, numel, n, dt)
@@ -850,7 +856,7 @@ def clip_grad_value(grads, limit: float, out=None) -> None:
     if not limit >= 0:
         raise _l.CcnetError(f"clip_grad_value: limit {limit}")
     optrs, outs = _clip_outputs(grads, ptrs, sizes, out, "clip_grad_value")
-    if _elsewhere(*grads) if outs is grads else _elsewhere(*grads, *outs):
+    if _all_elsewhere(grads if outs is grads else grads + outs):
         with torch.cuda.device(grads[0].device):
             return clip_grad_value(grads, limit, None if out is None else outs)
     _check_clip(lib.ccnet_clip_grad_value(ptrs, optrs, numel, n, dt, limit, _raw_stream()), "clip_grad_value")

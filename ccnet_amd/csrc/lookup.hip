@@ -17,61 +17,115 @@ namespace {
 
 typedef unsigned short bf16_t;
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(bf16_t v) { return bf16_bits_to_f32(v); }
 __device__ __forceinline__ void from_f32(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(bf16_t& d, float v) { d = f32_to_bf16_bits(v); }
 
-// Eight columns of a 512-column span a lane: VEC 8 neighbours (16-byte accesses), else every 64th.
-template <bool VEC>
-__device__ __forceinline__ int col_of(int lane, int j) { return VEC ? lane * 8 + j : lane + 64 * j; }
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* row, int lane, int cols, float* f) {
-    if constexpr (VEC) {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        if (lane * 8 < cols) {
-            a = *(const f32x4*)(row + lane * 8);
-            b = *(const f32x4*)(row + lane * 8 + 4);
+// Eight columns of a 512-column span a lane.  VECTOR: neighbours, rows 16-byte aligned and whole vectors long.  LOOSE: neighbours by
+// accesses of the same width at the elements' alignment, the row's last columns one by one (50021 x 1023 bf16: lookup 49 -> 34.5 us,
+// gradient 137 -> 100).  SPREAD, where all is fp32: every 64th column (78 us and 112, LOOSE 88 and 131).
+enum Cols { VECTOR, LOOSE, SPREAD };
+template <typename T, int L> struct Words;
+template <> struct Words<float, VECTOR> { typedef f32x4 V; };
+template <> struct Words<float, LOOSE> { typedef f32x4 __attribute__((aligned(4))) V; };
+template <> struct Words<bf16_t, VECTOR> { typedef u32x4 V; };
+template <> struct Words<bf16_t, LOOSE> { typedef u32x4 __attribute__((aligned(2))) V; };
+
+// Eight columns as they lie in memory, so that many rows in flight cost no more registers than their bytes.  PAST: past the
+// caches, for gradients that are larger than them (131k x 1024 bf16: 147 -> 132 us; 2464 x 1024, which stay in them: 50 -> 57).
+template <typename T, int L, bool PAST = false> struct Raw;
+template <int L, bool PAST> struct Raw<float, L, PAST> {
+    static constexpr int DEEP = 8;
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* row, int lane, int cols) {
+        a = b = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (L == SPREAD) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (lane + 64 * j < cols) a[j] = row[lane + 64 * j];
+                if (lane + 64 * (4 + j) < cols) b[j] = row[lane + 64 * (4 + j)];
+            }
+        } else {
+            typedef typename Words<float, L>::V V;
+            const int left = cols - lane * 8;
+            const float* p = row + lane * 8;
+            if (left >= (L == VECTOR ? 1 : 8)) {
+                if constexpr (PAST) {
+                    a = __builtin_nontemporal_load((const V*)p);
+                    b = __builtin_nontemporal_load((const V*)(p + 4));
+                } else {
+                    a = *(const V*)p;
+                    b = *(const V*)(p + 4);
+                }
+            } else if (L == LOOSE && left > 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j < left) a[j] = p[j];
+                    if (4 + j < left) b[j] = p[4 + j];
+                }
+            }
         }
+    }
+    __device__ __forceinline__ void get(float* f) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e) { f[e] = a[e]; f[4 + e] = b[e]; }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = lane + 64 * j < cols ? row[lane + 64 * j] : 0.f;
     }
-}
-template <bool VEC>
-__device__ __forceinline__ void load8(const bf16_t* row, int lane, int cols, float* f) {
-    if constexpr (VEC) {
-        u32x4 a = {0u, 0u, 0u, 0u};
-        if (lane * 8 < cols) a = *(const u32x4*)(row + lane * 8);
-        unpack8(a, f);
-    } else {
+};
+template <int L, bool PAST> struct Raw<bf16_t, L, PAST> {
+    static constexpr int DEEP = 16;
+    u32x4 a;
+    __device__ __forceinline__ void load(const bf16_t* row, int lane, int cols) {
+        typedef typename Words<bf16_t, L>::V V;
+        const int left = cols - lane * 8;
+        const bf16_t* p = row + lane * 8;
+        a = u32x4{0u, 0u, 0u, 0u};
+        if (left >= (L == VECTOR ? 1 : 8)) {
+            if constexpr (PAST) a = __builtin_nontemporal_load((const V*)p);
+            else a = *(const V*)p;
+        } else if (L == LOOSE && left > 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = lane + 64 * j < cols ? bf16_bits_to_f32(row[lane + 64 * j]) : 0.f;
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void store8(float* row, int lane, int cols, const float* f) {
-    if constexpr (VEC) {
-        if (lane * 8 < cols) {
-            *(f32x4*)(row + lane * 8) = f32x4{f[0], f[1], f[2], f[3]};
-            *(f32x4*)(row + lane * 8 + 4) = f32x4{f[4], f[5], f[6], f[7]};
+            for (int w = 0; w < 4; ++w) {
+                if (2 * w < left) a[w] = p[2 * w];
+                if (2 * w + 1 < left) a[w] |= (unsigned)p[2 * w + 1] << 16;
+            }
         }
-    } else {
+    }
+    __device__ __forceinline__ void get(float* f) const { unpack8(a, f); }
+};
+template <typename X>
+__device__ __forceinline__ void add_raw(const X& x, float* acc) {
+    float f[8];
+    x.get(f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+}
+template <int L, typename T>
+__device__ __forceinline__ void load8(const T* row, int lane, int cols, float* f) {
+    Raw<T, L> x;
+    x.load(row, lane, cols);
+    x.get(f);
+}
+template <int L, typename T>
+__device__ __forceinline__ void store8(T* row, int lane, int cols, const float* f) {
+    if constexpr (L == SPREAD) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (lane + 64 * j < cols) row[lane + 64 * j] = f[j];
-    }
-}
-template <bool VEC>
-__device__ __forceinline__ void store8(bf16_t* row, int lane, int cols, const float* f) {
-    if constexpr (VEC) {
-        if (lane * 8 < cols) *(u32x4*)(row + lane * 8) = pack8(f);
     } else {
+        typedef typename Words<T, L>::V V;
+        const int left = cols - lane * 8;
+        T* p = row + lane * 8;
+        if (left >= (L == VECTOR ? 1 : 8)) {
+            if constexpr (sizeof(T) == 4) {
+                *(V*)p = f32x4{f[0], f[1], f[2], f[3]};
+                *(V*)(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
+            } else {
+                *(V*)p = pack8(f);
+            }
+        } else if (L == LOOSE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane + 64 * j < cols) row[lane + 64 * j] = f32_to_bf16_bits(f[j]);
+            for (int j = 0; j < 7; ++j)
+                if (j < left) from_f32(p[j], f[j]);
+        }
     }
 }
 
@@ -83,7 +137,7 @@ __device__ __forceinline__ long long id_at(const void* ids, int wide, long long 
 // A wave per row, 512 columns at a time, 16 bytes a lane.  Bound by memory: every row written once, the rows of a table read from the
 // caches where tokens repeat (50021 tokens of 49408, bf16 1024 -> bf16: 23.8 us, 4.3 TB/s written; 77 tokens: 2.6 us, of which the
 // launch and two dependent loads are all).
-template <typename TW, typename TO, bool VEC>
+template <typename TW, typename TO, int L>
 __global__ __launch_bounds__(256) void lookup_kernel(const void* ids, int wide, int T, int vocab, const TW* table, long long ldt, int C,
                                                      float scale, TO* out, long long ldo) {
     const int lane = threadIdx.x & 63;
@@ -93,10 +147,10 @@ __global__ __launch_bounds__(256) void lookup_kernel(const void* ids, int wide, 
     const bool ok = id >= 0 && id < vocab;
     for (int c0 = 0; c0 < C; c0 += 512) {
         float f[8];
-        load8<VEC>(table + (ok ? id : 0) * ldt + c0, lane, ok ? C - c0 : 0, f);
+        load8<L>(table + (ok ? id : 0) * ldt + c0, lane, ok ? C - c0 : 0, f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] *= scale;
-        store8<VEC>(out + t * ldo + c0, lane, C - c0, f);
+        store8<L>(out + t * ldo + c0, lane, C - c0, f);
     }
 }
 
@@ -287,57 +341,10 @@ struct GradArgs {
     Fill fill;
 };
 
-// Eight columns as they lie in memory, so that many rows in flight cost no more registers than their bytes.  PAST: past the
-// caches, for gradients that are larger than them (131k x 1024 bf16: 147 -> 132 us; 2464 x 1024, which stay in them: 50 -> 57).
-template <typename V, bool PAST>
-__device__ __forceinline__ V load16(const void* p) {
-    if constexpr (PAST) return __builtin_nontemporal_load((const V*)p);
-    else return *(const V*)p;
-}
-template <typename T, bool VEC, bool PAST> struct Raw;
-template <bool PAST> struct Raw<float, true, PAST> {
-    static constexpr int DEEP = 8;
-    f32x4 a, b;
-    __device__ __forceinline__ void load(const float* row, int lane, int cols) {
-        a = b = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (lane * 8 < cols) { a = load16<f32x4, PAST>(row + lane * 8); b = load16<f32x4, PAST>(row + lane * 8 + 4); }
-    }
-    __device__ __forceinline__ void add(float* acc) const {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { acc[e] += a[e]; acc[4 + e] += b[e]; }
-    }
-};
-template <bool PAST> struct Raw<bf16_t, true, PAST> {
-    static constexpr int DEEP = 16;
-    u32x4 a;
-    __device__ __forceinline__ void load(const bf16_t* row, int lane, int cols) {
-        a = u32x4{0u, 0u, 0u, 0u};
-        if (lane * 8 < cols) a = load16<u32x4, PAST>(row + lane * 8);
-    }
-    __device__ __forceinline__ void add(float* acc) const {
-        float f[8];
-        unpack8(a, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += f[e];
-    }
-};
-template <typename T, bool PAST> struct Raw<T, false, PAST> {
-    static constexpr int DEEP = 8;
-    T v[8];
-    __device__ __forceinline__ void load(const T* row, int lane, int cols) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = lane + 64 * j < cols ? row[lane + 64 * j] : (T)0;
-    }
-    __device__ __forceinline__ void add(float* acc) const {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += to_f32(v[j]);
-    }
-};
-
 // acc += rows pos[0 .. n) of dy, pos[j] in lane j (n <= 64): DEEP rows in flight, their addresses from registers
-template <typename T, bool VEC, bool PAST>
+template <typename T, int L, bool PAST>
 __device__ __forceinline__ void add_rows(const GradArgs& a, int pos, int n, int c0, int lane, float* acc) {
-    typedef Raw<T, VEC, PAST> X;
+    typedef Raw<T, L, PAST> X;
     const T* dy = (const T*)a.dy + c0;
     for (int j = 0; j < n; j += X::DEEP) {
         X x[X::DEEP];
@@ -346,18 +353,18 @@ __device__ __forceinline__ void add_rows(const GradArgs& a, int pos, int n, int 
             x[u].load(dy + (long long)__builtin_amdgcn_readlane(pos, min(j + u, n - 1)) * a.lddy, lane, j + u < n ? a.C - c0 : 0);
         float part[2][8] = {};  // (rows that are not there add zeros)
 #pragma unroll
-        for (int u = 0; u < X::DEEP; ++u) x[u].add(part[u & 1]);
+        for (int u = 0; u < X::DEEP; ++u) add_raw(x[u], part[u & 1]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += part[0][e] + part[1][e];
     }
 }
 // acc += chunk sums first, first + 4, ... < end
-template <bool VEC>
+template <int L>
 __device__ __forceinline__ void add_chunks(const float* p, int C, int first, int end, int c0, int lane, float* acc) {
     for (int i = first; i < end; i += 16) {
         float f[4][8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) load8<VEC>(p + (long long)min(i + 4 * u, end - 1) * C + c0, lane, i + 4 * u < end ? C - c0 : 0, f[u]);
+        for (int u = 0; u < 4; ++u) load8<L>(p + (long long)min(i + 4 * u, end - 1) * C + c0, lane, i + 4 * u < end ? C - c0 : 0, f[u]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] += (f[0][e] + f[1][e]) + (f[2][e] + f[3][e]);
     }
@@ -367,7 +374,7 @@ __device__ __forceinline__ void add_chunks(const float* p, int C, int first, int
 // run of thousands of rows would be one wave's chain.  Other workgroups of the launch write the last of the table's zeros (2464 rows
 // of 1024 and half a table's zeros 21.8 us; 131071 rows and a fifth of the zeros 30.7 us).
 // 8 waves, workgroup (b, column span): wave w sums chunk 8 b + w if it lies inside one run, together they sum chunk b of 512
-template <typename T, bool VEC, bool PAST>
+template <typename T, int L, bool PAST>
 __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     __shared__ float red[8][512];
     __shared__ int key0[8];
@@ -380,8 +387,8 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
     const bool whole = first >= 0 && first < a.vocab && __all(key == first);
     float acc[8] = {};
     if (whole) {
-        add_rows<T, VEC, PAST>(a, pos, 64, c0, lane, acc);
-        store8<VEC>(a.p64 + (long long)(s / 64) * a.C + c0, lane, a.C - c0, acc);
+        add_rows<T, L, PAST>(a, pos, 64, c0, lane, acc);
+        store8<L>(a.p64 + (long long)(s / 64) * a.C + c0, lane, a.C - c0, acc);
     }
     if (lane == 0) key0[wave] = whole ? first : -1;
     __syncthreads();
@@ -398,7 +405,7 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
             for (int w = 0; w < 8; ++w) v += red[w][j * 64 + lane];
             acc[j] = v;
         }
-        store8<VEC>(a.p512 + (long long)b * a.C + c0, lane, a.C - c0, acc);
+        store8<L>(a.p512 + (long long)b * a.C + c0, lane, a.C - c0, acc);
     }
 }
 
@@ -408,7 +415,7 @@ __global__ __launch_bounds__(512) void chunk_sum_kernel(const GradArgs a) {
 // positions.  Runs of up to 32 positions it streams one after the other, eight positions at a time, across their borders.  A longer
 // one (at most one begins there, the last) is summed by the four waves together, from the chunk sums where they cover it.
 constexpr int RUN_SHORT = 32;
-template <typename T, bool VEC, bool PAST>
+template <typename T, int L, bool PAST>
 __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
     __shared__ float red[4][512];
     __shared__ int long_at[4];
@@ -417,14 +424,14 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
         float* row = a.grad + v * a.ldg + c0;
         if (a.accumulate) {
             float old[8];
-            load8<VEC>(row, lane, cols, old);
+            load8<L>(row, lane, cols, old);
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[j] = fmaf(acc[j], a.scale, old[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[j] *= a.scale;
         }
-        store8<VEC>(row, lane, cols, acc);
+        store8<L>(row, lane, cols, acc);
     };
     // this wave's positions and the 32 behind them: where runs begin (a position behind the last counts as a beginning)
     const int p0 = (blockIdx.x * 4 + wave) * a.per_wave, p = p0 + lane;
@@ -447,7 +454,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
         float acc[8] = {};
         int row = -1;
         for (int j = begin; j < end; j += 8) {
-            Raw<T, VEC, PAST> x[8];
+            Raw<T, L, PAST> x[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 x[u].load(dy + (long long)__builtin_amdgcn_readlane(pos, min(j + u, end - 1)) * a.lddy, lane, j + u < end ? cols : 0);
@@ -461,7 +468,7 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) acc[e] = 0.f;
                     }
-                    x[u].add(acc);
+                    add_raw(x[u], acc);
                 }
         }
         if (row >= 0) put(row, acc);
@@ -488,18 +495,18 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
             const int cnt = (to - from - wave + 3) / 4;
             if (cnt <= 0) return;
             const int at = lane < cnt ? a.perm[from + wave + 4 * lane] : 0;
-            add_rows<T, VEC, PAST>(a, at, cnt, c0, lane, acc);
+            add_rows<T, L, PAST>(a, at, cnt, c0, lane, acc);
         };
         if (ca >= cb) {
             rows(s, e);
         } else {
             rows(s, ca * 64);
             if (da >= db) {
-                add_chunks<VEC>(a.p64, a.C, ca + wave, cb, c0, lane, acc);
+                add_chunks<L>(a.p64, a.C, ca + wave, cb, c0, lane, acc);
             } else {
-                add_chunks<VEC>(a.p64, a.C, ca + wave, da * 8, c0, lane, acc);
-                add_chunks<VEC>(a.p512, a.C, da + wave, db, c0, lane, acc);
-                add_chunks<VEC>(a.p64, a.C, db * 8 + wave, cb, c0, lane, acc);
+                add_chunks<L>(a.p64, a.C, ca + wave, da * 8, c0, lane, acc);
+                add_chunks<L>(a.p512, a.C, da + wave, db, c0, lane, acc);
+                add_chunks<L>(a.p64, a.C, db * 8 + wave, cb, c0, lane, acc);
             }
             rows(cb * 64, e);
         }
@@ -518,25 +525,26 @@ __global__ __launch_bounds__(256) void run_sum_kernel(const GradArgs a) {
 template <typename TW, typename TO>
 void launch_lookup(bool vec, const void* ids, int wide, int T, int vocab, const void* table, int ldt, int C, float scale, void* out, int ldo,
                    hipStream_t st) {
+    constexpr int OTHER = sizeof(TW) == 4 && sizeof(TO) == 4 ? SPREAD : LOOSE;
     constexpr int MOST = 1 << 25;  // (a launch has less than 2^32 threads)
     for (long long t = 0; t < T; t += MOST) {
         const int n = (int)std::min<long long>(T - t, MOST);
         const dim3 grid((unsigned)((n + 3) / 4));
         const void* id = (const char*)ids + t * (wide ? 8 : 4);
         TO* to = (TO*)out + t * ldo;
-        if (vec) hipLaunchKernelGGL((lookup_kernel<TW, TO, true>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
-        else hipLaunchKernelGGL((lookup_kernel<TW, TO, false>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
+        if (vec) hipLaunchKernelGGL((lookup_kernel<TW, TO, VECTOR>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
+        else hipLaunchKernelGGL((lookup_kernel<TW, TO, OTHER>), grid, dim3(256), 0, st, id, wide, n, vocab, (const TW*)table, (long long)ldt, C, scale, to, (long long)ldo);
     }
 }
 
-template <typename T, bool VEC, bool PAST>
+template <typename T, int L, bool PAST>
 int launch_grad(GradArgs a, unsigned fillers, hipStream_t st) {
     // few positions a wave while the grid is small (2464 positions: 41 us against 46 with 16), more where waves abound (131071: 145 / 147)
     a.per_wave = a.T <= 65536 ? 8 : 16;
     const unsigned spans = (unsigned)((a.C + 511) / 512);
-    hipLaunchKernelGGL((chunk_sum_kernel<T, VEC, PAST>), dim3((unsigned)a.fill.workers + fillers), dim3(512), 0, st, a);
+    hipLaunchKernelGGL((chunk_sum_kernel<T, L, PAST>), dim3((unsigned)a.fill.workers + fillers), dim3(512), 0, st, a);
     CCNET_LAUNCH_CHECK();
-    hipLaunchKernelGGL((run_sum_kernel<T, VEC, PAST>), dim3((unsigned)((a.T + 4 * a.per_wave - 1) / (4 * a.per_wave)), spans), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((run_sum_kernel<T, L, PAST>), dim3((unsigned)((a.T + 4 * a.per_wave - 1) / (4 * a.per_wave)), spans), dim3(256), 0, st, a);
     CCNET_LAUNCH_CHECK();
     return CCNET_OK;
 }
@@ -661,7 +669,12 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     g.perm = perm[cur];
     g.fill = fill_next(chunk_workers, passes + 1, passes + 1);
     const bool vec = C % 8 == 0 && aligned16(dy, lddy, ds) && aligned16(grad, ldg, 4);
-    const bool past = vec && (long long)T * C * ds > 192ll << 20;  // (the memory-side cache holds 256 MiB)
-    if (dy_dtype == 0) return past ? launch_grad<float, true, true>(g, fillers, st) : vec ? launch_grad<float, true, false>(g, fillers, st) : launch_grad<float, false, false>(g, fillers, st);
-    return past ? launch_grad<bf16_t, true, true>(g, fillers, st) : vec ? launch_grad<bf16_t, true, false>(g, fillers, st) : launch_grad<bf16_t, false, false>(g, fillers, st);
+    const bool past = (long long)T * C * ds > 192ll << 20;  // (the memory-side cache holds 256 MiB)
+    auto go = [&](auto zero) {
+        typedef decltype(zero) D;
+        constexpr int OTHER = sizeof(D) == 4 ? SPREAD : LOOSE;
+        if (vec) return past ? launch_grad<D, VECTOR, true>(g, fillers, st) : launch_grad<D, VECTOR, false>(g, fillers, st);
+        return past && OTHER == LOOSE ? launch_grad<D, OTHER, OTHER == LOOSE>(g, fillers, st) : launch_grad<D, OTHER, false>(g, fillers, st);
+    };
+    return dy_dtype == 0 ? go(float{}) : go(bf16_t{});
 }

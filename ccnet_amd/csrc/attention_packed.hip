@@ -562,6 +562,19 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
     }
 }
 
+// Where dP begins: at -delta, or at zero with -delta added to the product (the first spills in dQ at d 128); the same to the bit in all
+// of the backward's kernels, so that which of them takes a sequence does not show.
+template <int D>
+constexpr bool FROM_DELTA = D == 64;
+__device__ __forceinline__ void add_delta(f32x16& dp, const float* stat, int hh) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 d4 = *(const f32x4*)(stat + 64 + 8 * g + 4 * hh);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] += d4[j];
+    }
+}
+
 // ------------------------------------------------------------------ backward: dQ (and delta)
 // The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
@@ -620,11 +633,10 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
 #pragma unroll
         for (int d = 0; d < ND; ++d) tr_lane<D>(lane, d, klo[d], khi[d]);
         const int last = q == 0 ? -1 : l31;  // the last key of the diagonal block whose dS counts: query 0 sees one key, P = 1, dS = 0
-        constexpr bool FROM_DELTA = D == 64;  // (dP begins at -delta, to the bit as in the other kernels; at d 128 that spills)
         f32x16 s, dp;
         auto scores = [&](f32x16& sr, f32x16& dr, const char* kb, const char* vb) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = FROM_DELTA ? dlt : 0.f; }
+            for (int e = 0; e < 16; ++e) { sr[e] = 0.f; dr[e] = FROM_DELTA<D> ? dlt : 0.f; }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
                 sr = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(kb + rread[ks]), qf[ks], sr, 0, 0, 0);
@@ -645,7 +657,7 @@ __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int e = 8 * sI + j;
-                    ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (FROM_DELTA ? dp[e] : dp[e] + dlt);
+                    ds[j] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale_log2e, -lse)) * (FROM_DELTA<D> ? dp[e] : dp[e] + dlt);
                     if (DIAG && (e & 3) + 8 * (e >> 2) + 4 * hh > last) ds[j] = 0.f;
                 }
                 const u32x4 hi = pack8(ds);
@@ -792,7 +804,7 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
             for (int g = 0; g < 4; ++g) {
                 const f32x4 d4 = *(const f32x4*)(stat + 64 + 8 * g + 4 * hh);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) { sr[4 * g + j] = 0.f; dr[4 * g + j] = d4[j]; }
+                for (int j = 0; j < 4; ++j) { sr[4 * g + j] = 0.f; dr[4 * g + j] = FROM_DELTA<D> ? d4[j] : 0.f; }
             }
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
@@ -805,6 +817,7 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
         // qb: Q of this query block (dO a tile behind it), stat: its lse, rel: its index counted from the wave's diagonal, statn: of
         // the next block, qnn: Q of the block after that
         auto step = [&](const char* qb, const float* stat, int rel, const float* statn, const char* qnn, auto fence_c) {
+            if constexpr (!FROM_DELTA<D>) add_delta(dp, stat, hh);
             if (rel <= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
@@ -917,16 +930,21 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // Sequences that are longer, a few among many, have the launch's first workgroups, which end at once where there are none: a tile of
 // 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.  That is slower
 // than the kernels above where one sequence holds most of the rows (3000 and 63 of 9, 16 heads: 151 us against 127, with 4 key heads
-// 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741).
+// 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741;
+// d 128 32 / 54, 154 / 230, 2352 / 3854).
 // Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.1 TB/s.
-constexpr int SHORT_ROWS = 64, SHORT_SMEM = 4 * PA_TILE * 128 + 16 * 128 + 512;  // Q, dO, K, dS; its low parts; lse, delta
+constexpr int SHORT_ROWS = 64;
+template <int D>
+constexpr int short_smem() {  // Q, dO, K; dS, its low parts; lse, delta (or what dq_walk needs)
+    return std::max(3 * PA_TILE * 2 * D + (SHORT_ROWS + 16) * 2 * SHORT_ROWS + 512, 5 * PA_TILE * 2 * D);
+}
 // dK and dV of 64 keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
-template <bool WHOLE>
+template <int D, bool WHOLE>
 __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len, int k0, bool tail, int kvh, char* smem) {
-    constexpr int D = 64, NK = 4, ND = 2, ROWB = 128, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
+    constexpr int NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, SROW = 2 * SHORT_ROWS;
     char *qs = smem, *dos = smem + TILEB, *ks_ = smem + 2 * TILEB, *dss = smem + 3 * TILEB;
-    char* lows = smem + 4 * TILEB;  // what the rounding of dS took away from keys 0 .. 15
-    float* stat = (float*)(smem + 4 * TILEB + 16 * ROWB);
+    char* lows = dss + SHORT_ROWS * SROW;  // what the rounding of dS took away from keys 0 .. 15
+    float* stat = (float*)(lows + 16 * SROW);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5, G = a.H / a.Hkv, own = wave * 32 + l31;
     const bool ok = k0 + own < len, busy = k0 + wave * 32 < len;
@@ -987,6 +1005,7 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
         }
         __syncthreads();
         if (busy) {
+#pragma nounroll
             for (int b = WHOLE || q0 == k0 ? wave : 0; b < 2 && b * 32 < left; ++b) {
                 const float* st = stat + 32 * b;
                 const char *qb = qs + b * BLOCKB, *db = dos + b * BLOCKB;
@@ -995,13 +1014,14 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                 for (int gq = 0; gq < 4; ++gq) {
                     const f32x4 d4 = *(const f32x4*)(st + 64 + 8 * gq + 4 * hh);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) { s[4 * gq + j] = 0.f; dp[4 * gq + j] = d4[j]; }
+                    for (int j = 0; j < 4; ++j) { s[4 * gq + j] = 0.f; dp[4 * gq + j] = FROM_DELTA<D> ? d4[j] : 0.f; }
                 }
 #pragma unroll
                 for (int ks = 0; ks < NK; ++ks) {
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], s, 0, 0, 0);
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(db + rread[ks]), vf[ks], dp, 0, 0, 0);
                 }
+                if constexpr (!FROM_DELTA<D>) add_delta(dp, st, hh);
                 if (b == wave && (WHOLE || q0 == k0)) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
@@ -1030,9 +1050,9 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     if constexpr (WHOLE) {  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
 #pragma unroll
                         for (int gq = 0; gq < 2; ++gq) {
-                            const int c = (((4 * b + 2 * sI + gq) ^ swz<D>(own)) << 4) + 8 * hh;
-                            *(u32x2*)(dss + own * ROWB + c) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
-                            if (own < 16) *(u32x2*)(lows + own * ROWB + c) = u32x2{low[2 * gq], low[2 * gq + 1]};
+                            const int c = (((4 * b + 2 * sI + gq) ^ swz<64>(own)) << 4) + 8 * hh;
+                            *(u32x2*)(dss + own * SROW + c) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
+                            if (own < 16) *(u32x2*)(lows + own * SROW + c) = u32x2{low[2 * gq], low[2 * gq + 1]};
                         }
                     }
                 }
@@ -1062,11 +1082,12 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
-            const int qlo = wave ? tlo[1] : tlo[0], qhi = wave ? thi[1] : thi[0];
+            int qlo, qhi;
+            tr_lane<64>(lane, wave, qlo, qhi);
             for (int b = 0; b <= wave; ++b)
 #pragma unroll
                 for (int sI = 0; sI < 2; ++sI) {
-                    const char *x = dss + b * BLOCKB + sI * 16 * ROWB, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
+                    const char *x = dss + (2 * b + sI) * 16 * SROW, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
                     const bf16x8 f = tr_pair(x + qlo, x + qhi);
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
@@ -1083,13 +1104,13 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
         store_row<D>(a.dV + row * a.lddv + kvh * D, nullptr, dv, 1.0f, hh, ok);
     }
 }
-__global__ __launch_bounds__(128, 2) void packed_bwd_short_kernel(const PackedArgs a) {
-    constexpr int BYTES = 5 * PA_TILE * 128 > SHORT_SMEM ? 5 * PA_TILE * 128 : SHORT_SMEM;
-    __shared__ __attribute__((aligned(1024))) char smem[BYTES];
+template <int D>
+__global__ __launch_bounds__(128, D == 64 ? 2 : 1) void packed_bwd_short_kernel(const PackedArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[short_smem<D>()];
     const int at = (int)blockIdx.x - a.rest;
     if (at >= 0) {
         const int i = at / a.Hkv, start = min(max(a.cu[i], 0), a.rows), len = min(max(a.cu[i + 1], start), a.rows) - start;
-        if (len > 0 && len <= a.skip) key_tile<true>(a, start, len, 0, false, at % a.Hkv, smem);
+        if (len > 0 && len <= a.skip) key_tile<D, true>(a, start, len, 0, false, at % a.Hkv, smem);
         return;
     }
     const int u = blockIdx.x, groups = (a.H + a.Hkv + a.per - 1) / a.per, u0 = u % groups;
@@ -1099,8 +1120,8 @@ __global__ __launch_bounds__(128, 2) void packed_bwd_short_kernel(const PackedAr
         if (j > u0) __syncthreads();
         // (one unit a workgroup: the longest walks come first, dQ's of the last tile and dK's of the first; more: their lengths add up
         // to the same for every tile)
-        if (j < a.Hkv) key_tile<false>(a, tl.start, tl.len, (a.per == 1 ? tl.ntiles - 1 - tl.tile : tl.tile) * PA_TILE, tl.tail, j, smem);
-        else dq_walk<64, 2>(a, tl, j - a.Hkv, smem);
+        if (j < a.Hkv) key_tile<D, false>(a, tl.start, tl.len, (a.per == 1 ? tl.ntiles - 1 - tl.tile : tl.tile) * PA_TILE, tl.tail, j, smem);
+        else dq_walk<D, 2>(a, tl, j - a.Hkv, smem);
     }
 }
 
@@ -1135,9 +1156,11 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
     return ((long long)rows + (long long)(n_seq + tail) * (step - 1)) / step;
 }
 
-// Two waves instead of four to a workgroup of the forward and dQ kernels where most sequences fit 64 rows (d 64): twice as many
-// workgroups are resident and fewer waves idle (64 x 40 rows, 16 heads: forward 11.0 -> 8.4 us; from 77 rows on there is nothing in it)
-int waves_of(int rows, int n_seq, int d) { return d == 64 && rows <= 64ll * n_seq ? 2 : 4; }
+// Whether most sequences fit 64 rows, as far as their mean says.
+bool mostly_short(int rows, int n_seq) { return rows <= 64ll * n_seq; }
+// Then the forward has two waves to a workgroup instead of four (d 64; d 128 gains nothing): twice as many workgroups are resident and
+// fewer waves idle (64 x 40 rows, 16 heads: 11.0 -> 8.4 us; from 77 rows on there is nothing in it).
+int waves_of(int rows, int n_seq, int d) { return d == 64 && mostly_short(rows, n_seq) ? 2 : 4; }
 
 // Into how many parts the walk of a key tile over its group's query heads is cut.  One workgroup walks G heads x the queries
 // behind its keys; with few key heads and long sequences the longest of those walks outlasts the rest of the grid.  Parts cost
@@ -1243,24 +1266,25 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     a.delta = (float*)workspace;
     a.part = (float*)((char*)workspace + delta_bytes(rows, H));
     a.parts = parts_of(n_seq, rows, H, Hkv);
-    const int waves = waves_of(rows, n_seq, d);
-    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, 32 * waves, a.zero_tail);
+    const bool prompts = mostly_short(rows, n_seq);
+    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, prompts ? PA_TILE : 128, a.zero_tail);
     if (qtiles * H > MOST_GROUPS) return CCNET_EUNSUP;
     if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
-    if (waves == 2) {  // most sequences fit 64 rows
+    if (prompts) {
         a.skip = SHORT_ROWS;
         a.per = (int)((qtiles * (H + Hkv) + MOST_EMPTY - 1) / MOST_EMPTY);
         const long long rest = qtiles * ((H + Hkv + a.per - 1) / a.per), groups = (long long)n_seq * Hkv + rest;
         a.rest = (int)rest;
         if (groups > MOST_GROUPS) return CCNET_EUNSUP;
-        hipLaunchKernelGGL(packed_bwd_short_kernel, dim3((unsigned)groups), dim3(128), 0, st, a);
+        if (d == 128) hipLaunchKernelGGL(packed_bwd_short_kernel<128>, dim3((unsigned)groups), dim3(128), 0, st, a);
+        else hipLaunchKernelGGL(packed_bwd_short_kernel<64>, dim3((unsigned)groups), dim3(128), 0, st, a);
         CCNET_LAUNCH_CHECK();
         return CCNET_OK;
     }
-    const dim3 gq((unsigned)(qtiles * H)), gk((unsigned)(tiles * Hkv * a.parts)), b(64 * waves);
-    if (d == 128) hipLaunchKernelGGL((packed_bwd_dq_kernel<128, 4>), gq, b, 0, st, a);
-    else hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 4>), gq, b, 0, st, a);
+    const dim3 gq((unsigned)(qtiles * H)), gk((unsigned)(tiles * Hkv * a.parts));
+    if (d == 128) hipLaunchKernelGGL((packed_bwd_dq_kernel<128, 4>), gq, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((packed_bwd_dq_kernel<64, 4>), gq, dim3(256), 0, st, a);
     CCNET_LAUNCH_CHECK();
     if (tiles == 0) return CCNET_OK;
     if (d == 128) hipLaunchKernelGGL((packed_bwd_dkv_kernel<128, 4>), gk, dim3(256), 0, st, a);

@@ -312,19 +312,20 @@ def test_packed_attention_head_layouts(cuda, H, Hkv, d):
         assert (got[name][sum(lens):] == 0).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("H,Hkv", [(64, 64), (63, 21)])
-def test_packed_attention_a_few_long_among_many_short(cuda, H, Hkv):
+def test_packed_attention_a_few_long_among_many_short(cuda, H, Hkv, d):
     """So many heads and sequences that a workgroup takes several heads of the sequences that are longer than most."""
     lens = tuple((i * 29) % 43 for i in range(100)) + (200,) + tuple((i * 29) % 41 for i in range(40)) + (65, 64) + (9,) * (8192 // Hkv // 2)
     lens = lens[:150] if Hkv == 64 else lens
-    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, 64, seed=8, pad=30)
-    got = _run_attention(q, k, v, do, cu, H, Hkv, 64, 0.125)
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=8, pad=30)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.125)
     picks = [1, 5, 42, 100, 120, 141, 142, len(lens) - 1]
     first = [0] + list(torch.tensor(lens).cumsum(0))
     for i in picks:
         r = slice(int(first[i]), int(first[i + 1]))
         part = {n: (got[n][:, r] if n == "lse" else got[n][r]) for n in NAMES}
-        _check_attention(part, _attention_ref(q[r], k[r], v[r], do[r], lens[i:i + 1], H, Hkv, 64, 0.125), f"sequence {i} of {lens[i]}")
+        _check_attention(part, _attention_ref(q[r], k[r], v[r], do[r], lens[i:i + 1], H, Hkv, d, 0.125), f"sequence {i} of {lens[i]}")
     n = sum(lens)
     assert all((got[x][n:] == 0).all() for x in ("o", "dq", "dk", "dv"))
 

@@ -79,7 +79,7 @@ __device__ __forceinline__ void stage_fence() {
 __device__ __forceinline__ unsigned lds_addr(const char* p) {
     return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p;
 }
-// buffer descriptor over `rows` (<= 64) rows of `width` bytes, `ld` bytes apart: an access behind the last row reads zero
+// buffer descriptor over `rows` (<= 96) rows of `width` bytes, `ld` bytes apart: an access behind the last row reads zero
 __device__ __forceinline__ u32x4 row_rsrc(const char* base, int rows, long long ld, int width) {
     const unsigned long long p = (unsigned long long)base;
     return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)p), (unsigned)__builtin_amdgcn_readfirstlane((int)((p >> 32) & 0xffffu)),
@@ -248,10 +248,11 @@ __device__ __forceinline__ void tr_lane(int lane, int d, int& lo, int& hi) {
     hi = (r + 8) * D * 2 + ((chunk ^ swz<D>(r + 8)) << 4) + (tp & 1) * 8;
 }
 
-// the DMA pieces of a 64-row tile that a wave brings: piece p holds 1024 / (2 D) rows, lane l of it chunk position l mod (D / 8)
-template <int D, int W>
+// the DMA pieces of a tile that a wave brings: piece p holds 1024 / (2 D) rows, lane l of it chunk position l mod (D / 8)
+template <int D, int W, int ROWS = PA_TILE>
 struct TileDma {
-    static constexpr int ROWB = 2 * D, CH = D / 8, BYTES = PA_TILE * ROWB, PIECES = BYTES / 1024 / W;
+    static constexpr int ROWB = 2 * D, CH = D / 8, BYTES = ROWS * ROWB, PIECES = BYTES / 1024 / W;
+    static_assert(BYTES % (1024 * W) == 0, "whole pieces a wave");
     unsigned voff[PIECES];
     int wave;
     __device__ __forceinline__ void init(int wave_, int lane, long long ldb) {
@@ -259,7 +260,7 @@ struct TileDma {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int r = (wave * PIECES + i) * (1024 / ROWB) + lane / CH, c = (lane % CH) ^ swz<D>(r);
-            voff[i] = (unsigned)(r * (int)ldb + c * 16);
+            voff[i] = (unsigned)r * (unsigned)ldb + c * 16;
         }
     }
     __device__ __forceinline__ void issue(const u32x4& rsrc, unsigned lds) const {
@@ -566,10 +567,10 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
 // of the backward's kernels, so that which of them takes a sequence does not show.
 template <int D>
 constexpr bool FROM_DELTA = D == 64;
-__device__ __forceinline__ void add_delta(f32x16& dp, const float* stat, int hh) {
+__device__ __forceinline__ void add_delta(f32x16& dp, const float* delta, int hh) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const f32x4 d4 = *(const f32x4*)(stat + 64 + 8 * g + 4 * hh);
+        const f32x4 d4 = *(const f32x4*)(delta + 8 * g + 4 * hh);
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[4 * g + j] += d4[j];
     }
@@ -817,7 +818,7 @@ __device__ __forceinline__ void dkv_walk(const PackedArgs& a, const Tile& tl, in
         // qb: Q of this query block (dO a tile behind it), stat: its lse, rel: its index counted from the wave's diagonal, statn: of
         // the next block, qnn: Q of the block after that
         auto step = [&](const char* qb, const float* stat, int rel, const float* statn, const char* qnn, auto fence_c) {
-            if constexpr (!FROM_DELTA<D>) add_delta(dp, stat, hh);
+            if constexpr (!FROM_DELTA<D>) add_delta(dp, stat + 64, hh);
             if (rel <= 0) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
@@ -933,24 +934,31 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741;
 // d 128 32 / 54, 154 / 230, 2352 / 3854).
 // Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.1 TB/s.
-constexpr int SHORT_ROWS = 64;
-template <int D>
-constexpr int short_smem() {  // Q, dO, K; dS, its low parts; lse, delta (or what dq_walk needs)
-    return std::max(3 * PA_TILE * 2 * D + (SHORT_ROWS + 16) * 2 * SHORT_ROWS + 512, 5 * PA_TILE * 2 * D);
+// W 3: the same for up to 96 rows (the padded prompts of 77).
+template <int D, int W>
+constexpr int short_smem() {  // Q, dO, K; dS and its low parts (the third block of queries in planes of its own); lse, delta; or what dq_walk needs
+    return std::max(3 * 32 * W * 2 * D + (W - 1) * (64 + 16) * 128 + 256 * W, 5 * PA_TILE * 2 * D);
 }
-// dK and dV of 64 keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
-template <int D, bool WHOLE>
+// dK and dV of 32 W keys from row k0 of a sequence on; WHOLE: they are all of it, dQ too
+template <int D, int W, bool WHOLE>
 __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len, int k0, bool tail, int kvh, char* smem) {
-    constexpr int NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB, SROW = 2 * SHORT_ROWS;
+    constexpr int ROWS = 32 * W;
+    constexpr int NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = ROWS * ROWB, BLOCKB = 32 * ROWB, SROW = 128;
     char *qs = smem, *dos = smem + TILEB, *ks_ = smem + 2 * TILEB, *dss = smem + 3 * TILEB;
-    char* lows = dss + SHORT_ROWS * SROW;  // what the rounding of dS took away from keys 0 .. 15
-    float* stat = (float*)(lows + 16 * SROW);
+    char* lows = dss + (W - 1) * 64 * SROW;  // what the rounding of dS took away from keys 0 .. 15 and 64 .. 79
+    float* stat = (float*)(lows + (W - 1) * 16 * SROW);
+    // dS of key block kb and query block b < 2: rows 32 kb + key, half b; of query block 2: rows (kb == 2 ? 32 : 0) + key of the second plane,
+    // half kb & 1.  Low parts of kb 0, b < 2: rows key, half b; b 2: rows key of the second plane, half kb / 2.
+    auto ds_row = [](int kb, int b) { return b < 2 ? 32 * kb : 64 + (kb == 2 ? 32 : 0); };
+    auto ds_half = [](int kb, int b) { return b < 2 ? b : kb & 1; };
+    auto low_row = [](int b) { return b < 2 ? 0 : 16; };
+    auto low_half = [](int kb, int b) { return b < 2 ? b : kb >> 1; };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l31 = lane & 31, hh = lane >> 5, G = a.H / a.Hkv, own = wave * 32 + l31;
     const bool ok = k0 + own < len, busy = k0 + wave * 32 < len;
     const long long row = start + (ok ? k0 + own : 0);
     const long long ldqb = a.ldq * 2, lddob = a.lddo * 2, ldkb = a.ldk * 2;
-    TileDma<D, 2> qd, dd, kd;
+    TileDma<D, W, ROWS> qd, dd, kd;
     qd.init(wave, lane, ldqb);
     dd.init(wave, lane, lddob);
     kd.init(wave, lane, ldkb);
@@ -971,7 +979,7 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
         for (int e = 0; e < 16; ++e) { dk[d][e] = 0.f; dv[d][e] = 0.f; }
     int g = 0, q0 = k0;  // head of the group, first row of the tile of queries
     for (bool first = true; g < (tail ? 0 : G); first = false) {
-        const int h = kvh * G + g, left = min(len - q0, PA_TILE);
+        const int h = kvh * G + g, left = min(len - q0, ROWS);
         const bool qok = WHOLE ? ok : own < left;
         const long long qrow = WHOLE ? row : start + q0 + (qok ? own : 0);
         if (!first) __syncthreads();
@@ -1001,18 +1009,18 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
         dlt = half_sum(dlt);
         if (hh == 0) {  // (queries behind the end: zero, P = 1 meets only zeros)
             stat[own] = lse;
-            stat[64 + own] = -dlt;
+            stat[ROWS + own] = -dlt;
         }
         __syncthreads();
         if (busy) {
 #pragma nounroll
-            for (int b = WHOLE || q0 == k0 ? wave : 0; b < 2 && b * 32 < left; ++b) {
+            for (int b = WHOLE || q0 == k0 ? wave : 0; b < W && b * 32 < left; ++b) {
                 const float* st = stat + 32 * b;
                 const char *qb = qs + b * BLOCKB, *db = dos + b * BLOCKB;
                 f32x16 s, dp;
 #pragma unroll
                 for (int gq = 0; gq < 4; ++gq) {
-                    const f32x4 d4 = *(const f32x4*)(st + 64 + 8 * gq + 4 * hh);
+                    const f32x4 d4 = *(const f32x4*)(st + ROWS + 8 * gq + 4 * hh);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) { s[4 * gq + j] = 0.f; dp[4 * gq + j] = FROM_DELTA<D> ? d4[j] : 0.f; }
                 }
@@ -1021,7 +1029,7 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(qb + rread[ks]), kf[ks], s, 0, 0, 0);
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8*)(db + rread[ks]), vf[ks], dp, 0, 0, 0);
                 }
-                if constexpr (!FROM_DELTA<D>) add_delta(dp, st, hh);
+                if constexpr (!FROM_DELTA<D>) add_delta(dp, st + ROWS, hh);
                 if (b == wave && (WHOLE || q0 == k0)) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
@@ -1048,11 +1056,14 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                     const u32x4 low = rounded_off(ds, packed);
                     if (sI == 0) low0 = __builtin_bit_cast(bf16x8, low);
                     if constexpr (WHOLE) {  // queries 32 b + 16 sI + 8 gq + 4 hh .. + 3 of the lane's key
+                        char* to = dss + (ds_row(wave, b) + l31) * SROW;
+                        char* lo = lows + (low_row(b) + l31) * SROW;
 #pragma unroll
                         for (int gq = 0; gq < 2; ++gq) {
-                            const int c = (((4 * b + 2 * sI + gq) ^ swz<64>(own)) << 4) + 8 * hh;
-                            *(u32x2*)(dss + own * SROW + c) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
-                            if (own < 16) *(u32x2*)(lows + own * SROW + c) = u32x2{low[2 * gq], low[2 * gq + 1]};
+                            const int c = 2 * sI + gq, x = swz<64>(l31);
+                            *(u32x2*)(to + (((4 * ds_half(wave, b) + c) ^ x) << 4) + 8 * hh) = u32x2{packed[2 * gq], packed[2 * gq + 1]};
+                            if (!(wave & 1) && l31 < 16)
+                                *(u32x2*)(lo + (((4 * low_half(wave, b) + c) ^ x) << 4) + 8 * hh) = u32x2{low[2 * gq], low[2 * gq + 1]};
                         }
                     }
                 }
@@ -1064,7 +1075,7 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
                         dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_pair(y + tlo[d], y + thi[d]), pfr[sI], dv[d], 0, 0, 0);
                         const bf16x8 qt = tr_pair(x + tlo[d], x + thi[d]);
                         dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, dsf[sI], dk[d], 0, 0, 0);
-                        if (b == 0 && sI == 0) dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, low0, dk[d], 0, 0, 0);
+                        if (!(b & 1) && sI == 0) dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, low0, dk[d], 0, 0, 0);
                     }
             }
         }
@@ -1082,20 +1093,23 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
             for (int d = 0; d < ND; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
-            int qlo, qhi;
-            tr_lane<64>(lane, wave, qlo, qhi);
-            for (int b = 0; b <= wave; ++b)
+            for (int b = 0; b <= wave; ++b) {
+                int qlo, qhi, llo, lhi;
+                tr_lane<64>(lane, ds_half(b, wave), qlo, qhi);
+                tr_lane<64>(lane, low_half(b, wave), llo, lhi);
+                const char* lw = lows + low_row(wave) * SROW;
 #pragma unroll
                 for (int sI = 0; sI < 2; ++sI) {
-                    const char *x = dss + (2 * b + sI) * 16 * SROW, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
+                    const char *x = dss + (ds_row(b, wave) + 16 * sI) * SROW, *y = ks_ + b * BLOCKB + sI * 16 * ROWB;
                     const bf16x8 f = tr_pair(x + qlo, x + qhi);
 #pragma unroll
                     for (int d = 0; d < ND; ++d) {
                         const bf16x8 kt = tr_pair(y + tlo[d], y + thi[d]);
                         dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, f, dq[d], 0, 0, 0);
-                        if (b == 0 && sI == 0) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, tr_pair(lows + qlo, lows + qhi), dq[d], 0, 0, 0);
+                        if (!(b & 1) && sI == 0) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, tr_pair(lw + llo, lw + lhi), dq[d], 0, 0, 0);
                     }
                 }
+            }
             store_row<D>(a.dQ + row * a.lddq + h * D, nullptr, dq, a.scale, hh, ok);
         }
     }
@@ -1104,15 +1118,16 @@ __device__ __forceinline__ void key_tile(const PackedArgs& a, int start, int len
         store_row<D>(a.dV + row * a.lddv + kvh * D, nullptr, dv, 1.0f, hh, ok);
     }
 }
-template <int D>
-__global__ __launch_bounds__(128, D == 64 ? 2 : 1) void packed_bwd_short_kernel(const PackedArgs a) {
-    __shared__ __attribute__((aligned(1024))) char smem[short_smem<D>()];
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_short_kernel(const PackedArgs a) {
+    __shared__ __attribute__((aligned(1024))) char smem[short_smem<D, W>()];
     const int at = (int)blockIdx.x - a.rest;
     if (at >= 0) {
         const int i = at / a.Hkv, start = min(max(a.cu[i], 0), a.rows), len = min(max(a.cu[i + 1], start), a.rows) - start;
-        if (len > 0 && len <= a.skip) key_tile<D, true>(a, start, len, 0, false, at % a.Hkv, smem);
+        if (len > 0 && len <= a.skip) key_tile<D, W, true>(a, start, len, 0, false, at % a.Hkv, smem);
         return;
     }
+    if (threadIdx.x >= 128) return;  // (a tile of 64 rows: two waves; barriers wait for those that are left)
     const int u = blockIdx.x, groups = (a.H + a.Hkv + a.per - 1) / a.per, u0 = u % groups;
     Tile tl;
     if (!find_tile<PA_TILE>(a, u / groups, false, tl)) return;
@@ -1120,7 +1135,7 @@ __global__ __launch_bounds__(128, D == 64 ? 2 : 1) void packed_bwd_short_kernel(
         if (j > u0) __syncthreads();
         // (one unit a workgroup: the longest walks come first, dQ's of the last tile and dK's of the first; more: their lengths add up
         // to the same for every tile)
-        if (j < a.Hkv) key_tile<D, false>(a, tl.start, tl.len, (a.per == 1 ? tl.ntiles - 1 - tl.tile : tl.tile) * PA_TILE, tl.tail, j, smem);
+        if (j < a.Hkv) key_tile<D, 2, false>(a, tl.start, tl.len, (a.per == 1 ? tl.ntiles - 1 - tl.tile : tl.tile) * PA_TILE, tl.tail, j, smem);
         else dq_walk<D, 2>(a, tl, j - a.Hkv, smem);
     }
 }
@@ -1158,7 +1173,9 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
 
 // Whether most sequences fit 64 rows, as far as their mean says.
 bool mostly_short(int rows, int n_seq) { return rows <= 64ll * n_seq; }
-// Then the forward has two waves to a workgroup instead of four (d 64; d 128 gains nothing): twice as many workgroups are resident and
+// What the backward of a batch of prompts takes in one piece: sequences of up to 64 or 96 rows; 0: no such batch.
+int short_rows_of(int rows, int n_seq) { return mostly_short(rows, n_seq) ? 64 : rows <= 96ll * n_seq ? 96 : 0; }
+// With at most 64 rows the forward has two waves to a workgroup instead of four (d 64; d 128 gains nothing): twice as many workgroups are resident and
 // fewer waves idle (64 x 40 rows, 16 heads: 11.0 -> 8.4 us; from 77 rows on there is nothing in it).
 int waves_of(int rows, int n_seq, int d) { return d == 64 && mostly_short(rows, n_seq) ? 2 : 4; }
 
@@ -1266,19 +1283,22 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     a.delta = (float*)workspace;
     a.part = (float*)((char*)workspace + delta_bytes(rows, H));
     a.parts = parts_of(n_seq, rows, H, Hkv);
-    const bool prompts = mostly_short(rows, n_seq);
-    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, prompts ? PA_TILE : 128, a.zero_tail);
+    const int short_rows = short_rows_of(rows, n_seq);
+    const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, short_rows ? PA_TILE : 128, a.zero_tail);
     if (qtiles * H > MOST_GROUPS) return CCNET_EUNSUP;
     if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
-    if (prompts) {
-        a.skip = SHORT_ROWS;
+    if (short_rows) {
+        a.skip = short_rows;
         a.per = (int)((qtiles * (H + Hkv) + MOST_EMPTY - 1) / MOST_EMPTY);
         const long long rest = qtiles * ((H + Hkv + a.per - 1) / a.per), groups = (long long)n_seq * Hkv + rest;
         a.rest = (int)rest;
         if (groups > MOST_GROUPS) return CCNET_EUNSUP;
-        if (d == 128) hipLaunchKernelGGL(packed_bwd_short_kernel<128>, dim3((unsigned)groups), dim3(128), 0, st, a);
-        else hipLaunchKernelGGL(packed_bwd_short_kernel<64>, dim3((unsigned)groups), dim3(128), 0, st, a);
+        const dim3 gs((unsigned)groups);
+        if (d == 128 && short_rows == 96) hipLaunchKernelGGL((packed_bwd_short_kernel<128, 3>), gs, dim3(192), 0, st, a);
+        else if (d == 128) hipLaunchKernelGGL((packed_bwd_short_kernel<128, 2>), gs, dim3(128), 0, st, a);
+        else if (short_rows == 96) hipLaunchKernelGGL((packed_bwd_short_kernel<64, 3>), gs, dim3(192), 0, st, a);
+        else hipLaunchKernelGGL((packed_bwd_short_kernel<64, 2>), gs, dim3(128), 0, st, a);
         CCNET_LAUNCH_CHECK();
         return CCNET_OK;
     }

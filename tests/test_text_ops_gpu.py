@@ -287,7 +287,7 @@ def _run_attention(q, k, v, do, cu, H, Hkv, d, scale):
 
 
 LENS = [(1,), (2,), (31,), (32,), (33,), (77,), (63, 64, 65), (127, 128, 129), (0, 5, 0, 0, 77, 0), (256,), (257, 300), (511, 3, 640),
-        tuple(range(1, 78)), (1,) * 130]
+        tuple(range(1, 78)), (1,) * 130, (96, 95, 65), (97, 64, 33, 96, 80), (0, 90, 200, 66, 1, 77, 96, 96)]
 MANY = tuple((i * 37 + i // 5) % 71 for i in range(290)) + (0, 0, 301, 0, 130) + (3,) * 10  # (more sequences than are searched in order)
 
 

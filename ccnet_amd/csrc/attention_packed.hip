@@ -92,15 +92,16 @@ struct Tile { int start, len, tile, ntiles; bool tail; };
 // all of them); values are not negative
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true); }
-__device__ __forceinline__ int wave_isum(int v) {
+__device__ __forceinline__ int wave_scan(int v) {  // each lane: the sum up to itself
     v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
     v += dpp<0x112, 0xf>(v);
     v += dpp<0x114, 0xf>(v);
     v += dpp<0x118, 0xf>(v);
     v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
     v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return __builtin_amdgcn_readlane(v, 63);
+    return v;
 }
+__device__ __forceinline__ int wave_isum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
 __device__ __forceinline__ int wave_imax(int v) {
     v = max(v, dpp<0x111, 0xf>(v));
     v = max(v, dpp<0x112, 0xf>(v));
@@ -116,29 +117,34 @@ __device__ __forceinline__ int wave_imax(int v) {
 // f(L) = sum_i max(0, ntiles_i - L), falling in L, so a bisection finds the level and a ballot the sequence.  Sequence n_seq
 // stands for the rows behind the last one (when they are to be written).  Offsets are clamped to [0, rows] and to rising
 // order: wrong ones give wrong results but no access outside.  False: there is no such tile.
-// The sums take every workgroup through all offsets.  With more than FEW_SEQS sequences the tiles have places instead: sequence i
-// those from floor(cu[i] / step) + i on, at least as many as it has tiles (some stay empty), found by a search of 64 probes a
-// round.  A sequence's longest walks still come first, not the longest of all: 192 prompts of up to 77 rows, 8 heads, d 64: forward
-// 16.3 -> 12.7 us, backward 52.9 -> 44.7; with a sequence of 4096 rows behind them 59 -> 70 and 155 -> 178; 1024 prompts: 182 -> 53
-// and 513 -> 211.
+// The sums take every workgroup through all offsets, several times.  More than FEW_SEQS sequences are therefore taken in groups of 64:
+// the group that begins with sequence i has the places from floor(cu[i] / step) + i on, at least as many as it has tiles, and its
+// tiles fill the first of them in order of the sequences (the longest walk of each first, not of all).  The group is found by a search
+// of 64 probes a round.  PLACEHOLDER
 constexpr int FEW_SEQS = 127;
 template <int step>
 __device__ __forceinline__ bool find_place(const PackedArgs& a, int idx, bool from_end, Tile& t) {
     const int lane = threadIdx.x & 63;
-    auto at = [&](int i) { return min(max(a.cu[i], 0), a.rows); };
-    int lo = 0, hi = a.n_seq + 1;  // place(lo) <= idx < place(hi)
+    auto at = [&](int i) { return min(max(a.cu[min(i, a.n_seq)], 0), a.rows); };
+    int lo = 0, hi = a.n_seq / 64 + 1;  // group lo begins at or in front of idx, group hi behind it
     while (hi - lo > 1) {
-        const int n = hi - lo, p = lo + (int)((long long)n * (lane + 1) / 65);
+        const int n = hi - lo, p = (lo + (int)((long long)n * (lane + 1) / 65)) * 64;
         const int in = __popcll(__ballot(at(p) / step + p <= idx));
         hi = in == 64 ? hi : lo + (int)((long long)n * (in + 1) / 65);
         lo += (int)((long long)n * in / 65);
     }
-    t.start = __builtin_amdgcn_readfirstlane(at(lo));
-    t.len = __builtin_amdgcn_readfirstlane(lo < a.n_seq ? max(at(lo + 1), t.start) : a.zero_tail ? a.rows : t.start) - t.start;
-    t.ntiles = (t.len + step - 1) / step;
-    t.tail = lo == a.n_seq;
-    const int k = idx - (t.start / step + lo);
-    if (k < 0 || k >= t.ntiles || (t.len <= a.skip && !t.tail)) return false;
+    const int i = lo * 64 + lane, s = at(i), e = at(i + 1);
+    const int len = i > a.n_seq ? 0 : i == a.n_seq ? (a.zero_tail ? a.rows - s : 0) : e - s <= a.skip ? 0 : e - s;
+    const int nt = (len + step - 1) / step, upto = wave_scan(nt);
+    int k = idx - (__builtin_amdgcn_readlane(s, 0) / step + lo * 64);
+    const unsigned long long behind = __ballot(upto > k);
+    if (k < 0 || behind == 0) return false;
+    const int src = __ffsll(behind) - 1;
+    k -= __builtin_amdgcn_readlane(upto - nt, src);
+    t.start = __builtin_amdgcn_readlane(s, src);
+    t.len = __builtin_amdgcn_readlane(len, src);
+    t.ntiles = __builtin_amdgcn_readlane(nt, src);
+    t.tail = lo * 64 + src == a.n_seq;
     t.tile = from_end ? k : t.ntiles - 1 - k;
     return true;
 }

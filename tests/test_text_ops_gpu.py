@@ -312,6 +312,14 @@ def test_packed_attention_head_layouts(cuda, H, Hkv, d):
         assert (got[name][sum(lens):] == 0).all()
 
 
+@pytest.mark.parametrize("lens", [tuple(i * 7 % 9 for i in range(2600)) + (130, 0, 0), tuple(97 + i % 60 for i in range(1030)) + (0, 1, 300)],
+                         ids=["short", "longer"])
+def test_packed_attention_of_more_than_a_group_of_sequences(cuda, lens):
+    q, k, v, do, cu = _packed_inputs(lens, 1, 1, 64, seed=9, pad=5)
+    got = _run_attention(q, k, v, do, cu, 1, 1, 64, 0.125)
+    _check_attention(got, _attention_ref(q, k, v, do, lens, 1, 1, 64, 0.125), f"{len(lens)} sequences")
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("H,Hkv", [(64, 64), (63, 21)])
 def test_packed_attention_a_few_long_among_many_short(cuda, H, Hkv, d):

@@ -120,7 +120,9 @@ __device__ __forceinline__ int wave_imax(int v) {
 // The sums take every workgroup through all offsets, several times.  More than FEW_SEQS sequences are therefore taken in groups of 64:
 // the group that begins with sequence i has the places from floor(cu[i] / step) + i on, at least as many as it has tiles, and its
 // tiles fill the first of them in order of the sequences (the longest walk of each first, not of all).  The group is found by a search
-// of 64 probes a round.  PLACEHOLDER
+// of 64 probes a round.  Forward of prompts of up to 77 rows, 8 heads, d 64: 192 of them 16.3 us by the sums, 12.4 by groups, 1024 of
+// them 182 / 52; with a sequence of 4096 rows behind 192 of them 59 / 66.  (A place for every sequence instead of every group left
+// every second place empty where all have 64 rows, and with it every second CU: 1024 x 64 rows, 16 heads 319 / 189 us.)
 constexpr int FEW_SEQS = 127;
 template <int step>
 __device__ __forceinline__ bool find_place(const PackedArgs& a, int idx, bool from_end, Tile& t) {
@@ -1202,8 +1204,9 @@ int parts_of(int n_seq, int rows, int H, int Hkv) {
 size_t delta_bytes(int rows, int H) { return ((size_t)rows * H * 4 + 255) & ~(size_t)255; }
 
 // Workgroups for sequences that are longer than most, of which there may be none: so many at most, each with several heads if need
-// be (prompts of up to 77 rows, 16 heads, backward: 256 of them 54.7 us with 8192, 63.8 with 2048; 4096 of them 1103 / 1020)
-constexpr long long MOST_EMPTY = 4096;
+// be (prompts of up to 77 rows, 8 heads, backward: 512 of them 56 us with 4096, 61 with 8192, 71 with 16384; 1024 and one sequence of 4096
+// rows 667 / 470 / 316); fewer where the kernel has fewer workgroups a CU (64 x 77 rows, 16 heads 28.5 us with 2048, 32 with 8192)
+long long most_empty(int d, int short_rows) { return d == 64 && short_rows == 64 ? 8192 : 2048; }
 constexpr long long MOST_GROUPS = (1 << 24) - 1;  // (a launch has less than 2^32 threads)
 
 RowSpan span(const void* p, int ld, int width, int rows) { return {p, 2ll * ld, 2ll * width, rows}; }
@@ -1296,8 +1299,11 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     hipStream_t st = (hipStream_t)stream;
     if (short_rows) {
         a.skip = short_rows;
-        a.per = (int)((qtiles * (H + Hkv) + MOST_EMPTY - 1) / MOST_EMPTY);
-        const long long rest = qtiles * ((H + Hkv + a.per - 1) / a.per), groups = (long long)n_seq * Hkv + rest;
+        long long longer = qtiles;  // tiles of sequences of more rows than that, or the rows behind the last
+        if (n_seq <= FEW_SEQS) longer = std::min(longer, (long long)rows / PA_TILE + rows / (short_rows + 1) + 1);
+        const long long most = most_empty(d, short_rows);
+        a.per = (int)((longer * (H + Hkv) + most - 1) / most);
+        const long long rest = longer * ((H + Hkv + a.per - 1) / a.per), groups = (long long)n_seq * Hkv + rest;
         a.rest = (int)rest;
         if (groups > MOST_GROUPS) return CCNET_EUNSUP;
         const dim3 gs((unsigned)groups);

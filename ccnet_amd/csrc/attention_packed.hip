@@ -939,10 +939,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // Sequences that are longer, a few among many, have the launch's first workgroups, which end at once where there are none: a tile of
 // 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.  That is slower
 // than the kernels above where one sequence holds most of the rows (3000 and 63 of 9, 16 heads: 151 us against 127, with 4 key heads
-// 501 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 14.9 / 22.9; 256 of up to 77: 56 / 92; 4096: 1020 / 1741;
-// d 128 32 / 54, 154 / 230, 2352 / 3854).
-// Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.1 TB/s.
-// W 3: the same for up to 96 rows (the padded prompts of 77).
+// 495 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 15.3 / 22.9; 256 of up to 77: 61 / 92; 4096: 1035 / 1741;
+// d 128 29 / 54, 140 / 230, 2207 / 3854).
+// Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.0 TB/s.
+// W 3: the same for up to 96 rows, where they have more than 64 in the mean (64 x 77 rows, 16 heads 28.5 us against 43 by the kernels above,
+// 256 of them 112 / 170; with fewer rows the two waves are faster: 64 of up to 77 rows 18.9 / 23.7).
 template <int D, int W>
 constexpr int short_smem() {  // Q, dO, K; dS and its low parts (the third block of queries in planes of its own); lse, delta; or what dq_walk needs
     return std::max(3 * 32 * W * 2 * D + (W - 1) * (64 + 16) * 128 + 256 * W, 5 * PA_TILE * 2 * D);

@@ -474,11 +474,15 @@ def test_packed_attention_gradients_against_differences(cuda, d):
         assert abs(have - slope) <= near + 1e-5 * abs(slope), (name, have, slope, near)
 
 
-def test_packed_attention_repeats_bit_for_bit(cuda):
-    lens = (300, 7, 129, 64)
-    q, k, v, do, cu = _packed_inputs(lens, 8, 2, 64, seed=5)
-    a, b = (_run_attention(q, k, v, do, cu, 8, 2, 64, 0.1) for _ in range(2))
-    assert all(torch.equal(a[x], b[x]) for x in NAMES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [(300, 7, 129, 64), (40, 64, 3, 77, 33) * 60, (77, 96, 70) * 30, (900, 2000, 64)],
+                         ids=["mixed", "prompts", "padded", "long"])
+def test_packed_attention_repeats_bit_for_bit(cuda, lens, d):
+    q, k, v, do, cu = _packed_inputs(lens, 8, 2, d, seed=5)
+    a = _run_attention(q, k, v, do, cu, 8, 2, d, 0.1)
+    for _ in range(5):
+        b = _run_attention(q, k, v, do, cu, 8, 2, d, 0.1)
+        assert all(torch.equal(a[x], b[x]) for x in NAMES)
 
 
 def test_packed_attention_rows_past_two_gigabytes(cuda):

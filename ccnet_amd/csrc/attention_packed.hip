@@ -1225,9 +1225,11 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     if ((uintptr_t)o_low & 15) return CCNET_EINVAL;
     if (ldk > (1 << 24) || ldv > (1 << 24)) return CCNET_EUNSUP;
     const RowSpan q = span(Q, ldq, H * d, rows), k = span(K, ldk, Hkv * d, rows), v = span(V, ldv, Hkv * d, rows), o = span(O, ldo, H * d, rows),
-                  low = span(o_low, H * d, H * d, rows);
+                  low = span(o_low, H * d, H * d, rows), stat = span(lse, 2 * rows, 2 * rows, H);
     if (!spans_apart(o, k) || !spans_apart(o, v) || !(spans_apart(o, q) || (O == Q && ldo == ldq))) return CCNET_EINVAL;
     if (!spans_apart(low, q) || !spans_apart(low, k) || !spans_apart(low, v) || !spans_apart(low, o)) return CCNET_EINVAL;
+    for (const RowSpan& s : {q, k, v, o, low})
+        if (!spans_apart(stat, s)) return CCNET_EINVAL;
     PackedArgs a{};
     a.Q = (const __bf16*)Q; a.K = (const __bf16*)K; a.V = (const __bf16*)V; a.out = (__bf16*)O;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldo = ldo;

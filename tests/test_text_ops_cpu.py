@@ -211,3 +211,20 @@ def test_packed_attention_wrapper_refusals():
             ops._packed_operands(q, k, v, cu, 4, 4, 64)
     with pytest.raises(_err(), match="all of dq"):
         ops.attention_packed_bwd(b, b, b, b, b, ops.PackedStats(b, b), cu, 4, 4, 64, 1.0, dq=b)
+
+
+def _packed_fwd(lse=None, low=None, cu=0, n_seq=1 << 28):
+    """The forward over 100 rows of q, k, v = column slices of one matrix at 1 MiB (4 heads of 64 each), o at 4 MiB; addresses that are
+    never dereferenced, and so many sequences that the call ends at the size no launch can have."""
+    m = 1 << 20
+    p = lambda b: C.c_void_p((1 << 31) + b)  # noqa: E731
+    return _lib().ccnet_attention_packed_bf16(p(m), 768, p(m + 512), 768, p(m + 1024), 768, p(4 * m), 256, p(cu), n_seq, 100, 4, 4, 64, 1.0, 1,
+                                              None if lse is None else p(lse), None if low is None else p(low), None)
+
+
+def test_row_statistics_must_not_share_memory_with_operands_or_results():
+    m = 1 << 20  # (q, k, v: 153,600 bytes; o and o_low: 51,200; lse: 1,600)
+    for lse in (8 * m, m + 153600, m - 1600, 4 * m + 51200, 4 * m - 1600, 5 * m + 51200):
+        assert _packed_fwd(lse=lse, low=5 * m) == EUNSUP, lse
+    for lse in (m, m + 153596, m - 1596, m + 512, m + 1024, 4 * m, 4 * m + 51196, 4 * m - 4, 5 * m, 5 * m + 51196):
+        assert _packed_fwd(lse=lse, low=5 * m) == EINVAL, lse

@@ -1273,12 +1273,17 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
         !row_ok(dQ, lddq, H * d) || !row_ok(dK, lddk, Hkv * d) || !row_ok(dV, lddv, Hkv * d))
         return CCNET_EINVAL;
     if (ldq > (1 << 24) || ldk > (1 << 24) || ldv > (1 << 24) || lddo > (1 << 24)) return CCNET_EUNSUP;
-    if (workspace_bytes < ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d)) return CCNET_EWS;
+    const size_t need = ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d);
+    if (workspace_bytes < need) return CCNET_EWS;
     const RowSpan in[] = {span(Q, ldq, H * d, rows),         span(K, ldk, Hkv * d, rows),  span(V, ldv, Hkv * d, rows),
                           span(O, ldo, H * d, rows),         span(dO, lddo, H * d, rows),  span(o_low, H * d, H * d, rows),
                           span(lse, 2 * rows, 2 * rows, H)};
     const RowSpan out[] = {span(dQ, lddq, H * d, rows), span(dK, lddk, Hkv * d, rows), span(dV, lddv, Hkv * d, rows)};
+    const RowSpan ws{workspace, (long long)need, (long long)need, 1};
+    for (const RowSpan& s : in)
+        if (!spans_apart(ws, s)) return CCNET_EINVAL;
     for (int i = 0; i < 3; ++i) {
+        if (!spans_apart(ws, out[i])) return CCNET_EINVAL;
         for (const RowSpan& s : in)
             if (!spans_apart(out[i], s)) return CCNET_EINVAL;
         for (int j = 0; j < i; ++j)

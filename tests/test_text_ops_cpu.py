@@ -228,3 +228,22 @@ def test_row_statistics_must_not_share_memory_with_operands_or_results():
         assert _packed_fwd(lse=lse, low=5 * m) == EUNSUP, lse
     for lse in (m, m + 153596, m - 1596, m + 512, m + 1024, 4 * m, 4 * m + 51196, 4 * m - 4, 5 * m, 5 * m + 51196):
         assert _packed_fwd(lse=lse, low=5 * m) == EINVAL, lse
+
+
+def _packed_bwd(ws, dq=6, lse=None, n_seq=1 << 28, extra=0, cu=0, shift=0):
+    """The backward over 100 rows, 4 heads of 64: q, k, v slices of one matrix at 1 MiB, o at 2, o_low 3, do 4, lse 5, dq 6, dk 7, dv 8."""
+    m, l = 1 << 20, _lib()
+    p = lambda b: C.c_void_p((1 << 31) + b)  # noqa: E731
+    size = l.ccnet_attention_packed_bwd_workspace_bytes(n_seq, 100, 4, 4, 64)
+    return l.ccnet_attention_packed_bwd_bf16(p(m), 768, p(m + 512), 768, p(m + 1024), 768, p(2 * m), 256, p(3 * m), p(4 * m), 256, p(5 * m + shift), p(dq * m),
+                                             256, p(7 * m), 256, p(8 * m), 256, p(cu), n_seq, 100, 4, 4, 64, 1.0, 1, p(ws), size + extra, None)
+
+
+def test_backward_workspace_must_not_share_memory_with_operands_or_results():
+    m = 1 << 20  # (the workspace: 100 x 4 sums of 4 bytes, in whole 256)
+    assert _lib().ccnet_attention_packed_bwd_workspace_bytes(1 << 28, 100, 4, 4, 64) == 1792
+    for ws in (9 * m, 8 * m + 51200, m - 1792, 5 * m + 1600):
+        assert _packed_bwd(ws) == EUNSUP, ws
+    assert _packed_bwd(m - 1792, extra=1 << 20) == EUNSUP  # what is handed over beyond the need is not touched
+    for ws in (m, m + 512, m + 1024, m + 153584, m - 1776, 2 * m, 3 * m + 16, 4 * m, 5 * m, 5 * m + 1584, 6 * m, 7 * m + 51184, 8 * m - 16, 8 * m):
+        assert _packed_bwd(ws) == EINVAL, ws

@@ -1210,6 +1210,7 @@ size_t delta_bytes(int rows, int H) { return ((size_t)rows * H * 4 + 255) & ~(si
 long long most_empty(int d, int short_rows) { return d == 64 && short_rows == 64 ? 8192 : 2048; }
 constexpr long long MOST_GROUPS = (1 << 24) - 1;  // (a launch has less than 2^32 threads)
 
+RowSpan offsets(const int32_t* cu, int n_seq) { return {cu, 4 * (n_seq + 1ll), 4 * (n_seq + 1ll), 1}; }
 RowSpan span(const void* p, int ld, int width, int rows) { return {p, 2ll * ld, 2ll * width, rows}; }
 bool row_ok(const void* p, int ld, long long width) { return p && !((uintptr_t)p & 15) && !(ld & 7) && ld >= width; }
 
@@ -1243,6 +1244,8 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     const int waves = waves_of(rows, n_seq, d);
     const long long grid = most_tiles(rows, n_seq, wide ? 256 : 32 * waves, a.zero_tail) * H;
     if (grid > MOST_GROUPS) return CCNET_EUNSUP;
+    for (const RowSpan& s : {o, low, stat})
+        if (!spans_apart(offsets(cu_seqlens, n_seq), s)) return CCNET_EINVAL;
     if (grid == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     const dim3 g((unsigned)grid), b(64 * waves);
@@ -1303,6 +1306,8 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
     const int short_rows = short_rows_of(rows, n_seq);
     const long long tiles = most_tiles(rows, n_seq, 128, a.zero_tail), qtiles = most_tiles(rows, n_seq, short_rows ? PA_TILE : 128, a.zero_tail);
     if (qtiles * H > MOST_GROUPS) return CCNET_EUNSUP;
+    for (const RowSpan& s : {out[0], out[1], out[2], ws})
+        if (!spans_apart(offsets(cu_seqlens, n_seq), s)) return CCNET_EINVAL;
     if (tiles == 0 && qtiles == 0) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     if (short_rows) {

@@ -247,3 +247,11 @@ def test_backward_workspace_must_not_share_memory_with_operands_or_results():
     assert _packed_bwd(m - 1792, extra=1 << 20) == EUNSUP  # what is handed over beyond the need is not touched
     for ws in (m, m + 512, m + 1024, m + 153584, m - 1776, 2 * m, 3 * m + 16, 4 * m, 5 * m, 5 * m + 1584, 6 * m, 7 * m + 51184, 8 * m - 16, 8 * m):
         assert _packed_bwd(ws) == EINVAL, ws
+
+
+def test_offsets_must_not_share_memory_with_results():
+    m = 1 << 20  # (4 offsets: 16 bytes, which every workgroup reads while others write results)
+    for cu in (4 * m, 4 * m + 51196, 4 * m - 12, 5 * m, 5 * m + 51196, 8 * m, 8 * m + 1596):
+        assert _packed_fwd(lse=8 * m, low=5 * m, cu=cu, n_seq=3) == EINVAL, cu
+    for cu in (6 * m, 6 * m - 4, 7 * m, 8 * m + 51196, 9 * m, 9 * m + 1788):
+        assert _packed_bwd(9 * m, cu=cu, n_seq=3) == EINVAL, cu

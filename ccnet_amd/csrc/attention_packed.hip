@@ -1223,7 +1223,7 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     if ((d != 64 && d != 128) || rows > (1 << 29) || H > (1 << 20)) return CCNET_EUNSUP;
     if (rows == 0) return CCNET_OK;
     if (!cu_seqlens || !row_ok(Q, ldq, H * d) || !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d)) return CCNET_EINVAL;
-    if ((uintptr_t)o_low & 15) return CCNET_EINVAL;
+    if (((uintptr_t)o_low & 15) || ((uintptr_t)lse & 3) || ((uintptr_t)cu_seqlens & 3)) return CCNET_EINVAL;
     if (ldk > (1 << 24) || ldv > (1 << 24)) return CCNET_EUNSUP;
     const RowSpan q = span(Q, ldq, H * d, rows), k = span(K, ldk, Hkv * d, rows), v = span(V, ldv, Hkv * d, rows), o = span(O, ldo, H * d, rows),
                   low = span(o_low, H * d, H * d, rows), stat = span(lse, 2 * rows, 2 * rows, H);
@@ -1275,6 +1275,7 @@ extern "C" int ccnet_attention_packed_bwd_bf16(const void* Q, int ldq, const voi
         !row_ok(K, ldk, Hkv * d) || !row_ok(V, ldv, Hkv * d) || !row_ok(O, ldo, H * d) || !row_ok(dO, lddo, H * d) ||
         !row_ok(dQ, lddq, H * d) || !row_ok(dK, lddk, Hkv * d) || !row_ok(dV, lddv, Hkv * d))
         return CCNET_EINVAL;
+    if (((uintptr_t)lse & 3) || ((uintptr_t)cu_seqlens & 3)) return CCNET_EINVAL;
     if (ldq > (1 << 24) || ldk > (1 << 24) || ldv > (1 << 24) || lddo > (1 << 24)) return CCNET_EUNSUP;
     const size_t need = ccnet_attention_packed_bwd_workspace_bytes(n_seq, rows, H, Hkv, d);
     if (workspace_bytes < need) return CCNET_EWS;

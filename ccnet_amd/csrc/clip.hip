@@ -333,7 +333,7 @@ extern "C" int ccnet_grad_norm(const void* const* grads, const int64_t* numel, i
     if ((dtype != 0 && dtype != 1) || !norm || !list_ok(grads, numel, count, dtype == 0 ? 4 : 2)) return CCNET_EINVAL;
     const long long tiles = all_tiles(grads, numel, count, dtype);
     if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
-    if (!workspace || ((uintptr_t)workspace & 7)) return CCNET_EINVAL;
+    if (!workspace || ((uintptr_t)workspace & 7) || ((uintptr_t)norm & 3)) return CCNET_EINVAL;
     if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
     hipStream_t st = (hipStream_t)stream;
     double* ws = (double*)workspace;
@@ -354,7 +354,7 @@ extern "C" int ccnet_clip_grad_norm(const void* const* grads, void* const* out, 
     if (rc != CCNET_OK) return rc;
     const long long tiles = all_tiles(grads, numel, count, dtype);
     if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
-    if (!workspace || ((uintptr_t)workspace & 7)) return CCNET_EINVAL;
+    if (!workspace || ((uintptr_t)workspace & 7) || ((uintptr_t)norm & 3)) return CCNET_EINVAL;
     if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
     hipStream_t st = (hipStream_t)stream;
     double* ws = (double*)workspace;

@@ -255,3 +255,15 @@ def test_offsets_must_not_share_memory_with_results():
         assert _packed_fwd(lse=8 * m, low=5 * m, cu=cu, n_seq=3) == EINVAL, cu
     for cu in (6 * m, 6 * m - 4, 7 * m, 8 * m + 51196, 9 * m, 9 * m + 1788):
         assert _packed_bwd(9 * m, cu=cu, n_seq=3) == EINVAL, cu
+
+
+def test_row_statistics_offsets_and_norms_are_aligned():
+    m = 1 << 20
+    assert _packed_fwd(lse=8 * m + 4) == EUNSUP
+    for bad in (1, 2):
+        assert _packed_fwd(lse=8 * m + bad) == EINVAL and _packed_fwd(cu=16 * m + bad) == EINVAL
+        assert _packed_bwd(9 * m, shift=bad) == EINVAL and _packed_bwd(9 * m, cu=16 * m + bad) == EINVAL
+        l, g, n = _lib(), (C.c_void_p * 1)(1 << 20), (C.c_int64 * 1)(1000)
+        p = lambda b: C.c_void_p((1 << 31) + b)  # noqa: E731
+        assert l.ccnet_grad_norm(g, n, 1, 0, p(0), 16, p(64 + bad), None) == EINVAL
+        assert l.ccnet_clip_grad_norm(g, g, n, 1, 0, 1.0, p(0), 16, p(64 + bad), None) == EINVAL

@@ -609,6 +609,9 @@ extern "C" int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vo
     if (T > 0 && workspace_bytes < l.bytes) return CCNET_EWS;
     const RowSpan to{grad, (long long)ldg * 4, (long long)C * 4, vocab};
     if (!spans_apart(to, {dy, (long long)lddy * ds, (long long)C * ds, T}) || !spans_apart(to, {ids, id_bytes, id_bytes, T})) return CCNET_EINVAL;
+    const RowSpan used{workspace, (long long)l.bytes, (long long)l.bytes, T > 0};
+    if (!spans_apart(used, to) || !spans_apart(used, {dy, (long long)lddy * ds, (long long)C * ds, T}) || !spans_apart(used, {ids, id_bytes, id_bytes, T}))
+        return CCNET_EINVAL;
     if (T == 0 && accumulate) return CCNET_OK;
     hipStream_t st = (hipStream_t)stream;
     // the table's zeros in parts [0, vocab): part k of n with a launch that has `workers` workgroups of its own

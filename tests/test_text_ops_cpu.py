@@ -267,3 +267,15 @@ def test_row_statistics_offsets_and_norms_are_aligned():
         p = lambda b: C.c_void_p((1 << 31) + b)  # noqa: E731
         assert l.ccnet_grad_norm(g, n, 1, 0, p(0), 16, p(64 + bad), None) == EINVAL
         assert l.ccnet_clip_grad_norm(g, g, n, 1, 0, 1.0, p(0), 16, p(64 + bad), None) == EINVAL
+
+
+def test_table_gradient_workspace_must_not_share_memory_with_operands_or_results():
+    l, m = _lib(), 1 << 20
+    p = lambda b: C.c_void_p((1 << 31) + b)  # noqa: E731
+    need = l.ccnet_embedding_grad_workspace_bytes(100, 64)  # ids: 800 bytes at 1 MiB, dy: 25,600 at 2, the table: 2,560 at 3
+
+    def go(ws):
+        return l.ccnet_embedding_grad(p(m), 8, 100, 10, p(2 * m), 0, 64, 64, 1.0, -1, p(3 * m), 64, 0, p(ws), need, None)
+
+    for ws in (m, m + 784, m - need + 16, 2 * m, 2 * m + 25584, 2 * m - need + 16, 3 * m, 3 * m + 2544, 3 * m - 16):
+        assert go(ws) == EINVAL, ws

@@ -315,6 +315,19 @@ int aliases_ok(const void* const* in, void* const* out, const int64_t* numel, in
     return ok ? CCNET_OK : CCNET_EINVAL;
 }
 
+// Whether the norm and the workspace (its `bytes` in use) lie apart from each other and from every tensor of the lists.
+bool norm_apart(const void* const* in, void* const* out, const int64_t* numel, int count, int esz, const void* workspace, size_t bytes, const float* norm) {
+    auto range = [](const void* p, long long n) { return RowSpan{p, n, n, n > 0}; };
+    const RowSpan ws = range(workspace, (long long)bytes), to = range(norm, 4);
+    bool ok = spans_apart(ws, to);
+    for (int i = 0; i < count; ++i)
+        for (const void* p : {in[i], out ? (const void*)out[i] : in[i]}) {
+            const RowSpan t = range(p, numel[i] * esz);
+            ok &= spans_apart(ws, t) && spans_apart(to, t);
+        }
+    return ok;
+}
+
 long long all_tiles(const void* const* g, const int64_t* numel, int count, int dtype) {
     long long t = 0;
     for (int i = 0; i < count; ++i) t += dtype == 0 ? tiles_of<float>(g[i], numel[i]) : tiles_of<unsigned short>(g[i], numel[i]);
@@ -335,6 +348,7 @@ extern "C" int ccnet_grad_norm(const void* const* grads, const int64_t* numel, i
     if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
     if (!workspace || ((uintptr_t)workspace & 7) || ((uintptr_t)norm & 3)) return CCNET_EINVAL;
     if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
+    if (!norm_apart(grads, nullptr, numel, count, dtype == 0 ? 4 : 2, workspace, 8 * (size_t)(1 + tiles), norm)) return CCNET_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     double* ws = (double*)workspace;
     const int rc = dtype == 0 ? norm_launches<float>(grads, numel, count, tiles, ws, st) : norm_launches<unsigned short>(grads, numel, count, tiles, ws, st);
@@ -356,6 +370,7 @@ extern "C" int ccnet_clip_grad_norm(const void* const* grads, void* const* out, 
     if (tiles > 0x7fffffffLL) return CCNET_EUNSUP;
     if (!workspace || ((uintptr_t)workspace & 7) || ((uintptr_t)norm & 3)) return CCNET_EINVAL;
     if (workspace_bytes < 8 * (size_t)(1 + tiles)) return CCNET_EWS;
+    if (!norm_apart(grads, out, numel, count, esz, workspace, 8 * (size_t)(1 + tiles), norm)) return CCNET_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     double* ws = (double*)workspace;
     float* factor = (float*)workspace;  // the workspace's first 8 bytes

@@ -279,3 +279,19 @@ def test_table_gradient_workspace_must_not_share_memory_with_operands_or_results
 
     for ws in (m, m + 784, m - need + 16, 2 * m, 2 * m + 25584, 2 * m - need + 16, 3 * m, 3 * m + 2544, 3 * m - 16):
         assert go(ws) == EINVAL, ws
+
+
+def test_norm_and_its_workspace_must_not_share_memory_with_the_tensors():
+    l, m = _lib(), 1 << 20
+    at = lambda b: (1 << 31) + b  # noqa: E731
+    p = lambda b: C.c_void_p(at(b))  # noqa: E731
+    g, o, n = (C.c_void_p * 3)(at(m), None, at(2 * m)), (C.c_void_p * 3)(at(3 * m), None, at(4 * m)), (C.c_int64 * 3)(1000, 0, 70000)
+    need = l.ccnet_grad_norm_workspace_bytes(g, n, 3, 0)
+    assert need == 8 * (1 + 1 + 5)
+    far = 8 * m
+    for ws, norm in ((m, far), (m + 3992, far), (m - 8, far), (2 * m + 279992, far), (far, m), (far, m + 3996), (far, 2 * m + 279996), (far, far),
+                     (far, far + need - 4)):
+        assert l.ccnet_grad_norm(g, n, 3, 0, p(ws), need, p(norm), None) == EINVAL, (ws, norm)
+        assert l.ccnet_clip_grad_norm(g, o, n, 3, 0, 1.0, p(ws), need, p(norm), None) == EINVAL, (ws, norm)
+    for ws, norm in ((3 * m, far), (3 * m - 8, far), (4 * m + 279992, far), (far, 3 * m), (far, 4 * m + 279996)):
+        assert l.ccnet_clip_grad_norm(g, o, n, 3, 0, 1.0, p(ws), need, p(norm), None) == EINVAL, (ws, norm)

@@ -840,20 +840,16 @@ def train_step(controlnet, unet, scheduler, optimizer, e, noise, timesteps, cond
             if p.grad is not None:
                 with_grad.append(p)
     # one pass over the gradients for their norm (it is not finite where one of them is not: what GradScaler.unscale_ records as
-    # found_inf) and, clipping by norm, one that scales them (a norm that is not finite scales nothing); one read of the result
+    # found_inf) and, clipping by norm, one that scales them; one read of the result.  Zero times the loss is one gradient more: it adds
+    # nothing to the norm of a step whose loss is finite and makes any other not finite, and such a norm scales nothing
     grads = [p.grad for p in with_grad]
+    guarded = grads + [loss.detach().float().reshape(1) * 0]
     by_norm = clip_grad_norm_by is not None and clip_grad_norm_or_value == "norm"
-    if not grads:
-        total = loss.new_zeros(())
-    elif by_norm:
-        total = ops.clip_grad_norm(grads, clip_grad_norm_by)
-    else:
-        total = ops.grad_norm(grads)
-    finite = bool(torch.isfinite(torch.stack([loss.float().reshape(()), total.float()])).all())
+    total = ops.clip_grad_norm(guarded, clip_grad_norm_by) if by_norm else ops.grad_norm(guarded)
     norm = None
-    if not finite:
+    if not bool(torch.isfinite(total)):
         logging.getLogger(__name__).warning("train_step: non-finite loss or gradient (loss %s, gradient norm %s): optimizer step "
-                                            "skipped", float(loss), float(total))
+                                            "skipped", float(loss), float(ops.grad_norm(grads)) if grads else 0.0)
         return loss, norm
     if clip_grad_norm_by is not None:
         norm = total

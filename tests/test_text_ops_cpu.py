@@ -1,5 +1,6 @@
 """What the entry points for token lookup, packed attention and gradient clipping refuse, on the host: nothing here launches."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -295,3 +296,46 @@ def test_norm_and_its_workspace_must_not_share_memory_with_the_tensors():
         assert l.ccnet_clip_grad_norm(g, o, n, 3, 0, 1.0, p(ws), need, p(norm), None) == EINVAL, (ws, norm)
     for ws, norm in ((3 * m, far), (3 * m - 8, far), (4 * m + 279992, far), (far, 3 * m), (far, 4 * m + 279996)):
         assert l.ccnet_clip_grad_norm(g, o, n, 3, 0, 1.0, p(ws), need, p(norm), None) == EINVAL, (ws, norm)
+
+
+@pytest.mark.parametrize("mode,limit", [("norm", 0.5), ("value", 0.5), ("norm", None)])
+@pytest.mark.parametrize("bad", [None, float("inf"), float("nan")])
+def test_train_step_leaves_the_gradients_of_a_skipped_step_as_they_are(monkeypatch, mode, limit, bad):
+    """A loss that is not finite skips the step even where every gradient is finite (an overflowing square has a finite derivative): no
+    parameter moves and no gradient is clipped.  The clipping calls are replaced by what they document, on the CPU."""
+    from ccnet_amd import ops, training
+
+    def norm_of(grads):
+        return torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+
+    def clip(grads, max_norm):
+        n = norm_of(grads)
+        f = min(1.0, max_norm / (float(n) + 1e-6)) if torch.isfinite(n) else 1.0
+        for g in grads:
+            g *= f
+        return n
+
+    def clip_value(grads, lim):
+        for g in grads:
+            g.clamp_(-lim, lim)
+
+    for name, fn in (("grad_norm", norm_of), ("clip_grad_norm", clip), ("clip_grad_value", clip_value)):
+        monkeypatch.setattr(ops, name, fn)
+    net = torch.nn.Linear(3, 2)
+    net._invalidate = lambda: None
+    grads = {p: torch.arange(1, p.numel() + 1).float().reshape(p.shape) for p in net.parameters()}
+    want = math.sqrt(sum(float(g.square().sum()) for g in grads.values()))
+    before = {p: (p.detach().clone(), g.clone()) for p, g in grads.items()}
+    loss = torch.tensor(2.0 if bad is None else bad)
+    monkeypatch.setattr(training, "controlnet_loss_and_grads", lambda *a: (loss, grads))
+    opt = torch.optim.SGD(net.parameters(), lr=0.1)
+    got, norm = training.train_step(net, None, None, opt, *[None] * 5, clip_grad_norm_by=limit, clip_grad_norm_or_value=mode)
+    assert got is loss and (norm is None) == (bad is not None or limit is None)
+    if norm is not None:
+        assert norm.shape == () and abs(float(norm) - want) <= 1e-6 * want
+    for p, (value, grad) in before.items():
+        if bad is not None:
+            assert torch.equal(p, value) and torch.equal(p.grad, grad)
+        else:
+            scaled = grad if limit is None else grad * (limit / (want + 1e-6)) if mode == "norm" else grad.clamp(-limit, limit)
+            assert torch.allclose(p.grad, scaled) and torch.allclose(p, value - 0.1 * scaled)

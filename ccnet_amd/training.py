@@ -444,7 +444,7 @@ class Tape:
                          scale: float) -> Var:
         """Causal self-attention of every sequence cu_seqlens[i] .. cu_seqlens[i+1] of the rows; q = q.a.t[:, q_off : q_off + H d],
         k / v columns of kv.a.t (Hkv d each).  The gradients go straight into the column slices of gradient buffers that nothing
-        else has written yet, and are added where something has."""
+        else has written yet, and are added where something has or where the slices share columns."""
         views = (q.a.t[:, q_off:q_off + H * d], kv.a.t[:, k_off:k_off + Hkv * d], kv.a.t[:, v_off:v_off + Hkv * d])
         rg = q.rg or kv.rg
         o = ops.attention_packed(*views, cu_seqlens, H, Hkv, d, scale, with_lse=rg)
@@ -457,7 +457,8 @@ class Tape:
             if out.g is None:
                 return
             places = ((q, q_off, H * d), (kv, k_off, Hkv * d), (kv, v_off, Hkv * d))
-            if q.g is None and kv.g is None and q.rg and kv.rg:
+            apart = all(v is not w or c + n <= b or b + m <= c for i, (v, c, n) in enumerate(places) for w, b, m in places[:i])
+            if apart and q.g is None and kv.g is None and q.rg and kv.rg:
                 into = [v.grad_buf()[:, c:c + n] for v, c, n in places]
                 ops.attention_packed_bwd(*views, o, out.g, stats, cu_seqlens, H, Hkv, d, scale, *into)
             else:

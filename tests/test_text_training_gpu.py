@@ -208,3 +208,26 @@ def test_train_step_clips_as_torch_does(cuda, mode, limit):
         assert abs(float(norm) - want) <= 1e-5 * want  # (torch sums in fp32)
     for p, q in twin.items():
         assert ((p.grad - q.grad).abs() <= 2e-5 * q.grad.abs()).all()
+
+
+@pytest.mark.parametrize("q_off,k_off,v_off", [(0, 128, 128), (0, 0, 128), (64, 0, 128), (0, 0, 0)])
+def test_tape_adds_where_queries_keys_and_values_share_columns(cuda, q_off, k_off, v_off):
+    """Columns that serve twice (one projection for keys and values, for queries and keys, or slices that overlap) get the sum of what
+    each use gives alone."""
+    ops, tr = _mods()
+    H, Hkv, d, n = 2, 2, 64, 90
+    g = torch.Generator().manual_seed(6)
+    x0 = torch.randn(n, 256, generator=g).to(BF16).to(cuda)
+    do = torch.randn(n, H * d, generator=g).to(BF16).to(cuda)
+    cu = torch.tensor([0, 40, 90], dtype=torch.int32, device=cuda)
+    T = tr.Tape()
+    x = tr._v2d(x0, True)
+    T.attention_packed(x, q_off, x, k_off, v_off, cu, H, Hkv, d, 0.125).accumulate(do)
+    T.backward()
+    views = [x0[:, c:c + 128] for c in (q_off, k_off, v_off)]
+    o, stats = ops.attention_packed(*views, cu, H, Hkv, d, 0.125, with_lse=True)
+    want, mag = torch.zeros(n, 256, dtype=torch.float64, device=cuda), torch.zeros(n, 256, dtype=torch.float64, device=cuda)
+    for c, gr in zip((q_off, k_off, v_off), ops.attention_packed_bwd(*views, o, do, stats, cu, H, Hkv, d, 0.125)):
+        want[:, c:c + 128] += gr.double()
+        mag[:, c:c + 128] += gr.double().abs()
+    assert ((x.g.double() - want).abs() <= 2 * 2.0 ** -8 * (1 + 2.0 ** -8) * mag).all()  # two sums in bf16, each rounded

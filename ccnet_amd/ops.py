@@ -626,7 +626,7 @@ def _rows_ld(t: torch.Tensor, what: str, rows: int, width: int, dtypes) -> int:
     if step != 1 and width > 1:
         raise _l.CcnetError(f"{what}: rows must be contiguous (column stride {step})")
     if rows <= 1:  # the stride of a single row says nothing
-        ld = max(ld, (width + 7) // 8 * 8)
+        ld = (width + 7) // 8 * 8
     if ld > 0x7fffffff or rows > 0x7fffffff:
         raise _l.CcnetError(f"{what}: {rows} rows of stride {ld} pass the 32 bits of the C ABI")
     return ld

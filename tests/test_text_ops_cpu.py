@@ -339,3 +339,16 @@ def test_train_step_leaves_the_gradients_of_a_skipped_step_as_they_are(monkeypat
         else:
             scaled = grad if limit is None else grad * (limit / (want + 1e-6)) if mode == "norm" else grad.clamp(-limit, limit)
             assert torch.allclose(p.grad, scaled) and torch.allclose(p, value - 0.1 * scaled)
+
+
+def test_the_stride_of_a_single_row_says_nothing():
+    """One row of a matrix whose stride is no multiple of 16 bytes, or is below the row's width (a view of one row may say so), is as
+    good as a row by itself."""
+    from ccnet_amd import ops
+    wide = torch.zeros(3, 100, dtype=BF16)
+    assert wide[:1, :64].stride() == (100, 1)
+    for t in (wide[:1, :64], wide[1:2, 32:96], wide[0, :64].expand(1, 64), torch.zeros(64, dtype=BF16).as_strided((1, 64), (1, 1)), wide[:0, :64]):
+        assert ops._rows_ld(t, "q", t.shape[0], 64, (BF16,)) == 64
+    assert ops._rows_ld(wide[:1, :61], "q", 1, 61, (BF16,)) == 64  # (whole 16-byte vectors)
+    assert ops._rows_ld(wide[:2, :64], "q", 2, 64, (BF16,)) == 100
+    assert ops._rows_ld(torch.zeros(1, 64, dtype=BF16).as_strided((1, 64), (1 << 40, 1)), "q", 1, 64, (BF16,)) == 64

@@ -673,3 +673,16 @@ def test_text_ops_on_another_stream(cuda):
     torch.cuda.synchronize()
     for g in got:
         assert torch.equal(g[0], want[0]) and all(torch.equal(g[1][x], want[1][x]) for x in NAMES) and torch.equal(g[2], want[2])
+
+
+def test_a_single_row_of_any_stride(cuda):
+    ops = _ops()
+    wide = _randn(3, 300, seed=1, dtype=BF16)  # (600 bytes a row: no multiple of 16)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    q, k, v = (wide[:1, c:c + 64] for c in (0, 64, 128))
+    assert torch.equal(ops.attention_packed(q, k, v, cu, 1, 1, 64, 0.1), v)
+    ids = torch.tensor([0], device="cuda")
+    assert torch.equal(ops.embedding(ids, wide[:1, :64]), wide[:1, :64])
+    out = torch.zeros(2, 67, device="cuda")
+    ops.embedding_grad(ids, wide[:1, :64], 1, out=out[:1, :64])
+    assert torch.equal(out[0, :64], wide[0, :64].float()) and (out[0, 64:] == 0).all() and (out[1] == 0).all()

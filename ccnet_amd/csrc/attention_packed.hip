@@ -330,8 +330,10 @@ __device__ __forceinline__ void store_row(__bf16* row, __bf16* low_row, const f3
         }
 }
 
-// what the rounding of f to the bf16 of `hi` took away, rounded itself
+// what the rounding of f to the bf16 of `hi` took away, rounded itself.  (Where f is a product, the compiler would fuse it with the
+// difference in some of the kernels and not in others, whose results then differ in a last bit here and there.)
 __device__ __forceinline__ u32x4 rounded_off(const float (&f)[8], const u32x4& hi) {
+#pragma clang fp contract(off)
     float r[8];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {

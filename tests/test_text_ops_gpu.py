@@ -686,3 +686,17 @@ def test_a_single_row_of_any_stride(cuda):
     out = torch.zeros(2, 67, device="cuda")
     ops.embedding_grad(ids, wide[:1, :64], 1, out=out[:1, :64])
     assert torch.equal(out[0, :64], wide[0, :64].float()) and (out[0, 64:] == 0).all() and (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,pad", [((96, 90, 70), 40), ((65, 96, 33, 81, 96), 120), ((60, 64, 1, 33), 300)])
+def test_which_kernels_take_prompts_does_not_show(cuda, lens, pad, d):
+    """The backward of prompts in one piece and the general one, which takes them where rows behind the last sequence lift the mean
+    above 96: equal bits (no head group is cut at these lengths)."""
+    H, Hkv, n = 6, 2, sum(lens)
+    assert n <= 96 * len(lens) < n + pad < 512 * len(lens)
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=n + d, pad=pad)
+    a = _run_attention(q[:n], k[:n], v[:n], do[:n], cu, H, Hkv, d, 0.1)
+    b = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    for x in ("o", "dq", "dk", "dv"):
+        assert torch.equal(a[x], b[x][:n]), x

@@ -688,6 +688,42 @@ def test_a_single_row_of_any_stride(cuda):
     assert torch.equal(out[0, :64], wide[0, :64].float()) and (out[0, 64:] == 0).all() and (out[1] == 0).all()
 
 
+# ------------------------------------------------------------------ batches of prompts of 64 to 96 rows, and what pins the precision
+def _check_picks(got, q, k, v, do, lens, H, Hkv, d, scale, picks):
+    first = [0] + torch.tensor(lens).cumsum(0).tolist()
+    for i in picks:
+        r = slice(first[i], first[i + 1])
+        part = {n: (got[n][:, r] if n == "lse" else got[n][r]) for n in NAMES}
+        _check_attention(part, _attention_ref(q[r], k[r], v[r], do[r], lens[i:i + 1], H, Hkv, d, scale), f"sequence {i} of {lens[i]}")
+    assert all((got[x][first[-1]:] == 0).all() for x in ("o", "dq", "dk", "dv"))
+
+
+PROMPTS = tuple(60 + i * 13 % 41 for i in range(140)) + (97, 0, 300, 200, 1)  # 60 to 100 rows, and a few longer ones
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("H,Hkv", [(2, 1), (32, 32), (48, 16)])
+def test_packed_attention_of_many_prompts_of_up_to_96_rows(cuda, H, Hkv, d):
+    """More sequences than are searched in order, a mean of 64 to 96 rows, longer ones among them and rows behind the last; with many
+    heads a workgroup takes several heads of the longer ones."""
+    pad = 75
+    rows, n_seq = sum(PROMPTS) + pad, len(PROMPTS)
+    assert n_seq > 127 and 64 * n_seq < rows <= 96 * n_seq
+    q, k, v, do, cu = _packed_inputs(PROMPTS, H, Hkv, d, seed=H + d, pad=pad)
+    got = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    picks = range(n_seq) if H == 2 else [0, 3, 37, 63, 64, 127, 128, 139, 140, 142, 143, 144]
+    _check_picks(got, q, k, v, do, PROMPTS, H, Hkv, d, 0.1, picks)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_of_a_few_prompts_of_up_to_96_rows_with_many_heads(cuda, d):
+    lens = tuple(70 + i * 7 % 27 for i in range(50)) + (130, 97, 0, 260)
+    q, k, v, do, cu = _packed_inputs(lens, 64, 64, d, seed=d, pad=40)
+    assert 64 * len(lens) < sum(lens) + 40 <= 96 * len(lens)
+    got = _run_attention(q, k, v, do, cu, 64, 64, d, 0.1)
+    _check_picks(got, q, k, v, do, lens, 64, 64, d, 0.1, [0, 1, 26, 49, 50, 51, 53])
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("lens,pad", [((96, 90, 70), 40), ((65, 96, 33, 81, 96), 120), ((60, 64, 1, 33), 300)])
 def test_which_kernels_take_prompts_does_not_show(cuda, lens, pad, d):
@@ -700,3 +736,55 @@ def test_which_kernels_take_prompts_does_not_show(cuda, lens, pad, d):
     b = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
     for x in ("o", "dq", "dk", "dv"):
         assert torch.equal(a[x], b[x][:n]), x
+
+
+# every backward kernel: general, its walks cut into parts, prompts of up to 64 and 96 rows, longer sequences among prompts
+KERNELS = {"general": ((200, 130, 300, 64), 8, 4), "parts": ((700, 600), 8, 2), "64": ((64, 60, 33, 64) * 8, 8, 4), "96": ((96, 90, 77) * 8, 8, 4),
+           "among": ((40,) * 40 + (300, 200), 8, 4), "among96": ((80,) * 40 + (300, 200), 8, 4)}
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("which", KERNELS)
+def test_precision_of_the_row_sums_and_of_the_low_parts(cuda, which, d):
+    """What the rounding of o takes away (o_low) and what the rounding of dS takes away from the first 16 of every 64 keys (queries)
+    are carried, to 2^-8 of themselves.  Scores are zero here (q = 0 or k = 0), so that P has one value a row and its rounding
+    in the forward takes nothing away; only those 16 rows of k (q) are not zero, so that only their dS enters dq (dk).  What is left
+    beside the last rounding of a gradient: dS to 2^-17 and fp32 sums, together below 2^-14 of the result (its terms have independent
+    signs), so the error is that of rounding the exact gradient, to (1 + (2^-14 / 1.6e-3)^2)^(1/2) < 1.001.  Without the low parts it
+    would be 2^(1/2) of that; without o_low a query's dS would be off by 2^-9 of |o| |dO| altogether: above 1.05 in all of these.
+    1.02 leaves room for elements that lie next to the border between two roundings."""
+    lens, H, Hkv = KERNELS[which]
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, seed=d + len(lens))
+    at = torch.cat([torch.arange(n) for n in lens]).cuda()
+    few, zero = (at % 64 < 16)[:, None], torch.zeros_like
+    for name, (q1, k1) in {"dq": (zero(q), k * few), "dk": (q * few, zero(k))}.items():
+        got = _run_attention(q1, k1, v, do, cu, H, Hkv, d, 0.125)
+        ref = _attention_ref(q1, k1, v, do, lens, H, Hkv, d, 0.125)
+        x = ref[name][0]
+        one = (x.to(BF16).double() - x).norm()
+        ratio = float((got[name].double() - x).norm() / one)
+        print(f"{which} d {d} {name}: {ratio:.4f} times one rounding")
+        assert 0 < ratio <= 1.02, (name, ratio)
+        # o_low: half a step of itself, at most half a step of o (2^-8 each), the division 2^-21; sums of at + 1 values in fp32
+        _within(got["o"].double() + got["stats"].o_low.double(), ref["o"][0],
+                (2.0 ** -16 + 2.0 ** -21) * ref["o"][0].abs() + 2.0 ** -23 * (at + 1)[:, None] * float(v.abs().max()), "o + o_low")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_packed_attention_gradients_of_scores_of_hundreds(cuda, sign, d):
+    """Scores up to 1592 (2297 in base 2: fp32 knows them to 2^-13, inside the 2^-10 of the reference's bounds), rising or falling along the
+    keys by 8 a key."""
+    n = 200
+    q, k = (torch.zeros(n, d, dtype=BF16, device="cuda") for _ in range(2))
+    q[:, 0] = sign
+    k[:, 0] = (torch.arange(n, device="cuda") * 8.0).to(BF16)
+    v, do = _randn(n, d, seed=1, dtype=BF16), _randn(n, d, seed=2, dtype=BF16)
+    for pad in (0, 20):
+        cu = torch.tensor([0, n] if pad == 0 else [0, n] + [n] * 3, dtype=torch.int32, device="cuda")  # (general; among prompts)
+        got = _run_attention(q, k, v, do, cu, 1, 1, d, 1.0)
+        ref = _attention_ref(q, k, v, do, (n,), 1, 1, d, 1.0)
+        for x in ("o", "dq", "dk", "dv"):
+            # P and dS below 2^-126, out of the normal range of fp32 and bf16, may count as zero: each of the n < 2^8 terms of a sum is
+            # then off by at most 2^-126 times |dO|, |V| or |dP - delta| (below 2^8) and |q| or |k| (below 2^11)
+            _within(got[x], ref[x][0], ref[x][1] + 2.0 ** (8 + 8 + 11 - 126), f"{x} {pad}")

@@ -788,3 +788,27 @@ def test_packed_attention_gradients_of_scores_of_hundreds(cuda, sign, d):
             # P and dS below 2^-126, out of the normal range of fp32 and bf16, may count as zero: each of the n < 2^8 terms of a sum is
             # then off by at most 2^-126 times |dO|, |V| or |dP - delta| (below 2^8) and |q| or |k| (below 2^11)
             _within(got[x], ref[x][0], ref[x][1] + 2.0 ** (8 + 8 + 11 - 126), f"{x} {pad}")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,pad", [((300, 77, 40, 0, 200, 129), 50), ((64, 1, 33, 90, 77, 50), 9), ((700, 1200, 513), 0), ((40, 64, 3, 77, 33) * 30, 20)],
+                         ids=["mixed", "prompts", "parts", "many"])
+def test_bits_of_a_sequence_follow_from_its_rows_and_the_totals(cuda, lens, pad, d):
+    """The same sequences in another order, beside other values: equal totals (rows, sequences, heads), equal bits."""
+    H, Hkv = 8, 2
+    q, k, v, do, cu = _packed_inputs(lens, H, Hkv, d, pad=pad, seed=d)
+    a = _run_attention(q, k, v, do, cu, H, Hkv, d, 0.1)
+    first = cu.tolist()
+    order = torch.randperm(len(lens), generator=torch.Generator().manual_seed(1)).tolist()
+    keep = order[::2]  # these keep their values, the others get new ones
+    q2, k2, v2, do2, cu2 = _packed_inputs([lens[i] for i in order], H, Hkv, d, pad=pad, seed=d + 1)
+    at = cu2.tolist()
+    where = [(slice(first[i], first[i + 1]), slice(at[j], at[j + 1])) for j, i in enumerate(order) if i in keep]
+    for x, y in ((q, q2), (k, k2), (v, v2), (do, do2)):
+        for r, s in where:
+            y[s] = x[r]
+    b = _run_attention(q2, k2, v2, do2, cu2, H, Hkv, d, 0.1)
+    for r, s in where:
+        assert torch.equal(a["lse"][:, r], b["lse"][:, s])
+        for x in ("o", "dq", "dk", "dv"):
+            assert torch.equal(a[x][r], b[x][s]), x

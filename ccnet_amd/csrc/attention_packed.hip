@@ -359,9 +359,11 @@ __device__ __forceinline__ float half_sum(float v) {
 // pipe, which need about 512 cycles a step each at d = 128, run at once.  Half way through a tile's two steps lies the fence at
 // which the next tile has landed (its keys are needed by the second step) and the tile after it is sent for: K in a ring of
 // two, V, which is needed a step longer, in a ring of three.
-// Bound by both pipes' issue at d = 128 (4 sequences of 2811 to 8192 rows, 32 / 8 heads: 856 us = 1022 TFLOP/s, a square product of
-// 16384 reaches 1364), by the exponentials at d = 64 (5 of 1528 to 4096 rows, 16 / 4 heads: 107 us = 800 TFLOP/s, where every product
-// has half the work an exponential), by latency for prompts (77 rows, 16 heads: 5.8 us; 32 prompts 6.6 us).
+// Bound by both pipes' issue at d = 128 (4 sequences of 2811 to 8192 rows, 32 / 8 heads: 862 to 883 us = 990 to 1015 TFLOP/s, a square
+// product of 16384 reaches 1364; counters at 5 sequences of 1528 to 4096 rows: the matrix pipe busy 0.44 of the time, the vector pipe
+// 0.49), by vector issue at d = 64, where every product has half the work an exponential (those 5, 16 / 4 heads: 114 us = 750 TFLOP/s with
+// the statistics for the backward; vector pipe 0.67, matrix pipe 0.36, a CU without work 0.16), by latency for prompts (77 rows, 16 heads:
+// 5.9 us; 32 prompts 6.6 us; 4096 of up to 77 rows: 484 us, 578 with the statistics; matrix pipe 0.04, half of the waves' time waits).
 template <int D, int QB, int W>
 __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs a) {
     constexpr int BM = 32 * W * QB, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
@@ -574,7 +576,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_fwd_kernel(const PackedArgs 
 }
 
 // Where dP begins: at -delta, or at zero with -delta added to the product (the first spills in dQ at d 128); the same to the bit in all
-// of the backward's kernels, so that which of them takes a sequence does not show.
+// of the backward's kernels, so that which of them takes a sequence does not show.  (Into how many parts a key head's walk is cut does,
+// in the last bits of dK and dV: parts_of.)
 template <int D>
 constexpr bool FROM_DELTA = D == 64;
 __device__ __forceinline__ void add_delta(f32x16& dp, const float* delta, int hh) {
@@ -589,8 +592,9 @@ __device__ __forceinline__ void add_delta(f32x16& dp, const float* delta, int hh
 // ------------------------------------------------------------------ backward: dQ (and delta)
 // The forward's walk with 32 queries a wave: S^T = K Q^T and dP^T = V dO^T from row reads, a block ahead of dQ^T += K^T dS^T
 // from transposed reads, so here K is needed a step longer (ring of three).  delta is taken from the wave's own dO and O rows
-// and left for the dK / dV kernel.  Bound by matrix and vector issue side by side: 13.6k rows, 16 / 4 heads,
-// d 64: 151 us = 850 TFLOP/s of its three products (a twelfth more are for dS's low parts).
+// and left for the dK / dV kernel.  Bound by matrix and vector issue side by side: 13.6k rows, 16 / 4 heads, d 64: 149 to 154 us =
+// 830 to 860 TFLOP/s of its three products (a twelfth more are for dS's low parts); matrix pipe busy 0.45, vector pipe 0.52; at d 128
+// 279 to 286 us, 0.48 and 0.39.
 template <int D, int W>
 __device__ __forceinline__ void dq_walk(const PackedArgs& a, const Tile& tl, int h, char* smem) {
     constexpr int BM = 32 * W, NK = D / 16, ND = D / 32, ROWB = 2 * D, TILEB = PA_TILE * ROWB, BLOCKB = 32 * ROWB;
@@ -751,7 +755,9 @@ __global__ __launch_bounds__(64 * W, 2) void packed_bwd_dq_kernel(const PackedAr
 // group (or of its part of it) in turn, so the group's sum is taken in the accumulators, in a fixed order.  As above the scores
 // of the next query block are computed beside the exponentials of this one; Q and dO are both needed a step longer (rings of
 // three).  Query blocks in front of a wave's own keys (in the first two tiles of a head) are masked whole.
-// Bound like dQ, with one workgroup a CU less (256 registers, 50 KB): the same 13.6k rows 198 us = 860 TFLOP/s of its four products.
+// Bound like dQ, two workgroups a CU both: the same 13.6k rows 195 to 200 us = 850 to 875 TFLOP/s of its four products; matrix pipe busy
+// 0.47, vector pipe 0.41, LDS 0.33.  At d 128 (430 registers, 99,840 bytes) one workgroup a CU, so one wave a SIMD and nothing beside it
+// while it waits: 410 to 437 us, matrix pipe 0.39, vector pipe 0.29.
 template <int D>
 constexpr int dkv_stage() { return 2 * PA_TILE * 2 * D + 512; }  // Q, dO, lse and delta of 64 queries
 template <int D, int W>
@@ -942,8 +948,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? 2 : 1) void packed_bwd_dkv_kernel
 // 64 rows and a head for dQ by the walk above, or a key head for dK and dV in steps of one stage, delta taken anew.  That is slower
 // than the kernels above where one sequence holds most of the rows (3000 and 63 of 9, 16 heads: 151 us against 127, with 4 key heads
 // 495 / 251), faster where prompts are prompts (64 of up to 64 rows, 16 heads 15.3 / 22.9; 256 of up to 77: 61 / 92; 4096: 1035 / 1741;
-// d 128 29 / 54, 140 / 230, 2207 / 3854).
-// Bound by the latency of a workgroup's chain of loads and barriers; at 4096 prompts it moves 3.0 TB/s.
+// d 128 29 / 54, 140 / 230, 2207 / 3854).  What sends a batch here is its mean length, in which empty sequences count, and rows behind the
+// last one too: 16 sequences of 1000 rows and 300 empty ones take 325 us against 189 without the empty ones, with 4 key heads 408 / 187.
+// Bound by the latency of a workgroup's chain of loads and barriers: at 4096 prompts it moves 3.0 TB/s, the matrix pipe busy 0.06 and the
+// vector pipe 0.26 of the time, the waves waiting half of theirs; at d 128 one wave a SIMD (426 registers), 2.2 ms.
 // W 3: the same for up to 96 rows, where they have more than 64 in the mean (64 x 77 rows, 16 heads 28.5 us against 43 by the kernels above,
 // 256 of them 112 / 170; with fewer rows the two waves are faster: 64 of up to 77 rows 18.9 / 23.7).
 template <int D, int W>
@@ -1186,14 +1194,16 @@ long long most_tiles(int rows, int n_seq, int step, int tail) {
 bool mostly_short(int rows, int n_seq) { return rows <= 64ll * n_seq; }
 // What the backward of a batch of prompts takes in one piece: sequences of up to 64 or 96 rows; 0: no such batch.
 int short_rows_of(int rows, int n_seq) { return mostly_short(rows, n_seq) ? 64 : rows <= 96ll * n_seq ? 96 : 0; }
-// With at most 64 rows the forward has two waves to a workgroup instead of four (d 64; d 128 gains nothing): twice as many workgroups are resident and
-// fewer waves idle (64 x 40 rows, 16 heads: 11.0 -> 8.4 us; from 77 rows on there is nothing in it).
+// With at most 64 rows the forward has two waves to a workgroup instead of four (d 64; d 128 gains nothing): tiles of 64 rows, where most of
+// 128 would have no queries, and four workgroups a CU (as many as their LDS allows) instead of three (64 x 40 rows, 16 heads: 11.0 -> 8.4 us;
+// from 77 rows on there is nothing in it).  A wave does the same in both, so a sequence's bits do not show which it was.
 int waves_of(int rows, int n_seq, int d) { return d == 64 && mostly_short(rows, n_seq) ? 2 : 4; }
 
 // Into how many parts the walk of a key tile over its group's query heads is cut.  One workgroup walks G heads x the queries
 // behind its keys; with few key heads and long sequences the longest of those walks outlasts the rest of the grid.  Parts cost
 // fp32 sums through memory (16 bytes a channel), so only walks of at least 8 tiles a head on average are cut, and only while the
-// grid has fewer than 768 workgroups (three a CU).
+// grid has fewer than 768 workgroups (three a CU).  The order of a group's sum, and with it the last bits of dK and dV, follows from the
+// number of parts.
 int parts_of(int n_seq, int rows, int H, int Hkv) {
     const int G = H / Hkv;
     if (rows < 512ll * (n_seq > 0 ? n_seq : 1)) return 1;
@@ -1241,7 +1251,8 @@ extern "C" int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K
     a.o_low = (__bf16*)o_low;
     // 64 queries a wave (a K or V fragment feeds two products) where whole 256-query tiles are the rule and there are at least four of
     // them a CU: 64 x 1024 rows, 16 heads 231 us against 255, 4 x 8192 rows, 32 heads 1160 / 1236; with fewer the longest walks
-    // outlast the rest (2048 rows, 16 heads 47 / 31), with shorter sequences the last tiles are mostly empty (300 x 300 rows 381 / 371)
+    // outlast the rest (2048 rows, 16 heads 47 / 31), with shorter sequences the last tiles are mostly empty (300 x 300 rows 381 / 371).
+    // Both blocks' running maxima move together, so that P, and o and lse in their last bits, may round differently than in the narrow form.
     const bool wide = d == 64 && rows >= 512ll * n_seq && (long long)rows * H >= 256ll * 1024;
     const int waves = waves_of(rows, n_seq, d);
     const long long grid = most_tiles(rows, n_seq, wide ? 256 : 32 * waves, a.zero_tail) * H;

@@ -74,7 +74,7 @@ __device__ __forceinline__ float erf_fast(float x) {
 }
 __device__ __forceinline__ float gelu_erf_f(float g) { return 0.5f * g * (1.0f + erf_fast(g * 0.70710678118654752f)); }
 
-// a * gelu_erf(g) on two lanes of packed fp32 math (v_pk_fma_f32 / v_pk_mul_f32 run two fp32 ops per lane per issue).
+// a * gelu_erf(g), two elements at a time (the build emits no packed fp32 instructions: two scalar ones each).
 // erfc(|g| / sqrt 2) = exp2(|g| Q(|g|)) with Q a degree-5 fit (tools/fit_gelu.py: max abs error of gelu 3.1e-7 over
 // all fp32 g, at the fp32 evaluation floor), so gelu(g) = max(g, 0) - |g|/2 * exp2(|g| Q(|g|)): one exponential per
 // element, no reciprocal (the two quarter-rate instructions dominated the A&S 7.1.26 form in this epilogue).

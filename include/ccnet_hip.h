@@ -386,8 +386,9 @@ int ccnet_resample_bwd_bf16(const void* in, int ldi, void* out, int ldo, int N, 
  * Token lookup, causal attention over packed prompts and gradient clipping: the text side of training.  dtype codes of these
  * entry points: 0 = fp32, 1 = bf16.  Sums and statistics are fp32 or fp64, in an order that the inputs alone fix (no float
  * atomics), so equal inputs give equal bits.  Wrong ids or offsets in device memory give wrong rows, never an access outside.
- * Results that share memory with an operand or with one another are refused (CCNET_EINVAL) except where said; column slices of
- * rows of one stride share none. */
+ * Results (row statistics, norms and workspaces among them) that share memory with an operand, with ids or offsets, or with one another
+ * are refused (CCNET_EINVAL) except where said; column slices of rows of one stride share none.  So are addresses that are not
+ * aligned to their elements. */
 
 /* out[t][0..C) = scale * table[ids[t]][0..C), rounded once; an id outside [0, vocab) gives a row of zeros.  ids: id_bytes (4 or
  * 8) wide.  Any C and strides >= C (16-byte accesses where C % 8 == 0 and both matrices' rows are 16-byte aligned). */
@@ -409,7 +410,11 @@ int ccnet_embedding_grad(const void* ids, int id_bytes, int T, int vocab, const 
  *   o_low [rows][H d] (may be NULL) = what the rounding of out to bf16 took away, itself rounded to bf16
  * Rows behind the last sequence: left as they are, or with zero_tail != 0 written as zeros (lse: -inf).  A key or value that is
  * not finite reaches only the queries of its sequence that see it.  16-byte aligned rows (ld % 8 == 0); out may be q
- * itself.  Grids follow from rows and n_seq alone: a captured graph serves other lengths with the same totals. */
+ * itself.  Grids follow from rows, n_seq and the head counts: a captured graph serves other lengths with the same totals, and with the
+ * same totals a sequence's bits follow from its own rows, whatever stands beside it.  Other totals may change last bits (at d 64 of out
+ * and lse, whose tiles may be wider; of dK and dV, whose sums over a head group may be cut into other parts).  The totals also choose the
+ * kernels, by the mean length rows / n_seq: empty sequences and rows behind the last one count in it, so offsets padded with hundreds of
+ * empty sequences make a batch of long ones slower (the backward up to 2.2 times). */
 int ccnet_attention_packed_bf16(const void* Q, int ldq, const void* K, int ldk, const void* V, int ldv, void* O, int ldo,
                                 const int32_t* cu_seqlens, int n_seq, int rows, int H, int Hkv, int d, float scale, int zero_tail,
                                 float* lse, void* o_low, void* stream);
